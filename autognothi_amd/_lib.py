@@ -35,6 +35,7 @@ AG_MASK_VIT_MUL, AG_MASK_BERT_ADD = 0, 1
 AG_EPI_BIAS, AG_EPI_BIAS_GELU, AG_EPI_BIAS_RESID, AG_EPI_BIAS_F32, AG_EPI_BIAS_TANH, AG_EPI_BIAS_GELU_ADD = 0, 1, 2, 3, 4, 5
 AG_EX_STORE, AG_EX_GELU_DUAL, AG_EX_GELU_BWD, AG_EX_SLABS = 0, 1, 2, 3
 AG_MT_STATE_BYTES = 2560
+AG_LOGITS_MAX_V, AG_LOGITS_MAX_TOP = 524288, 128
 
 vp, i32, i64, u32, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_float, C.c_size_t
 
@@ -114,6 +115,10 @@ SIGNATURES = {
     "ag_shapley_normalize_rows_bwd": (i32, [vp, i32, i32, i32, vp, vp]),
     "ag_shapley_loss": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]),
     "ag_kl_loss": (i32, [vp, vp, i32, i32, vp, vp, vp]),
+    "ag_token_logprobs": (i32, [vp, i64, i32, i32, i32, f32, vp, i32, vp, vp, vp, vp, vp, vp, vp]),
+    "ag_token_logprobs_bwd": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, i64, vp]),
+    "ag_topk_distill": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp, i64, vp]),
+    "ag_topk_distill_bwd": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp, i64, vp]),
     "ag_transpose_f32": (i32, [vp, i32, i32, i64, vp, i64, vp]),
     "ag_transpose_f32_bf16": (i32, [vp, i32, i32, i64, vp, i64, vp]),
     "ag_cast_transpose_f32_bf16": (i32, [vp, i32, i32, i64, vp, vp, i64, vp]),

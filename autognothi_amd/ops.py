@@ -5,7 +5,7 @@ kernel of ``libautognothi_hip.so`` launched on ``torch.cuda.current_stream()``.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import ctypes as C
 
@@ -746,6 +746,169 @@ def kl_loss(ref: Tensor, cur: Tensor, want_grad: bool = True):
     with L.on(ref.device):
         L.check(L.lib().ag_kl_loss(L.ptr(ref), L.ptr(cur), ref.shape[0], ref.shape[1], L.ptr(loss), L.ptr(d), L.stream()))
     return loss, d
+
+
+# ----------------------------------------------------------------------------- wide rows of logits
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results for N rows; everything but the ids fp32.  ``stats`` is what the backward reads."""
+    logp: Optional[Tensor]        # [N] log-probability of the given token (None: no tokens given)
+    entropy: Tensor               # [N]
+    lse: Tensor                   # [N] ln sum exp(logits / temperature)
+    top_ids: Optional[Tensor]     # [N, top_k] int64, descending, ties by the lower index (None: top_k = 0)
+    top_logp: Optional[Tensor]    # [N, top_k]
+    stats: Tensor                 # [N, 2]
+    temperature: float
+
+
+class TopkDistill(NamedTuple):
+    loss: Tensor                  # [1] sum of weights * row_loss
+    row_loss: Tensor              # [N]
+    dlogits: Optional[Tensor]     # [N, V] in the logits' dtype: d loss / d logits (None: not asked for)
+    stats: Tensor                 # [N, 4], what topk_distill_bwd reads
+
+
+def _logit_rows(who: str, logits: Tensor) -> Tuple[Tensor, int, int, int, int]:
+    """-> (logits with unit column stride, rows, row length, row stride, storage dtype)"""
+    if logits.dim() != 2:
+        raise ValueError(f"{who}: logits must be [rows, vocabulary]; got {tuple(logits.shape)}")
+    if logits.dtype == torch.bfloat16:
+        dtype = BF16
+    elif logits.dtype == torch.float32:
+        dtype = F32
+    else:
+        raise TypeError(f"{who}: logits must be fp32 or bf16; got {logits.dtype}")
+    n, v = logits.shape
+    if not 1 <= v <= L.AG_LOGITS_MAX_V:
+        raise ValueError(f"{who}: rows of {v} logits (1 to {L.AG_LOGITS_MAX_V})")
+    if logits.stride(1) != 1 and v > 1:
+        logits = logits.contiguous()
+    return logits, n, v, logits.stride(0), dtype
+
+
+def _row_arg(who: str, name: str, t: Optional[Tensor], shape: Tuple[int, ...], dtype: torch.dtype, device) -> Optional[Tensor]:
+    """a small per-row argument: checked, contiguous"""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{who}: {name} must be {dtype}; got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{who}: {name} must be {list(shape)}; got {list(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{who}: {name} is on {t.device}, the logits are on {device}")
+    return t.contiguous()
+
+
+def _check_temperature(who: str, temperature: float) -> float:
+    t = float(temperature)
+    if not 0.0 < t < 3.0e38:
+        raise ValueError(f"{who}: temperature must be a positive number; got {temperature}")
+    return t
+
+
+def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """ln p of a given token in every row of ``logits`` [N, V] (fp32 / bf16, any row stride), the row's entropy and log-normaliser, and its
+    ``top_k`` (<= 128) likeliest alternatives, p = softmax(logits / temperature).  tokens [N] int64: negative = ignored (0), >= V = NaN."""
+    who = "token_logprobs"
+    logits, n, v, ld, dtype = _logit_rows(who, logits)
+    temperature = _check_temperature(who, temperature)
+    if not 0 <= top_k <= min(v, L.AG_LOGITS_MAX_TOP):
+        raise ValueError(f"{who}: top_k = {top_k} (0 to min({L.AG_LOGITS_MAX_TOP}, {v} logits))")
+    dev = logits.device
+    tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
+    L.require_gpu(logits)
+    logp = torch.empty(n, dtype=torch.float32, device=dev) if tokens is not None else None
+    entropy, lse = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    ids = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
+    top = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
+    with L.on(dev):
+        L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, L.ptr(logp), L.ptr(entropy),
+                                          L.ptr(lse), L.ptr(stats), L.ptr(ids), L.ptr(top), L.stream()))
+    return TokenLogprobs(logp, entropy, lse, ids, top, stats, temperature)
+
+
+def token_logprobs_bwd(logits: Tensor, fwd: TokenLogprobs, tokens: Optional[Tensor] = None, d_logp: Optional[Tensor] = None,
+                       d_entropy: Optional[Tensor] = None, d_lse: Optional[Tensor] = None, d_top_logp: Optional[Tensor] = None) -> Tensor:
+    """the gradient of sum(d_logp * logp + d_entropy * entropy + d_lse * lse + d_top_logp * top_logp) -> [N, V] in the logits' dtype;
+    ``fwd``, ``tokens``: of the forward call on the same logits."""
+    who = "token_logprobs_bwd"
+    logits, n, v, ld, dtype = _logit_rows(who, logits)
+    dev = logits.device
+    f32 = torch.float32
+    k = fwd.top_ids.shape[1] if fwd.top_ids is not None else 0
+    if d_logp is not None and tokens is None:
+        raise ValueError(f"{who}: d_logp without tokens")
+    if d_top_logp is not None and k == 0:
+        raise ValueError(f"{who}: d_top_logp without alternatives in the forward call")
+    tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
+    stats, entropy = _row_arg(who, "stats", fwd.stats, (n, 2), f32, dev), _row_arg(who, "entropy", fwd.entropy, (n,), f32, dev)
+    d_logp, d_entropy = _row_arg(who, "d_logp", d_logp, (n,), f32, dev), _row_arg(who, "d_entropy", d_entropy, (n,), f32, dev)
+    d_lse, d_top = _row_arg(who, "d_lse", d_lse, (n,), f32, dev), _row_arg(who, "d_top_logp", d_top_logp, (n, k), f32, dev)
+    ids = _row_arg(who, "top_ids", fwd.top_ids, (n, k), torch.int64, dev) if k else None
+    L.require_gpu(logits)
+    out = torch.empty((n, v), dtype=logits.dtype, device=dev)
+    with L.on(dev):
+        L.check(L.lib().ag_token_logprobs_bwd(L.ptr(logits), ld, n, v, dtype, fwd.temperature, L.ptr(stats), L.ptr(entropy), L.ptr(tokens),
+                                              L.ptr(d_logp), L.ptr(d_entropy), L.ptr(d_lse), k, L.ptr(ids), L.ptr(d_top), L.ptr(out), v,
+                                              L.stream()))
+    return out
+
+
+def _teacher_args(who: str, n: int, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor], dev):
+    if teacher_ids.dim() != 2 or not 1 <= teacher_ids.shape[1] <= L.AG_LOGITS_MAX_TOP:
+        raise ValueError(f"{who}: teacher_ids must be [rows, 1 to {L.AG_LOGITS_MAX_TOP}]; got {list(teacher_ids.shape)}")
+    if teacher_logp.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{who}: teacher_logp must be fp32 or bf16; got {teacher_logp.dtype}")
+    k = teacher_ids.shape[1]
+    ids = _row_arg(who, "teacher_ids", teacher_ids, (n, k), torch.int64, dev)
+    logp = _row_arg(who, "teacher_logp", teacher_logp, (n, k), teacher_logp.dtype, dev)
+    return ids, logp, (BF16 if logp.dtype == torch.bfloat16 else F32), k, _row_arg(who, "weights", weights, (n,), torch.float32, dev)
+
+
+def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor] = None, temperature: float = 1.0,
+                 tail: bool = False, want_grad: bool = True) -> TopkDistill:
+    """Distillation of a student's ``logits`` [N, V] (fp32 / bf16, any row stride) from a teacher's list of K <= 128 tokens per row:
+    ``teacher_ids`` [N, K] int64 (negative = empty slot) and ``teacher_logp`` [N, K] (fp32 / bf16), log-probabilities at ``temperature`` as
+    token_logprobs gives them.  Row loss: temperature^2 KL(teacher's list, renormalised || student), or with ``tail`` the list as it is and
+    the rest of the teacher's mass as one more class.  weights [N] fp32 (None: 1 / N); a row of weight 0 takes no part (its logits are not
+    read).  -> loss, row losses and (want_grad) the loss' gradient, rounded to the logits' dtype once."""
+    who = "topk_distill"
+    logits, n, v, ld, dtype = _logit_rows(who, logits)
+    temperature = _check_temperature(who, temperature)
+    dev = logits.device
+    if n == 0:
+        raise ValueError(f"{who}: no rows")
+    ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
+    L.require_gpu(logits)
+    row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.float32, device=dev)
+    stats = torch.empty((n, 4), dtype=torch.float32, device=dev)
+    out = torch.empty((n, v), dtype=logits.dtype, device=dev) if want_grad else None
+    with L.on(dev):
+        L.check(L.lib().ag_topk_distill(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w), 1 if tail else 0,
+                                        L.ptr(row), L.ptr(loss), L.ptr(stats), L.ptr(out), v, L.stream()))
+    return TopkDistill(loss, row, out, stats)
+
+
+def topk_distill_bwd(logits: Tensor, fwd: TopkDistill, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor] = None,
+                     temperature: float = 1.0, tail: bool = False, d_loss: Optional[Tensor] = None, d_row_loss: Optional[Tensor] = None) -> Tensor:
+    """the gradient apart from the loss: of d_loss [1] * loss + sum(d_row_loss [N] * row_loss) (both None: of the loss) -> [N, V] in the
+    logits' dtype; the other arguments as topk_distill had them."""
+    who = "topk_distill_bwd"
+    logits, n, v, ld, dtype = _logit_rows(who, logits)
+    temperature = _check_temperature(who, temperature)
+    dev = logits.device
+    if n == 0:
+        raise ValueError(f"{who}: no rows")
+    ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
+    stats = _row_arg(who, "stats", fwd.stats, (n, 4), torch.float32, dev)
+    d_loss = _row_arg(who, "d_loss", d_loss, (1,), torch.float32, dev)
+    d_row = _row_arg(who, "d_row_loss", d_row_loss, (n,), torch.float32, dev)
+    L.require_gpu(logits)
+    out = torch.empty((n, v), dtype=logits.dtype, device=dev)
+    with L.on(dev):
+        L.check(L.lib().ag_topk_distill_bwd(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w),
+                                            1 if tail else 0, L.ptr(stats), L.ptr(d_loss), L.ptr(d_row), L.ptr(out), v, L.stream()))
+    return out
 
 
 def seq_compact_plan(mask_bits: Tensor, t: int, sync: bool = True):

@@ -501,6 +501,45 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
                                  void* d_dqkv, int R, int T, int H, int heads, int mask_mode, float p_drop, uint32_t seed, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Wide rows of logits (csrc/logits.hip): log-probabilities of given tokens, and distillation from a teacher's top log-probabilities.
+ * No counterpart in the reference, whose distillation (models/shapley.py:96-106, scripts/train_surrogate.py:133-147) compares the full
+ * probability vectors of a handful of classes: these are the same quantities for a vocabulary, where the teacher is recorded as a list.
+ * d_logits [N, V] in `dtype`, row stride ld elements (any alignment; 0 = one row for all), 1 <= V <= AG_LOGITS_MAX_V; x = z / temperature,
+ * p = softmax(x), every sum in fp32.  A logit of -inf has probability 0; a row of nothing but -inf has no distribution (below); a NaN or
+ * +inf makes its row's results NaN.  Nothing is read back to the host; all calls can be captured.  Outputs must not alias inputs.
+ * ---------------------------------------------------------------------------------------------- */
+#define AG_LOGITS_MAX_V 524288
+#define AG_LOGITS_MAX_TOP 128
+/* d_lse [N] = ln sum exp x;  d_entropy [N] = -sum p ln p;  d_logp [N] = ln p of d_tokens[n] (NULL: not asked for; a token < 0 is ignored: 0;
+ * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
+ * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0. */
+int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
+                      float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp, void* stream);
+/* dlogits [N, V] (dtype, row stride ldd >= V) = the gradient of sum(d_g_logp . logp + d_g_entropy . entropy + d_g_lse . lse + d_g_top_logp . top_logp)
+ * (each NULL: zero).  d_stats, d_entropy and d_top_ids of the forward call on the same logits.  An ignored token and a row of -inf get zero. */
+int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const float* d_stats,
+                          const float* d_entropy, const int64_t* d_tokens, const float* d_g_logp, const float* d_g_entropy,
+                          const float* d_g_lse, int top_k, const int64_t* d_top_ids, const float* d_g_top_logp, void* d_dlogits, int64_t ldd,
+                          void* stream);
+/* d_teacher_ids / d_teacher_logp [N, K] (dense; teacher_dtype AG_F32 / AG_BF16): a teacher's tokens and log-probabilities at the same
+ * temperature (ag_token_logprobs records them).  An id < 0 is an empty slot; an id >= V makes the row NaN; a token listed twice has both
+ * masses.  tail == 0: the list's masses are renormalised (so a constant per row cancels: logits / temperature serve as well), and
+ *     L_n = temperature^2 sum_j q_j (ln q_j - ln p_id_j);                     an empty list: L = 0
+ * tail != 0: the masses are taken as they are and rest = max(0, 1 - sum q_j) is a class of its own against p_off, the student's mass off the
+ * list:  L_n = temperature^2 [ sum_j q_j (ln q_j - ln p_id_j) + rest (ln rest - ln p_off) ]   (rest = 0 if the list names every token).
+ * d_loss [1] = sum_n w_n L_n with w = d_weights [N] (NULL: 1 / N); a row of weight 0 takes no part: its logits are not read, L_n and its
+ * gradient are 0.  d_dlogits (optional): d loss / d logits in `dtype`.  d_stats [N, 4]: what ag_topk_distill_bwd reads.  A student row of
+ * -inf: L = +inf where the teacher has mass, gradient 0. */
+int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
+                    const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, float* d_row_loss, float* d_loss,
+                    float* d_stats, void* d_dlogits, int64_t ldd, void* stream);
+/* the gradient apart from the loss: d (d_g_loss[0] * loss + sum_n d_g_row_loss[n] L_n) / d logits (each NULL: no such term; both NULL:
+ * d_g_loss = 1), rows of weight 0 zero.  The other arguments as the forward call had them. */
+int ag_topk_distill_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
+                        const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, const float* d_stats,
+                        const float* d_g_loss, const float* d_g_row_loss, void* d_dlogits, int64_t ldd, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * In-library kernel timing (used by bench.py for the roofline block): when enabled, every launch of
  * an instrumented kernel class is bracketed by hipEvents on the launch stream.  ag_profile_collect
  * synchronises those events, returns the totals of one class since the last collect and clears it.

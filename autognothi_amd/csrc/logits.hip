@@ -3,314 +3,973 @@
 //
 // With x = z / temperature, m a reference of the row and s = sum_i exp(x_i - m):
 //     log p_i = (x_i - m) - ln s,   lse = m + ln s,   H = ln s - (1/s) sum_i exp(x_i - m) (x_i - m).
-// Everything below is one pass (or few) over the row with (m, s, ...) in fp32; one workgroup per row, no atomics in sums: results are
+// One pass over the row computes all of it: every lane keeps its own (m, s, t) and moves its reference only when a logit passes it by more
+// than LG_SLACK, the lanes are joined once at the end.  A row belongs to a TEAM of 16 or 64 lanes (rows of a few to 2048 logits) or to a
+// workgroup of 256, 512 or 1024 threads, and is read in 16-byte pieces ("chunks") from the 16-byte boundary at or below its start, so that
+// every whole chunk is one aligned load whatever the row stride is.  Sums are fp32 in a fixed order, no atomics: results are
 // bit-reproducible.
 #include "common.h"
 
 namespace {
 
-constexpr int LG_THREADS = 256;
-constexpr int LG_WAVES = LG_THREADS / 64;
 constexpr float LG_NEG = -3.402823466e38f;   // the reference of a row (or part of one) that holds nothing above -inf
+// how far (in powers of two) a logit may lie above its lane's reference before the reference moves: 3 keeps |y| <= 3 where the exponentials
+// are large, i.e. the rounding of y adds at most 2^-23 ln 2 to a term, and after a few chunks a row no longer moves any reference
+constexpr float LG_SLACK = 3.0f;
+constexpr float LG_LN2 = 0.69314718055994530942f;
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = red[0];
+template <typename T> struct Chunk;   // E logits of 16 bytes
+template <> struct Chunk<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[4]) {
+        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+};
+template <> struct Chunk<bf16_t> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int w = 1; w < LG_WAVES; ++w) r += red[w];
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+        return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    }
+};
+
+// a row as chunks: chunk c holds the logits [c E - sh, c E - sh + E) of [0, V)
+template <typename T>
+struct Row {
+    static constexpr int E = Chunk<T>::E;
+    const T* z;
+    int V, sh, n;   // logits, those of the first chunk that lie before the row, chunks
+    __device__ __forceinline__ Row(const T* p, int v) : z(p), V(v) {
+        sh = (int)(((uintptr_t)p & 15) / sizeof(T));
+        n = (v + sh + E - 1) / E;
+    }
+    // chunks 1 .. n - 2 lie inside the row
+    __device__ __forceinline__ uint4 inner(int c) const { return *reinterpret_cast<const uint4*>(z + (c * E - sh)); }
+    // any chunk; one that reaches over an end of the row is read element by element (nothing outside the row is touched), -inf outside
+    __device__ __forceinline__ uint4 load(int c) const {
+        const int lo = c * E - sh;
+        if (lo >= 0 && lo + E <= V) return *reinterpret_cast<const uint4*>(z + lo);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = lo + e >= 0 && lo + e < V ? Store<T>::load(z + lo + e) : -INFINITY;
+        return Chunk<T>::pack(x);
+    }
+    // the chunk's place in another row of the same length (16-byte stores at the logits' alignment: the hardware takes any)
+    __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const {
+        typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t any_uint4;
+        const int lo = c * E - sh;
+        const uint4 r = Chunk<T>::pack(x);
+        if (lo >= 0 && lo + E <= V) {
+            const any_uint4 v = {r.x, r.y, r.z, r.w};
+            *reinterpret_cast<any_uint4*>(d + lo) = v;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (lo + e >= 0 && lo + e < V) Store<T>::store(d + lo + e, x[e]);
+    }
+};
+
+// ---- joining lanes: the value of every lane of a team of W <= 64 lanes, the same bits on all of them ---------------------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int W, typename F> __device__ __forceinline__ float lanes_join(float v, F f) {
+    static_assert(W == 4 || W == 8 || W == 16 || W == 64, "team of lanes");
+    v = f(v, dpp<0xB1>(v));                   // quad_perm 1 0 3 2
+    v = f(v, dpp<0x4E>(v));                   // quad_perm 2 3 0 1
+    if (W >= 8) v = f(v, dpp<0x141>(v));      // row_half_mirror (a quad already agrees)
+    if (W >= 16) v = f(v, dpp<0x140>(v));     // row_mirror
+    if (W == 64) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    }
+    return v;
+}
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+
+// TH threads that own a row; red: TH / 64 floats of LDS per use (three planes for Acc), only for TH > 64
+template <int TH>
+struct Team {
+    static constexpr int LANES = TH < 64 ? TH : 64, WAVES = TH / 64;
+    static __device__ __forceinline__ int rank() { return TH >= 64 && TH < 256 ? threadIdx.x & 63 : threadIdx.x & (TH - 1); }
+    static __device__ __forceinline__ void sync() {
+        if (TH > 64) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the LDS and the loads / stores of one wave keep their order
+    }
+    template <typename F> static __device__ __forceinline__ float join(float v, F f, float* red) {
+        v = lanes_join<LANES>(v, f);
+        if (TH <= 64) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return lanes_join<(WAVES > 1 ? WAVES : 4)>(red[threadIdx.x & (WAVES - 1)], f);
+    }
+    static __device__ __forceinline__ float sum(float v, float* red) { return join(v, Add(), red); }
+    static __device__ __forceinline__ float max(float v, float* red) { return join(v, Max(), red); }
+};
+
+struct Acc { float m, s, t; };   // reference (a logit), sum of exp2(y), sum of exp2(y) y,  y = (z - m) c,  c = log2(e) / temperature
+
+// the same sums with respect to the reference `to` >= m (or equal); an empty one stays empty, a NaN a NaN
+__device__ __forceinline__ Acc rebase(const Acc& a, float to, float c) {
+    const float dm = (a.m - to) * c, f = __builtin_amdgcn_exp2f(dm);
+    Acc r;
+    r.m = to;
+    r.s = a.m == to ? a.s : a.s * f;
+    r.t = a.m == to ? a.t : f == 0.f ? a.s * f : f * fmaf(a.s, dm, a.t);
     return r;
 }
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = red[0];
-#pragma unroll
-    for (int w = 1; w < LG_WAVES; ++w) r = fmaxf(r, red[w]);
+template <int W> __device__ __forceinline__ Acc lanes_join(const Acc& a, float c) {
+    Acc r = rebase(a, lanes_join<W>(a.m, Max()), c);
+    r.s = lanes_join<W>(r.s, Add());
+    r.t = lanes_join<W>(r.t, Add());
     return r;
 }
-__device__ __forceinline__ unsigned long long block_max_u64(unsigned long long v, unsigned long long* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long u = __shfl_xor(v, o, 64);
-        v = u > v ? u : v;
+template <int TH> __device__ __forceinline__ Acc team_join(Acc a, float c, float* red) {
+    constexpr int WAVES = TH / 64;
+    a = lanes_join<Team<TH>::LANES>(a, c);
+    if (TH <= 64) return a;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        float* p = red + 3 * (threadIdx.x >> 6);
+        p[0] = a.m; p[1] = a.s; p[2] = a.t;
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    unsigned long long r = red[0];
-#pragma unroll
-    for (int w = 1; w < LG_WAVES; ++w) r = red[w] > r ? red[w] : r;
-    return r;
+    const float* p = red + 3 * (threadIdx.x & (WAVES - 1));
+    const Acc b = {p[0], p[1], p[2]};
+    return lanes_join<(WAVES > 1 ? WAVES : 4)>(b, c);
 }
 
-// a total order on the logits of a row: by value (-0 = +0, NaN above everything, as torch.topk orders them), ties by the lower index
+// y = z c - m c in one instruction: the product m c is rounded, so every y of the reference is off by the same `delta`, which is known exactly
+// (and taken out of the sums at the end); past 2^20 delta is no longer small and y is computed as (z - m) c.
+struct Ref {
+    float m, nr, delta;
+    bool far;
+    __device__ __forceinline__ Ref(float m_, float c) : m(m_) {
+        nr = -(m * c);
+        far = !(fabsf(nr) < 1048576.f);
+        delta = far ? 0.f : fmaf(m, c, nr);
+    }
+    __device__ __forceinline__ float y(float x, float c) const { return far ? (x - m) * c : fmaf(x, c, nr); }   // (z - m) c + delta
+};
+
+// One lane's running sums.  A chunk costs about 8.5 instruction slots per logit (an exp2 is four of them): unpack, max (two logits an
+// instruction), y, exp2, + and the entropy's fma.
+template <typename T, bool ENTROPY>
+struct Sums {
+    static constexpr int E = Chunk<T>::E;
+    float c, slack, s = 0.f, t = 0.f;
+    float lim = LG_NEG;   // what a logit must pass to move the reference
+    float zero;           // 0, or NaN where the reference is `far`: every chunk then takes the guarded form below
+    Ref ref;
+    __device__ __forceinline__ Sums(float c_) : c(c_), slack(LG_SLACK / c_), ref(LG_NEG, c_) { zero = NAN; }
+    // (s, t) without the reference's delta
+    __device__ __forceinline__ Acc acc() const {
+        const float f = __builtin_amdgcn_exp2f(-ref.delta);
+        return {ref.m, f * s, f * fmaf(-ref.delta, s, t)};
+    }
+    // x: the chunk's logits (-inf: none), cmax: the largest of them
+    __device__ __forceinline__ void add(const float (&x)[E], float cmax) {
+        if (cmax > lim) {
+            const Acc a = rebase(acc(), cmax, c);
+            ref = Ref(cmax, c);
+            lim = cmax + slack;
+            zero = ref.far ? NAN : 0.f;
+            const float f = __builtin_amdgcn_exp2f(ref.delta);
+            s = f * a.s;
+            t = f * fmaf(ref.delta, a.s, a.t);
+        }
+        float cs = zero, ct = zero;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float y = fmaf(x[e], c, ref.nr), p = __builtin_amdgcn_exp2f(y);
+            cs += p;
+            if (ENTROPY) ct = fmaf(p, y, ct);
+        }
+        // 0 * -inf (a masked logit), or a far reference: the same sums, every step guarded
+        const float bad = ENTROPY ? ct : cs;
+        if (bad != bad) {
+            cs = 0.f; ct = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float y = ref.y(x[e], c), p = x[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y);
+                cs += p;
+                ct += p == 0.f ? 0.f : p * y;
+            }
+        }
+        s += cs;
+        t += ct;
+    }
+};
+// exp2((z - m) c) as the sums above have it, at any magnitude
+__device__ __forceinline__ float exp2_from(float z, float m, float c) {
+    return z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((z - m) * c);
+}
+
+template <int E> __device__ __forceinline__ float max_of(const float (&x)[E]) {
+    float m = fmaxf(fmaxf(x[0], x[1]), x[2]);
+#pragma unroll
+    for (int e = 3; e + 1 < E; e += 2) m = fmaxf(fmaxf(m, x[e]), x[e + 1]);
+    return fmaxf(m, x[E - 1]);
+}
+
+// a total order on the logits of a row: by value (-0 = +0, NaN above everything), ties by the lower index
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {   // (at least -inf)
+    k = k < 0x007FFFFFu ? 0x007FFFFFu : k;
+    return k == 0xFFFFFFFFu ? NAN : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 __device__ __forceinline__ unsigned long long order_key(float x, int i) {
     return ((unsigned long long)order_key(x) << 32) | (0xFFFFFFFFu - (uint32_t)i);
 }
 
-struct RowSums { float m, s, t; };   // reference (in logits), sum of exp, sum of exp * (x - m)
+// ---- token_logprobs -------------------------------------------------------------------------------------------------------------
+// Top alternatives of a row that a workgroup owns.  Every lane remembers the largest logit of each of its SLOTS (the chunks it reads, in
+// rounds of LG_SLOTS).  Each wave finds the j-th largest of its lanes' maxima, j = ceil(k / waves); the least of them over the waves is a
+// bound that at least k logits reach, and few others: the chunks of the slots that reach it (about two per alternative asked for) are read
+// again, their logits at or above the bound are the candidates, and every candidate's place is the number of candidates that beat it.
+// Rows with more candidates than fit (many equal logits) or a NaN take a radix selection over the whole row.
+constexpr int LG_SLOTS = 16, LG_CAND = 1024;
 
-// d = z - m is exact enough at any magnitude (both near the type's lowest value included); a NaN or +inf in the row makes s NaN
-template <typename T, bool SKIP>
-__device__ RowSums row_sums(const T* __restrict__ z, int V, float inv_t, const uint32_t* skip, float* red) {
-    float m = LG_NEG;
-    for (int i = threadIdx.x; i < V; i += LG_THREADS)
-        if (!SKIP || !((skip[i >> 5] >> (i & 31)) & 1u)) m = fmaxf(m, Store<T>::load(z + i));
-    m = block_max(m, red);
-    float s = 0.f, t = 0.f;
-    for (int i = threadIdx.x; i < V; i += LG_THREADS) {
-        if (SKIP && ((skip[i >> 5] >> (i & 31)) & 1u)) continue;
-        const float x = Store<T>::load(z + i);
-        const float d = (x - m) * inv_t;
-        const float e = x == -INFINITY ? 0.f : expf(d);
-        s += e;
-        t += e == 0.f ? 0.f : e * d;
+struct TopLds {
+    unsigned long long cand[LG_CAND];
+    int list[LG_CAND];      // chunks to read again; the radix selection's counters
+    int place[LG_CAND];
+    uint32_t bound[16];
+    int n_list, n_cand;
+};
+
+// count(keys of the wave >= result) >= j, from the top bit down; stops when it is j
+template <int LOW> __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int j) {
+    uint32_t r = 0;
+    for (int b = 31; b >= LOW; --b) {
+        const uint32_t t = r | (1u << b);
+        const int n = __popcll(__ballot(key >= t));
+        if (n < j) continue;
+        r = t;
+        if (n == j) break;
     }
-    RowSums r;
-    r.m = m;
-    r.s = block_sum(s, red);
-    r.t = block_sum(t, red);
     return r;
 }
 
+// exact: the k-th largest key by radix (four digits of 8 bits over the row), then every larger logit and the first of the equal ones
+template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k, TopLds& lds) {
+    const int tid = threadIdx.x;
+    uint32_t prefix = 0;
+    int left = k;                       // how many of the logits with the digits found so far are still wanted
+    for (int d = 24; d >= 0; d -= 8) {
+        for (int i = tid; i < 256; i += TH) lds.list[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < row.V; i += TH) {
+            const uint32_t key = order_key(Store<T>::load(row.z + i));
+            if (d != 24 && (key >> (d + 8)) != prefix) continue;
+            const int digit = (key >> d) & 255;
+            const unsigned long long on = __ballot(1);
+            const int one = __builtin_amdgcn_readfirstlane(digit);
+            if (__all(digit == one)) {                       // (rows of equal logits: one addition for the wave)
+                if ((tid & 63) == __ffsll(on) - 1) atomicAdd(&lds.list[one], __popcll(on));
+            } else {
+                atomicAdd(&lds.list[digit], 1);
+            }
+        }
+        __syncthreads();
+        int digit = 255, above = 0;
+        for (; digit > 0; --digit) {                         // (every thread, the same broadcast reads)
+            const int n = lds.list[digit];
+            if (above + n >= left) break;
+            above += n;
+        }
+        left -= above;
+        prefix = d == 24 ? (uint32_t)digit : (prefix << 8) | digit;
+        __syncthreads();
+    }
+    // prefix is the k-th largest key; `left` of the logits equal to it belong to the top, the first ones
+    if (tid == 0) { lds.n_cand = 0; lds.n_list = 0; }
+    __syncthreads();
+    for (int i0 = 0; i0 < row.V; i0 += TH) {
+        const int i = i0 + tid;
+        const uint32_t key = i < row.V ? order_key(Store<T>::load(row.z + i)) : 0u;
+        if (i < row.V && key > prefix) lds.cand[atomicAdd(&lds.n_cand, 1)] = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (uint32_t)i);
+        const bool eq = i < row.V && key == prefix;
+        const unsigned long long m = __ballot(eq);
+        const int before = lds.n_list;                       // equal logits of the rounds so far
+        if (before >= left) continue;                        // (uniform: all of them are found, only larger ones are still wanted)
+        __syncthreads();
+        if ((tid & 63) == 0) lds.place[tid >> 6] = __popcll(m);
+        __syncthreads();
+        int at = before;
+        for (int w = 0; w < (tid >> 6); ++w) at += lds.place[w];
+        int total = before;
+        for (int w = 0; w < TH / 64; ++w) total += lds.place[w];
+        at += __popcll(m & ((1ull << (tid & 63)) - 1ull));
+        if (eq && at < left) lds.cand[atomicAdd(&lds.n_cand, 1)] = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (uint32_t)i);
+        __syncthreads();
+        if (tid == 0) lds.n_list = total;
+        __syncthreads();
+    }
+    __syncthreads();
+}
+
+// candidates [0, n) of LDS (at least k, all different) -> their places; the first k are written
+template <int TH> __device__ __forceinline__ void write_top(TopLds& lds, int n, int k, const Acc& a, float inv_t, float log_s, bool empty,
+                                                            int64_t* __restrict__ ids, float* __restrict__ logp) {
+    const int tid = threadIdx.x;
+    // P threads share a candidate, each compares it with a part of the others
+    int cap = 64;
+    while (cap < n) cap <<= 1;
+    const int P = cap < TH ? TH / cap : 1, q0 = tid & (cap - 1), part = cap < TH ? tid / cap : 0;
+    if (P > 1) {
+        for (int i = tid; i < n; i += TH) lds.place[i] = 0;
+        __syncthreads();
+    }
+    for (int q = cap < TH ? q0 : tid; q < n; q += cap < TH ? cap : TH) {
+        const unsigned long long me = lds.cand[q];
+        int r = 0;
+        const int lo = (int)((int64_t)n * part / P), hi = (int)((int64_t)n * (part + 1) / P);
+        for (int j = lo; j < hi; ++j) r += lds.cand[j] > me;
+        if (P > 1) atomicAdd(&lds.place[q], r);
+        else lds.place[q] = r;
+    }
+    __syncthreads();
+    for (int q = tid; q < n; q += TH) {
+        const int r = lds.place[q];
+        if (r >= k) continue;
+        const unsigned long long me = lds.cand[q];
+        const float x = key_value((uint32_t)(me >> 32));
+        ids[r] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
+        logp[r] = empty ? -INFINITY : (x - a.m) * inv_t - log_s;
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(LG_THREADS) void token_logprobs_kernel(const T* __restrict__ z, int64_t ld, int V, float inv_t,
-                                                                    const int64_t* __restrict__ tokens, int top_k, float* __restrict__ logp,
-                                                                    float* __restrict__ entropy, float* __restrict__ lse,
-                                                                    float* __restrict__ stats, int64_t* __restrict__ top_ids,
-                                                                    float* __restrict__ top_logp) {
-    __shared__ float red[LG_WAVES];
-    __shared__ unsigned long long red64[LG_WAVES];
-    const int64_t row = blockIdx.x;
-    const T* zr = z + row * ld;
-    const RowSums r = row_sums<T, false>(zr, V, inv_t, nullptr, red);
-    const bool empty = r.s == 0.f;
-    const float log_s = empty ? -INFINITY : logf(r.s);
-    if (threadIdx.x == 0) {
-        stats[row * 2] = r.m;
-        stats[row * 2 + 1] = r.s;
-        lse[row] = empty ? -INFINITY : r.m * inv_t + log_s;
-        entropy[row] = empty ? 0.f : log_s - r.t / r.s;
-        if (tokens) {
-            const int64_t t = tokens[row];
-            float v = 0.f;
-            if (t >= V) v = NAN;
-            else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(zr + t) - r.m) * inv_t - log_s;
-            logp[row] = v;
+__device__ __forceinline__ void write_row(const Row<T>& row, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
+                                          float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats) {
+    stats[r * 2] = a.m;
+    stats[r * 2 + 1] = a.s;
+    lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
+    entropy[r] = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
+    if (tokens) {
+        const int64_t t = tokens[r];
+        float v = 0.f;
+        if (t >= row.V) v = NAN;
+        else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(row.z + t) - a.m) * inv_t - log_s;
+        logp[r] = v;
+    }
+}
+
+template <typename T, int TH, bool TOP>
+__global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
+                                                         int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
+                                                         float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+    constexpr int E = Chunk<T>::E, U = 4;   // U chunks of a lane are in flight
+    __shared__ float red[3 * (TH / 64)];
+    const int64_t r = blockIdx.x;
+    const Row<T> row(z + r * ld, V);
+    const int tid = threadIdx.x;
+    Sums<T, true> sums(c);
+    float slot[LG_SLOTS], ends = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < LG_SLOTS; ++i) slot[i] = -INFINITY;
+    // the first and the last chunk (threads 0 and 1) reach over the row's ends; their loads are the first in flight
+    const int last = row.n - 1;
+    const bool has_end = tid == 0 || (tid == 1 && last > 0);
+    uint4 end_v = make_uint4(0, 0, 0, 0);
+    if (has_end) end_v = row.load(tid ? last : 0);
+    for (int c0 = 1; c0 < last; c0 += LG_SLOTS * TH) {
+#pragma unroll
+        for (int i = 0; i < LG_SLOTS; i += U) {
+            if (c0 + i * TH >= last) break;
+            uint4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int ch = c0 + (i + u) * TH + tid;
+                if (ch < last) v[u] = row.inner(ch);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int ch = c0 + (i + u) * TH + tid;
+                if (ch < last) {
+                    float x[E];
+                    Chunk<T>::unpack(v[u], x);
+                    const float cmax = max_of(x);
+                    if (TOP) slot[i + u] = fmaxf(slot[i + u], cmax);
+                    sums.add(x, cmax);
+                }
+            }
         }
     }
-    unsigned long long below = ~0ull;   // (no element has this key: its index would be beyond every row)
-    for (int k = 0; k < top_k; ++k) {
-        unsigned long long best = 0;
-        for (int i = threadIdx.x; i < V; i += LG_THREADS) {
-            const unsigned long long key = order_key(Store<T>::load(zr + i), i);
-            if (key < below && key > best) best = key;
+    if (has_end) {
+        float x[E];
+        Chunk<T>::unpack(end_v, x);
+        ends = max_of(x);
+        sums.add(x, ends);
+    }
+    const Acc a = team_join<TH>(sums.acc(), c, red);
+    const bool empty = a.s == 0.f;
+    const float log_s = empty ? -INFINITY : logf(a.s);
+    if (tid == 0) write_row(row, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (!TOP) return;
+    __shared__ TopLds lds;
+    if (tid == 0) { lds.n_list = 0; lds.n_cand = 0; }
+    float mine = ends;
+#pragma unroll
+    for (int i = 0; i < LG_SLOTS; ++i) mine = fmaxf(mine, slot[i]);
+    const uint32_t kth = wave_kth<(E == 8 ? 16 : 0)>(order_key(mine), (k + TH / 64 - 1) / (TH / 64));
+    if ((tid & 63) == 0) lds.bound[tid >> 6] = kth;
+    __syncthreads();
+    uint32_t least = lds.bound[0];
+#pragma unroll
+    for (int w = 1; w < TH / 64; ++w) least = min(least, lds.bound[w]);
+    const float bound = key_value(least);
+    bool whole = a.s != a.s;   // a NaN or +inf in the row
+    if (!whole) {
+        const auto again = [&](int ch) {
+            const int at = atomicAdd(&lds.n_list, 1);
+            if (at < LG_CAND) lds.list[at] = ch;
+        };
+        if (has_end && ends >= bound) again(tid ? last : 0);
+#pragma unroll
+        for (int i = 0; i < LG_SLOTS; ++i)
+            if (slot[i] >= bound)
+                for (int ch = 1 + i * TH + tid; ch < last; ch += LG_SLOTS * TH) again(ch);
+        __syncthreads();
+        const int n_list = lds.n_list;
+        whole = n_list > LG_CAND;
+        if (!whole) {
+            for (int q = tid; q < n_list; q += TH) {
+                const int ch = lds.list[q], lo = ch * E - row.sh;
+                float x[E];
+                Chunk<T>::unpack(row.load(ch), x);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (x[e] >= bound && lo + e >= 0 && lo + e < V) {
+                        const int at = atomicAdd(&lds.n_cand, 1);
+                        if (at < LG_CAND) lds.cand[at] = order_key(x[e], lo + e);
+                    }
+            }
+            __syncthreads();
+            whole = lds.n_cand > LG_CAND;
         }
-        below = block_max_u64(best, red64);
-        if (threadIdx.x == 0) {
-            const int i = (int)(0xFFFFFFFFu - (uint32_t)below);
-            top_ids[row * top_k + k] = i;
-            top_logp[row * top_k + k] = empty ? -INFINITY : (Store<T>::load(zr + i) - r.m) * inv_t - log_s;
+        __syncthreads();
+    }
+    if (whole) top_radix<T, TH>(row, k, lds);
+    write_top<TH>(lds, lds.n_cand, k, a, inv_t, log_s, empty, top_ids + r * k, top_logp + r * k);
+}
+
+// Rows of up to 64 (W = 16 lanes a row) or 2041 / 2045 logits (W = 64): the whole row lives in registers, the maximum is found first.
+template <typename T, int W> struct Small;
+template <typename T> struct Small<T, 16> {   // element j of a lane: lane + 16 j
+    static constexpr int NE = 4, G = 1;
+    static __host__ __device__ constexpr int max_v() { return 16 * NE; }
+    const T* z;
+    int V, lane;
+    __device__ __forceinline__ Small(const T* p, int v, int l) : z(p), V(v), lane(l) {}
+    __device__ __forceinline__ int index(int j) const { return lane + 16 * j; }
+    __device__ __forceinline__ int groups() const { return NE; }
+    __device__ __forceinline__ void load(float (&x)[NE]) const {
+#pragma unroll
+        for (int j = 0; j < NE; ++j) x[j] = index(j) < V ? Store<T>::load(z + index(j)) : -INFINITY;
+    }
+};
+template <typename T> struct Small<T, 64> {   // chunks of a lane: lane + 64 i
+    static constexpr int E = Chunk<T>::E, NE = 32, G = E, NC = NE / E;
+    static __host__ __device__ constexpr int max_v() { return 64 * NE - E + 1; }
+    Row<T> row;
+    int V, lane;
+    __device__ __forceinline__ Small(const T* p, int v, int l) : row(p, v), V(v), lane(l) {}
+    __device__ __forceinline__ int index(int j) const { return ((j / E) * 64 + lane) * E + j % E - row.sh; }
+    __device__ __forceinline__ int groups() const { return (row.n + 63) / 64; }
+    __device__ __forceinline__ void load(float (&x)[NE]) const {
+        uint4 v[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (i * 64 + lane < row.n) v[i] = row.load(i * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float y[E];
+            Chunk<T>::unpack(v[i], y);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[i * E + e] = i * 64 + lane < row.n ? y[e] : -INFINITY;
+        }
+    }
+};
+
+template <typename T, int W, bool TOP>
+__global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t,
+                                                             const int64_t* __restrict__ tokens, int k, float* __restrict__ logp,
+                                                             float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats,
+                                                             int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+    using S = Small<T, W>;
+    constexpr int NE = S::NE, G = S::G, CAP = W == 16 ? 64 : 256;
+    const int lane = threadIdx.x & (W - 1), team = threadIdx.x / W;
+    const int64_t r = (int64_t)blockIdx.x * (256 / W) + team;
+    if (r >= N) return;
+    const T* zr = z + r * ld;
+    const S row(zr, V, lane);
+    float x[NE];
+    row.load(x);
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < NE; ++j) m = fmaxf(m, x[j]);
+    m = fmaxf(lanes_join<W>(m, Max()), LG_NEG);
+    Acc a = {m, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NE / G; ++g) {
+        if (g >= row.groups()) break;
+#pragma unroll
+        for (int j = g * G; j < g * G + G; ++j) {
+            const float y = (x[j] - m) * c, p = __builtin_amdgcn_exp2f(y);
+            const bool none = x[j] == -INFINITY;      // (m may be the type's lowest value: y = -inf, or NaN where m is +inf)
+            a.s += none ? 0.f : p;
+            a.t += p == 0.f || none ? 0.f : p * y;
+        }
+    }
+    a.s = lanes_join<W>(a.s, Add());
+    a.t = lanes_join<W>(a.t, Add());
+    const bool empty = a.s == 0.f;
+    const float log_s = empty ? -INFINITY : logf(a.s);
+    if (lane == 0) {
+        stats[r * 2] = a.m;
+        stats[r * 2 + 1] = a.s;
+        lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
+        entropy[r] = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
+        if (tokens) {
+            const int64_t t = tokens[r];
+            float v = 0.f;
+            if (t >= V) v = NAN;
+            else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(zr + t) - a.m) * inv_t - log_s;
+            logp[r] = v;
+        }
+    }
+    if (!TOP) return;
+    __shared__ unsigned long long cand_lds[256 / W][CAP];
+    unsigned long long* cand = cand_lds[team];
+    int n;
+    if (W == 16) {   // every logit is a candidate
+        n = V;
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+            if (row.index(j) < V) cand[row.index(j)] = order_key(x[j], row.index(j));
+    } else {
+        // the k-th largest key from the top bit down, until at most `most` keys reach it (then those are the candidates) or it is exact
+        const auto valid = [&](int j) { return row.index(j) >= 0 && row.index(j) < V; };
+        uint32_t key[NE];
+#pragma unroll
+        for (int j = 0; j < NE; ++j) key[j] = valid(j) ? order_key(x[j]) : 0u;
+        const int most = min(CAP, k + max(8, k >> 2)), ng = row.groups();
+        uint32_t at = 0;
+        n = V;
+        for (int b = 31; b >= 0 && n > most; --b) {
+            const uint32_t t = at | (1u << b);
+            int cnt = 0;
+#pragma unroll
+            for (int g = 0; g < NE / G; ++g) {
+                if (g >= ng) break;
+#pragma unroll
+                for (int j = g * G; j < g * G + G; ++j) cnt += __popcll(__ballot(key[j] >= t));
+            }
+            if (cnt >= k) { at = t; n = cnt; }
+        }
+        const uint32_t above = n <= CAP ? (at ? at - 1u : 0u) : at;   // (at = 0: every valid key, they are at least 1)
+        const unsigned long long lt = (1ull << lane) - 1ull;
+        int n_out = 0;
+#pragma unroll
+        for (int g = 0; g < NE / G; ++g) {
+            if (g >= ng) break;
+#pragma unroll
+            for (int j = g * G; j < g * G + G; ++j) {
+                const unsigned long long on = __ballot(key[j] > above);
+                if (key[j] > above) cand[n_out + __popcll(on & lt)] = ((unsigned long long)key[j] << 32) | (0xFFFFFFFFu - (uint32_t)row.index(j));
+                n_out += __popcll(on);
+            }
+        }
+        if (n > CAP) {   // many logits equal the k-th: the first of them in the row's order (rounds of chunks, lanes, elements)
+            int left = k - n_out;
+#pragma unroll
+            for (int g = 0; g < NE / G; ++g) {
+                if (g >= ng || left <= 0) break;
+                int before = 0, total = 0;
+#pragma unroll
+                for (int j = g * G; j < g * G + G; ++j) {
+                    const unsigned long long on = __ballot(key[j] == at);
+                    before += __popcll(on & lt);
+                    total += __popcll(on);
+                }
+#pragma unroll
+                for (int j = g * G; j < g * G + G; ++j)
+                    if (key[j] == at) {
+                        if (before < left) cand[n_out + before] = ((unsigned long long)key[j] << 32) | (0xFFFFFFFFu - (uint32_t)row.index(j));
+                        ++before;
+                    }
+                const int took = min(total, left);
+                n_out += took;
+                left -= took;
+            }
+        }
+        n = n_out;
+    }
+    Team<W>::sync();
+    for (int q = lane; q < n; q += W) {
+        const unsigned long long me = cand[q];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += cand[j] > me;
+        if (place < k) {
+            top_ids[r * k + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
+            top_logp[r * k + place] = empty ? -INFINITY : (key_value((uint32_t)(me >> 32)) - a.m) * inv_t - log_s;
         }
     }
 }
 
-// dz_i = inv_t [ p_i (A + B log p_i) + g_t 1[i = t] + sum_j g_j 1[i = id_j] ],  A = g_lse - g_t - sum_j g_j - g_H H,  B = -g_H
-template <typename T>
-__global__ __launch_bounds__(LG_THREADS) void token_logprobs_bwd_kernel(const T* __restrict__ z, int64_t ld, int V, float inv_t,
-                                                                        const float* __restrict__ stats, const float* __restrict__ entropy,
-                                                                        const int64_t* __restrict__ tokens, const float* __restrict__ g_logp,
-                                                                        const float* __restrict__ g_entropy, const float* __restrict__ g_lse,
-                                                                        int top_k, const int64_t* __restrict__ top_ids,
-                                                                        const float* __restrict__ g_top, T* __restrict__ dz, int64_t ldd) {
-    __shared__ float red[LG_WAVES];
-    const int64_t row = blockIdx.x;
-    const T* zr = z + row * ld;
-    T* dr = dz + row * ldd;
-    const float m = stats[row * 2], s = stats[row * 2 + 1];
-    if (s == 0.f) {   // nothing in the row has a probability
-        for (int i = threadIdx.x; i < V; i += LG_THREADS) Store<T>::store(dr + i, 0.f);
-        return;
-    }
-    const float inv_s = 1.f / s, log_s = logf(s);
-    const int64_t t = tokens ? tokens[row] : -1;
-    const float gt = t < 0 || !g_logp ? 0.f : t < V ? g_logp[row] : NAN;
-    const float gh = g_entropy ? g_entropy[row] : 0.f;
+// ---- gradients ------------------------------------------------------------------------------------------------------------------
+// Both gradients are one map over the row, e_i = exp2((z_i - m) c) times a number of the row (the entropy's: times a linear function of its
+// exponent), and a few places (the given token, the listed ones) where something is added: those are written again once the row is done.
+// One read and one write of the row; a lane has U chunks in flight.
+
+// dz_i = inv_t [ p_i (A + B ln p_i) + g_t 1[i = t] + sum_j g_j 1[i = id_j] ],  A = g_lse - g_t - sum_j g_j - g_H H,  B = -g_H
+struct LogprobsGrad {
+    const float *stats, *entropy, *g_logp, *g_entropy, *g_lse, *g_top;
+    const int64_t *tokens, *top_ids;
+    int k;
+};
+template <typename T, int TH>
+__global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t, LogprobsGrad q,
+                                                                           T* __restrict__ dz, int64_t ldd) {
+    constexpr int E = Chunk<T>::E, U = 4, PER = TH < 256 ? 256 / TH : 1;
+    __shared__ float red[TH < 64 ? 1 : TH / 64];
+    const int64_t r = (int64_t)blockIdx.x * PER + (PER > 1 ? threadIdx.x / TH : 0);
+    if (PER > 1 && r >= N) return;
+    const int tid = Team<TH>::rank();
+    const Row<T> row(z + r * ld, V);
+    T* d = dz + r * ldd;
+    const Acc a = {q.stats[r * 2], q.stats[r * 2 + 1], 0.f};
+    const int64_t t = q.tokens ? q.tokens[r] : -1;
+    const float gt = t < 0 ? 0.f : t < V ? q.g_logp[r] : NAN, gh = q.g_entropy ? q.g_entropy[r] : 0.f;
     float gs = 0.f;
-    if (g_top)
-        for (int j = threadIdx.x; j < top_k; j += LG_THREADS) gs += g_top[row * top_k + j];
-    const float A = (g_lse ? g_lse[row] : 0.f) - gt - block_sum(gs, red) - gh * entropy[row], B = -gh;
-    for (int i = threadIdx.x; i < V; i += LG_THREADS) {
-        const float d = (Store<T>::load(zr + i) - m) * inv_t;
-        const float p = expf(d) * inv_s;
-        Store<T>::store(dr + i, p == 0.f ? 0.f : inv_t * p * (A + B * (d - log_s)));
+    for (int j = tid; j < q.k; j += TH) gs += q.g_top[r * q.k + j];
+    if (q.k) gs = Team<TH>::sum(gs, red);
+    const bool empty = a.s == 0.f;
+    const float f = empty ? 0.f : inv_t / a.s, log_s = empty ? 0.f : logf(a.s);
+    const float A = (q.g_lse ? q.g_lse[r] : 0.f) - gt - gs - gh * q.entropy[r];
+    // p (A + B ln p) inv_t = e (c0 + c1 y):  ln p = y ln2 - ln s
+    const Ref ref(a.m, c);
+    const float undo = __builtin_amdgcn_exp2f(-ref.delta), c1 = undo * -f * gh * LG_LN2, c0 = empty ? 0.f : undo * f * (A + gh * log_s) - c1 * ref.delta;
+    const auto one = [&](float x) {
+        const float y = fmaxf(ref.y(x, c), -200.f);   // (a masked logit: e = 0, whatever c1 is)
+        return __builtin_amdgcn_exp2f(y) * fmaf(c1, y, c0);
+    };
+    for (int ch0 = tid; ch0 < row.n; ch0 += U * TH) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch0 + u * TH < row.n) v[u] = row.load(ch0 + u * TH);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch0 + u * TH < row.n) {
+                float x[E];
+                Chunk<T>::unpack(v[u], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = one(x[e]);
+                row.store(d, ch0 + u * TH, x);
+            }
     }
-    __syncthreads();
-    // the listed places again, with what lands on them alone (top ids are distinct; the given token may be one of them)
-    for (int j = threadIdx.x; j <= top_k; j += LG_THREADS) {
-        const bool is_token = j == top_k;
-        if (is_token ? (t < 0 || t >= V) : !g_top) continue;
-        const int64_t i = is_token ? t : top_ids[row * top_k + j];
+    if (empty) return;
+    Team<TH>::sync();
+    // (top ids are distinct; the given token may be one of them)
+    for (int j = tid; j <= q.k; j += TH) {
+        const bool is_token = j == q.k;
+        const int64_t i = is_token ? t : q.top_ids[r * q.k + j];
         if (i < 0 || i >= V) continue;
-        float g = is_token ? gt : g_top[row * top_k + j];
+        float g = is_token ? gt : q.g_top[r * q.k + j];
         if (!is_token && i == t) g += gt;
-        bool dup = false;
-        if (is_token && g_top)
-            for (int q = 0; q < top_k; ++q) dup |= top_ids[row * top_k + q] == i;
-        if (dup) continue;
-        const float d = (Store<T>::load(zr + i) - m) * inv_t;
-        const float p = expf(d) * inv_s;
-        Store<T>::store(dr + i, inv_t * ((p == 0.f ? 0.f : p * (A + B * (d - log_s))) + g));
+        bool again = false;
+        if (is_token)
+            for (int p = 0; p < q.k; ++p) again |= q.top_ids[r * q.k + p] == i;
+        if (!again) Store<T>::store(d + i, one(Store<T>::load(row.z + i)) + inv_t * g);
     }
 }
+
+// ---- distillation ---------------------------------------------------------------------------------------------------------------
+// L = tau^2 [ sum_j q_j (ln q_j - ln p_j) + rest (ln rest - ln p_off) ]
+// dL/dz_i = tau [ p_i (Q + rest) - q_i - 1[i off the list] rest p_i / p_off ]
+// With the tail, the sums over the row leave the listed tokens out (a bit per logit in LDS, set from the list) and the listed ones are added
+// from the list: p_off is summed, not the difference of two sums, and holds where the student leaves the rest next to nothing.
+struct Distill {
+    const int64_t* ids;
+    const void* logp;
+    int dtype, K;
+    const float* weights;
+    float weight0;
+};
+
+// the list of a row in LDS: token (-1: empty slot, V: no token of the row), mass, and the mass of all slots that name the same token for the
+// first of them (-1 for the others)
+template <int TH> struct ListLds {
+    static constexpr int PER = TH < 256 ? 256 / TH : 1;
+    int id[PER][AG_LOGITS_MAX_TOP];
+    float q[PER][AG_LOGITS_MAX_TOP];
+};
 
 struct Teacher { float Q, rest, qlogq; };
 
-// the list's masses q_j (LDS) and their sums; ids below 0 are empty slots, ids beyond the row make every sum NaN
-__device__ Teacher teacher_row(const int64_t* __restrict__ ids, const void* __restrict__ logp, int logp_dtype, int64_t at, int K, int V, bool tail,
-                               int* sid, float* sq, float* red) {
-    const int tid = threadIdx.x;
-    float lp = -INFINITY;
-    int id = -1;
-    if (tid < K) {
-        const int64_t i = ids[at + tid];
-        id = i < 0 ? -1 : i >= V ? V : (int)i;
-        lp = logp_dtype == AG_BF16 ? bf16_to_f32(((const bf16_t*)logp)[at + tid]) : ((const float*)logp)[at + tid];
-        if (id < 0) lp = -INFINITY;
-        if (id == V) lp = NAN;
+template <int TH, bool TAIL>
+__device__ __forceinline__ Teacher read_list(const Distill& p, int64_t r, int V, int* sid, float* sq, float* red) {
+    constexpr int J = (AG_LOGITS_MAX_TOP + TH - 1) / TH;
+    const int tid = Team<TH>::rank();
+    float lp[J];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+        const int j = tid + i * TH;
+        lp[i] = -INFINITY;
+        if (j >= p.K) continue;
+        const int64_t id = p.ids[r * p.K + j];
+        const float v = p.dtype == AG_BF16 ? bf16_to_f32(((const bf16_t*)p.logp)[r * p.K + j]) : ((const float*)p.logp)[r * p.K + j];
+        sid[j] = id < 0 ? -1 : id >= V ? V : (int)id;
+        lp[i] = id < 0 ? -INFINITY : id >= V ? NAN : v;
+        m = fmaxf(m, lp[i]);
     }
-    const float m = block_max(lp, red);
-    if (!tail) {
-        const float e = lp == -INFINITY ? 0.f : expf(lp - m);
-        const float s = block_sum(e, red);
-        lp = s == 0.f ? -INFINITY : (lp - m) - logf(s);
+    m = Team<TH>::max(m, red);
+    if (!TAIL) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < J; ++i) s += lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
+        s = Team<TH>::sum(s, red);
+        const float ls = logf(s);
+#pragma unroll
+        for (int i = 0; i < J; ++i) lp[i] = s == 0.f ? -INFINITY : (lp[i] - m) - ls;
     }
-    const float q = lp == -INFINITY ? 0.f : expf(lp);
-    if (tid < K) { sid[tid] = id; sq[tid] = q; }
-    Teacher r;
-    r.Q = block_sum(q, red);
-    r.qlogq = block_sum(q == 0.f ? 0.f : q * lp, red);
-    // 1 - sum q without the cancellation of its largest term: -expm1(lp) of that one, minus the others
-    r.rest = 0.f;
-    if (tail) {
-        __shared__ int first;
-        if (tid == 0) first = K;
-        __syncthreads();
-        if (tid < K && lp == m) atomicMin(&first, tid);
-        __syncthreads();
-        const float part = tid == first && lp > -INFINITY ? -expm1f(lp) : -q;
-        const float sum = block_sum(part, red);
-        r.rest = m == -INFINITY ? 1.f : fmaxf(sum, 0.f);
-        if (r.Q != r.Q) r.rest = r.Q;
+    Teacher t = {0.f, 0.f, 0.f};
+    float others = 0.f;   // the masses that are not the largest
+    int top = 0;          // slots that have the largest
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+        const int j = tid + i * TH;
+        const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
+        if (j < p.K) sq[j] = q;
+        t.Q += q;
+        t.qlogq += q == 0.f ? 0.f : q * lp[i];
+        if (TAIL) { if (lp[i] == m) ++top; else others += q; }
     }
-    return r;
+    t.Q = Team<TH>::sum(t.Q, red);
+    t.qlogq = Team<TH>::sum(t.qlogq, red);
+    if (TAIL) {
+        // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
+        const float n_top = Team<TH>::sum((float)top, red);
+        others = Team<TH>::sum(others, red);
+        t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (n_top - 1.f) * expf(m) - others, 0.f);
+        if (t.Q != t.Q) t.rest = t.Q;
+    }
+    return t;
 }
 
-// L = tau^2 [ sum_j q_j (ln q_j - ln p_j) + rest (ln rest - ln p_off) ];  dL/dz_i = tau [ p_i (Q + rest) - q_i - 1[i off the list] rest p_i / p_off ]
-// stats (m_off, a, m, on): the gradient is tau g a exp((z - m_off) / tau) off the list and tau g (on exp((z - m) / tau) - q) on it
-template <typename T, bool TAIL>
-__global__ __launch_bounds__(LG_THREADS) void topk_distill_kernel(const T* __restrict__ z, int64_t ld, int V, float tau, float inv_t,
-                                                                  const int64_t* __restrict__ ids, const void* __restrict__ t_logp, int t_dtype, int K,
-                                                                  const float* __restrict__ weights, float* __restrict__ row_loss,
-                                                                  float* __restrict__ stats) {
-    extern __shared__ uint32_t bits[];
-    __shared__ float red[LG_WAVES];
-    __shared__ int sid[LG_THREADS];
-    __shared__ float sq[LG_THREADS];
-    __shared__ int distinct;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const T* zr = z + row * ld;
-    if (weights && weights[row] == 0.f) {
-        if (tid == 0) row_loss[row] = 0.f;
-        if (tid < 4) stats[row * 4 + tid] = 0.f;
-        return;
-    }
-    Teacher tc = teacher_row(ids, t_logp, t_dtype, row * K, K, V, TAIL, sid, sq, red);
-    if (TAIL) {
-        if (tid == 0) distinct = 0;
-        for (int i = tid; i < (V + 31) / 32; i += LG_THREADS) bits[i] = 0u;
-        __syncthreads();
-        if (tid < K && sid[tid] >= 0 && sid[tid] < V) {
-            const uint32_t b = 1u << (sid[tid] & 31);
-            if (!(atomicOr(&bits[sid[tid] >> 5], b) & b)) atomicAdd(&distinct, 1);
-        }
-        __syncthreads();
-        if (distinct == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
-    }
-    const RowSums off = row_sums<T, TAIL>(zr, V, inv_t, bits, red);   // over the tokens off the list (TAIL) or over all of them
-    const bool mine = tid < K && sid[tid] >= 0 && sid[tid] < V;       // this thread's slot names a token
-    bool first = mine;                                                // ... that no earlier slot names
-    float x = LG_NEG;
-    if (mine) {
-        x = Store<T>::load(zr + sid[tid]);
-        for (int j = 0; j < tid; ++j) first &= sid[j] != sid[tid];
-    }
-    float m = off.m, s = off.s;
-    if (TAIL) {
-        m = fmaxf(m, block_max(x, red));
-        s = block_sum(first && x != -INFINITY ? expf((x - m) * inv_t) : 0.f, red) + (off.s == 0.f ? 0.f : off.s * expf((off.m - m) * inv_t));
-    }
-    const bool empty = s == 0.f;
-    const float log_s = empty ? -INFINITY : logf(s);
-    const float q = tid < K ? sq[tid] : 0.f;
-    const float cross = block_sum(q == 0.f ? 0.f : !mine ? NAN : q * (empty ? INFINITY : log_s - (x - m) * inv_t), red);
-    if (tid == 0) {
-        float L = tc.qlogq + cross;
-        const float log_off = off.s == 0.f ? -INFINITY : (off.m - m) * inv_t + logf(off.s) - log_s;
-        if (TAIL && tc.rest != 0.f) L += tc.rest * (logf(tc.rest) - log_off);
-        row_loss[row] = tau * tau * L;
-        const float on = empty ? 0.f : (tc.Q + tc.rest) / s;
-        stats[row * 4] = off.m;
-        stats[row * 4 + 1] = !TAIL ? on : off.s == 0.f ? 0.f : on * expf((off.m - m) * inv_t) - tc.rest / off.s;
-        stats[row * 4 + 2] = empty ? -INFINITY : m;
-        stats[row * 4 + 3] = on;
-    }
-}
+// what a row's gradient takes from the forward pass: g a exp2((z - m_off) c) off the list, g (on exp2((z - m) c) - q) on it
+struct GradOf { float m_off, a, m, on; };
 
-template <typename T>
-__global__ __launch_bounds__(LG_THREADS) void topk_distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int V, float tau, float inv_t,
-                                                                      const int64_t* __restrict__ ids, const void* __restrict__ t_logp, int t_dtype,
-                                                                      int K, const float* __restrict__ weights, float weight0, int tail,
-                                                                      const float* __restrict__ stats, const float* __restrict__ g_loss,
-                                                                      const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
-    __shared__ float red[LG_WAVES];
-    __shared__ int sid[LG_THREADS];
-    __shared__ float sq[LG_THREADS];
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const T* zr = z + row * ld;
-    T* dr = dz + row * ldd;
-    const float w = weights ? weights[row] : weight0;
-    const float m_off = stats[row * 4], a = stats[row * 4 + 1], m = stats[row * 4 + 2], on = stats[row * 4 + 3];
-    if (w == 0.f || m == -INFINITY) {   // the row takes no part, or none of its logits is above -inf
-        for (int i = tid; i < V; i += LG_THREADS) Store<T>::store(dr + i, 0.f);
-        return;
-    }
-    const float g = tau * ((g_loss ? w * g_loss[0] : 0.f) + (g_row ? g_row[row] : 0.f) + (!g_loss && !g_row ? w : 0.f));
-    teacher_row(ids, t_logp, t_dtype, row * K, K, V, tail != 0, sid, sq, red);
-    for (int i = tid; i < V; i += LG_THREADS) {
-        const float e = expf((Store<T>::load(zr + i) - m_off) * inv_t);
-        Store<T>::store(dr + i, e == 0.f ? 0.f : g * a * e);
-    }
-    __syncthreads();
-    if (tid < K && sid[tid] >= 0 && sid[tid] < V) {
+template <typename T, int TH>
+__device__ __forceinline__ void listed_gradients(const Row<T>& row, const int* sid, const float* sq, int K, const GradOf& s, float g, float c, T* d) {
+    for (int j = Team<TH>::rank(); j < K; j += TH) {
+        const int i = sid[j];
+        if (i < 0 || i >= row.V) continue;
         float q = 0.f;
         bool first = true;
-        for (int j = 0; j < K; ++j)
-            if (sid[j] == sid[tid]) { q += sq[j]; first &= j >= tid; }
-        const float e = expf((Store<T>::load(zr + sid[tid]) - m) * inv_t);
-        if (first) Store<T>::store(dr + sid[tid], g * ((e == 0.f ? 0.f : e * on) - q));
+        for (int p = 0; p < K; ++p)
+            if (sid[p] == i) { q += sq[p]; first &= p >= j; }
+        if (first) Store<T>::store(d + i, g * (exp2_from(Store<T>::load(row.z + i), s.m, c) * s.on - q));
     }
+}
+template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const uint4& v, float c, const Ref& ref, float ga, T* d) {
+    constexpr int E = Chunk<T>::E;
+    float x[E];
+    Chunk<T>::unpack(v, x);
+    if (!ref.far) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = ga * __builtin_amdgcn_exp2f(fmaf(x[e], c, ref.nr));
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = ga * exp2_from(x[e], ref.m, c);
+    }
+    row.store(d, ch, x);
+}
+template <typename T, int TH> __device__ __forceinline__ void zero_row(const Row<T>& row, T* d) {
+    constexpr int E = Chunk<T>::E;
+    const float x[E] = {};
+    for (int ch = Team<TH>::rank(); ch < row.n; ch += TH) row.store(d, ch, x);
+}
+
+// words of LDS for a bit per logit of a row's chunks, whatever its alignment
+template <typename T> __host__ __device__ constexpr int bit_words(int V) { return (V + Chunk<T>::E - 1 + 31) / 32 + 1; }
+
+// Loss, and (GRAD) its gradient from the same pass: a lane holds NC chunks of the row in registers between the sums and the gradient, so a
+// row of up to TH NC chunks is read once; a longer one takes several rounds and reads all but its last round again.
+template <typename T, int TH, int NC, bool TAIL, bool GRAD>
+__global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p,
+                                                                      float* __restrict__ row_loss, float* __restrict__ stats, T* __restrict__ dz,
+                                                                      int64_t ldd) {
+    constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1, BITS = 32 / E;   // chunks whose bits share a word
+    extern __shared__ uint32_t bits_lds[];
+    __shared__ float red[TH < 64 ? 1 : 3 * (TH / 64)];
+    __shared__ ListLds<TH> list;
+    const int team = PER > 1 ? threadIdx.x / TH : 0, tid = Team<TH>::rank();
+    const int64_t r = (int64_t)blockIdx.x * PER + team;
+    if (PER > 1 && r >= N) return;
+    const Row<T> row(z + r * ld, V);
+    T* d = dz + r * ldd;
+    const float w = p.weights ? p.weights[r] : p.weight0;
+    if (w == 0.f) {   // the row takes no part
+        if (tid == 0) row_loss[r] = 0.f;
+        if (!GRAD && tid < 4) stats[r * 4 + tid] = 0.f;
+        if (GRAD) zero_row<T, TH>(row, d);
+        return;
+    }
+    uint4 v[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+        if (i * TH + tid < row.n) v[i] = row.load(i * TH + tid);
+    int* sid = list.id[team];
+    float* sq = list.q[team];
+    Teacher tc = read_list<TH, TAIL>(p, r, V, sid, sq, red);
+    uint32_t* bits = bits_lds + (TAIL ? team * bit_words<T>(V) : 0);
+    if (TAIL) {
+        for (int i = tid; i < (row.n + BITS - 1) / BITS; i += TH) bits[i] = 0u;
+        Team<TH>::sync();
+        float fresh = 0.f;
+        for (int j = tid; j < p.K; j += TH) {
+            if (sid[j] < 0 || sid[j] >= V) continue;
+            const int at = sid[j] + row.sh;
+            const uint32_t b = 1u << (at & 31);
+            fresh += atomicOr(&bits[at >> 5], b) & b ? 0.f : 1.f;
+        }
+        if ((int)Team<TH>::sum(fresh, red) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
+        Team<TH>::sync();
+    } else {
+        Team<TH>::sync();
+    }
+    Sums<T, false> sums(c);
+    for (int c0 = 0;;) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int ch = c0 + i * TH + tid;
+            if (ch < row.n) {
+                float y[E];
+                Chunk<T>::unpack(v[i], y);
+                if (TAIL) {
+                    const uint32_t b = bits[ch / BITS] >> ((ch % BITS) * E);
+                    if (b & ((1u << E) - 1u)) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if ((b >> e) & 1u) y[e] = -INFINITY;
+                    }
+                }
+                sums.add(y, max_of(y));
+            }
+        }
+        if (c0 + NC * TH >= row.n) break;
+        c0 += NC * TH;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (c0 + i * TH + tid < row.n) v[i] = row.load(c0 + i * TH + tid);
+    }
+    const Acc off = team_join<TH>(sums.acc(), c, red);
+    // the listed tokens' logits: their part of the sums (with the tail), and of the loss
+    Acc all = off;
+    float cross = 0.f, lm = LG_NEG;
+    for (int j = tid; j < p.K; j += TH)
+        if (sid[j] >= 0 && sid[j] < V) lm = fmaxf(lm, Store<T>::load(row.z + sid[j]));
+    if (TAIL) {
+        all = rebase(off, fmaxf(off.m, Team<TH>::max(lm, red)), c);
+        float s = 0.f;
+        for (int j = tid; j < p.K; j += TH) {
+            if (sid[j] < 0 || sid[j] >= V) continue;
+            bool first = true;
+            for (int i = 0; i < j; ++i) first &= sid[i] != sid[j];
+            if (first) s += exp2_from(Store<T>::load(row.z + sid[j]), all.m, c);
+        }
+        all.s += Team<TH>::sum(s, red);
+    }
+    const bool empty = all.s == 0.f;
+    const float log_s = empty ? -INFINITY : logf(all.s);
+    for (int j = tid; j < p.K; j += TH) {
+        const float q = sq[j];
+        if (q == 0.f) continue;
+        cross += sid[j] >= V ? NAN : q * (empty ? INFINITY : log_s - (Store<T>::load(row.z + sid[j]) - all.m) * inv_t);
+    }
+    cross = Team<TH>::sum(cross, red);
+    GradOf s;
+    s.m_off = off.m;
+    s.m = empty ? -INFINITY : all.m;
+    s.on = empty ? 0.f : (tc.Q + tc.rest) / all.s;
+    s.a = !TAIL ? s.on : off.s == 0.f ? 0.f : s.on * __builtin_amdgcn_exp2f((off.m - all.m) * c) - tc.rest / off.s;
+    if (tid == 0) {
+        float L = tc.qlogq + cross;
+        if (TAIL && tc.rest != 0.f) L += tc.rest * (logf(tc.rest) - (off.s == 0.f ? -INFINITY : (off.m - all.m) * inv_t + logf(off.s) - log_s));
+        row_loss[r] = tau * tau * L;
+        if (!GRAD) *reinterpret_cast<float4*>(stats + r * 4) = make_float4(s.m_off, s.a, s.m, s.on);
+    }
+    if (!GRAD) return;
+    if (empty) { zero_row<T, TH>(row, d); return; }
+    const Ref ref(s.m_off, c);
+    const float g = tau * w, ga = g * s.a * __builtin_amdgcn_exp2f(-ref.delta);
+    for (int c0 = (row.n - 1) / (NC * TH) * (NC * TH);;) {   // the last round's chunks are still here
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (c0 + i * TH + tid < row.n) gradient_chunk(row, c0 + i * TH + tid, v[i], c, ref, ga, d);
+        c0 -= NC * TH;
+        if (c0 < 0) break;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = row.load(c0 + i * TH + tid);
+    }
+    Team<TH>::sync();
+    listed_gradients<T, TH>(row, sid, sq, p.K, s, g, c, d);
+}
+
+template <typename T, int TH, bool TAIL>
+__global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
+                                                                          const float* __restrict__ stats, const float* __restrict__ g_loss,
+                                                                          const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
+    constexpr int U = 4, PER = TH < 256 ? 256 / TH : 1;
+    __shared__ float red[TH < 64 ? 1 : TH / 64];
+    __shared__ ListLds<TH> list;
+    const int team = PER > 1 ? threadIdx.x / TH : 0, tid = Team<TH>::rank();
+    const int64_t r = (int64_t)blockIdx.x * PER + team;
+    if (PER > 1 && r >= N) return;
+    const Row<T> row(z + r * ld, V);
+    T* d = dz + r * ldd;
+    const float w = p.weights ? p.weights[r] : p.weight0;
+    const float4 st = *reinterpret_cast<const float4*>(stats + r * 4);
+    const GradOf s = {st.x, st.y, st.z, st.w};
+    if (w == 0.f || s.m == -INFINITY) {   // the row takes no part, or none of its logits is above -inf
+        zero_row<T, TH>(row, d);
+        return;
+    }
+    const Ref ref(s.m_off, c);
+    const float g = tau * (g_loss || g_row ? (g_loss ? w * g_loss[0] : 0.f) + (g_row ? g_row[r] : 0.f) : w);
+    const float ga = g * s.a * __builtin_amdgcn_exp2f(-ref.delta);
+    for (int ch0 = tid; ch0 < row.n; ch0 += U * TH) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch0 + u * TH < row.n) v[u] = row.load(ch0 + u * TH);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch0 + u * TH < row.n) gradient_chunk(row, ch0 + u * TH, v[u], c, ref, ga, d);
+    }
+    read_list<TH, TAIL>(p, r, V, list.id[team], list.q[team], red);
+    Team<TH>::sync();
+    listed_gradients<T, TH>(row, list.id[team], list.q[team], p.K, s, g, c, d);
 }
 
 // sum_n w_n L_n in a fixed order
@@ -333,12 +992,99 @@ __global__ __launch_bounds__(1024) void weighted_sum_kernel(const float* __restr
     }
 }
 
+// ---- host -----------------------------------------------------------------------------------------------------------------------
 int check_rows(const char* who, const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature) {
     AG_REQUIRE(N >= 0 && V >= 1 && V <= AG_LOGITS_MAX_V, "%s: %d rows x %d logits (1 to %d logits per row)", who, N, V, AG_LOGITS_MAX_V);
     AG_REQUIRE(d_logits || N == 0, "%s: null pointer", who);
     AG_REQUIRE(dtype == AG_F32 || dtype == AG_BF16, "%s: dtype %d (AG_F32 or AG_BF16)", who, dtype);
     AG_REQUIRE(ld >= 0, "%s: row stride %lld", who, (long long)ld);
     AG_REQUIRE(temperature > 0.f && temperature <= 3.0e38f, "%s: temperature %g (a positive number)", who, (double)temperature);
+    return AG_OK;
+}
+int check_teacher(const char* who, const void* ids, const void* t_logp, int t_dtype, int K, int N) {
+    AG_REQUIRE(K >= 1 && K <= AG_LOGITS_MAX_TOP, "%s: lists of %d tokens (1 to %d)", who, K, AG_LOGITS_MAX_TOP);
+    AG_REQUIRE(N == 0 || (ids && t_logp), "%s: null pointer", who);
+    AG_REQUIRE(t_dtype == AG_F32 || t_dtype == AG_BF16, "%s: teacher dtype %d (AG_F32 or AG_BF16)", who, t_dtype);
+    return AG_OK;
+}
+float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
+float one_over(float temperature) { return (float)(1.0 / (double)temperature); }
+
+// threads that own a row of V logits
+template <typename T> int team_of(int V, int N) {
+    if (V <= Small<T, 16>::max_v()) return 16;
+    if (V <= Small<T, 64>::max_v()) return 64;
+    const int chunks = (V + Chunk<T>::E - 1) / Chunk<T>::E;
+    if (N <= 256) return 1024;
+    return chunks <= 16 * 256 ? 256 : chunks <= 16 * 512 ? 512 : 1024;
+}
+#define AG_TEAM_SWITCH(th, CALL)                   \
+    switch (th) {                                  \
+        case 16: { CALL(16); break; }              \
+        case 64: { CALL(64); break; }              \
+        case 256: { CALL(256); break; }            \
+        case 512: { CALL(512); break; }            \
+        default: { CALL(1024); break; }            \
+    }
+template <int TH> dim3 team_grid(int N) { return dim3(TH < 256 ? ceil_div(N, 256 / TH) : N); }
+
+template <typename T, bool TOP>
+int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_tokens, int k, float* d_logp, float* d_entropy, float* d_lse,
+             float* d_stats, int64_t* d_top_ids, float* d_top_logp, hipStream_t s) {
+    const float c = log2e_over(temperature), inv_t = one_over(temperature);
+    const T* z = (const T*)d_logits;
+#define LG_SMALL(W) hipLaunchKernelGGL((logprobs_small_kernel<T, W, TOP>), team_grid<W>(N), dim3(256), 0, s, z, ld, N, V, c, inv_t, d_tokens, k, d_logp, \
+                                       d_entropy, d_lse, d_stats, d_top_ids, d_top_logp)
+#define LG_WG(TH) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP>), dim3(N), dim3(TH), 0, s, z, ld, V, c, inv_t, d_tokens, k, d_logp, d_entropy, d_lse, \
+                                     d_stats, d_top_ids, d_top_logp)
+    switch (team_of<T>(V, N)) {
+        case 16: LG_SMALL(16); break;
+        case 64: LG_SMALL(64); break;
+        case 256: LG_WG(256); break;
+        case 512: LG_WG(512); break;
+        default: LG_WG(1024); break;
+    }
+#undef LG_SMALL
+#undef LG_WG
+    AG_LAUNCH_CHECK();
+    return AG_OK;
+}
+
+template <typename T>
+int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const LogprobsGrad& q, void* d_dlogits, int64_t ldd, hipStream_t s) {
+#define LG_CALL(TH) hipLaunchKernelGGL((logprobs_bwd_kernel<T, TH>), team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, \
+                                       log2e_over(temperature), one_over(temperature), q, (T*)d_dlogits, ldd)
+    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+#undef LG_CALL
+    AG_LAUNCH_CHECK();
+    return AG_OK;
+}
+
+template <typename T, bool TAIL, bool GRAD>
+int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, float* d_row_loss, float* d_stats, void* d_dlogits,
+            int64_t ldd, hipStream_t s) {
+    constexpr int E = Chunk<T>::E;
+#define LG_CALL(TH)                                                                                                                                   \
+    constexpr int NC = TH == 16 ? (E == 8 ? 1 : 2) : TH == 64 ? (E == 8 ? 4 : 8) : GRAD ? 16 : 4;                                                     \
+    const size_t lds = TAIL ? (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1) : 0;                                                                      \
+    hipLaunchKernelGGL((distill_kernel<T, TH, NC, TAIL, GRAD>), team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), lds, s, (const T*)d_logits, ld, N, V,     \
+                       temperature, log2e_over(temperature), one_over(temperature), p, d_row_loss, d_stats, (T*)d_dlogits, ldd)
+    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+#undef LG_CALL
+    AG_LAUNCH_CHECK();
+    return AG_OK;
+}
+
+template <typename T>
+int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, int tail, const float* d_stats, const float* d_g_loss,
+                const float* d_g_row, void* d_dlogits, int64_t ldd, hipStream_t s) {
+#define LG_CALL(TH)                                                                                                                                   \
+    const auto kernel = tail ? distill_bwd_kernel<T, TH, true> : distill_bwd_kernel<T, TH, false>;                                                    \
+    hipLaunchKernelGGL(kernel, team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, temperature, log2e_over(temperature), p, \
+                       d_stats, d_g_loss, d_g_row, (T*)d_dlogits, ldd)
+    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+#undef LG_CALL
+    AG_LAUNCH_CHECK();
     return AG_OK;
 }
 
@@ -352,16 +1098,8 @@ extern "C" int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V,
                AG_LOGITS_MAX_TOP, V);
     if (N == 0) return AG_OK;
     AG_REQUIRE(d_entropy && d_lse && d_stats && (!d_tokens || d_logp) && (top_k == 0 || (d_top_ids && d_top_logp)), "ag_token_logprobs: null pointer");
-    const float inv_t = (float)(1.0 / (double)temperature);
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == AG_BF16)
-        hipLaunchKernelGGL(token_logprobs_kernel<bf16_t>, dim3(N), dim3(LG_THREADS), 0, s, (const bf16_t*)d_logits, ld, V, inv_t, d_tokens, top_k, d_logp,
-                           d_entropy, d_lse, d_stats, d_top_ids, d_top_logp);
-    else
-        hipLaunchKernelGGL(token_logprobs_kernel<float>, dim3(N), dim3(LG_THREADS), 0, s, (const float*)d_logits, ld, V, inv_t, d_tokens, top_k, d_logp,
-                           d_entropy, d_lse, d_stats, d_top_ids, d_top_logp);
-    AG_LAUNCH_CHECK();
-    return AG_OK;
+    const auto run = dtype == AG_BF16 ? (top_k ? logprobs<bf16_t, true> : logprobs<bf16_t, false>) : (top_k ? logprobs<float, true> : logprobs<float, false>);
+    return run(d_logits, ld, N, V, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, (hipStream_t)stream);
 }
 
 extern "C" int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const float* d_stats,
@@ -374,82 +1112,38 @@ extern "C" int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, in
     if (N == 0) return AG_OK;
     AG_REQUIRE(d_stats && d_entropy && d_dlogits && (!d_g_logp || d_tokens) && (!d_g_top_logp || d_top_ids), "ag_token_logprobs_bwd: null pointer");
     AG_REQUIRE(ldd >= V, "ag_token_logprobs_bwd: gradient row stride %lld < %d logits", (long long)ldd, V);
-    const float inv_t = (float)(1.0 / (double)temperature);
-    hipStream_t s = (hipStream_t)stream;
-    if (!d_g_top_logp) top_k = 0;
-    if (!d_g_logp) d_tokens = nullptr;
-    if (dtype == AG_BF16)
-        hipLaunchKernelGGL(token_logprobs_bwd_kernel<bf16_t>, dim3(N), dim3(LG_THREADS), 0, s, (const bf16_t*)d_logits, ld, V, inv_t, d_stats, d_entropy,
-                           d_tokens, d_g_logp, d_g_entropy, d_g_lse, top_k, d_top_ids, d_g_top_logp, (bf16_t*)d_dlogits, ldd);
-    else
-        hipLaunchKernelGGL(token_logprobs_bwd_kernel<float>, dim3(N), dim3(LG_THREADS), 0, s, (const float*)d_logits, ld, V, inv_t, d_stats, d_entropy,
-                           d_tokens, d_g_logp, d_g_entropy, d_g_lse, top_k, d_top_ids, d_g_top_logp, (float*)d_dlogits, ldd);
-    AG_LAUNCH_CHECK();
-    return AG_OK;
-}
-
-static int check_teacher(const char* who, int V, const void* ids, const void* t_logp, int t_dtype, int K, int N) {
-    AG_REQUIRE(K >= 1 && K <= AG_LOGITS_MAX_TOP, "%s: lists of %d tokens (1 to %d)", who, K, AG_LOGITS_MAX_TOP);
-    AG_REQUIRE(N == 0 || (ids && t_logp), "%s: null pointer", who);
-    AG_REQUIRE(t_dtype == AG_F32 || t_dtype == AG_BF16, "%s: teacher dtype %d (AG_F32 or AG_BF16)", who, t_dtype);
-    return AG_OK;
-}
-
-template <typename T>
-static int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_ids, const void* d_t_logp, int t_dtype, int K,
-                       const float* d_weights, int tail, const float* d_stats, const float* d_g_loss, const float* d_g_row, void* d_dlogits,
-                       int64_t ldd, hipStream_t s) {
-    hipLaunchKernelGGL(topk_distill_bwd_kernel<T>, dim3(N), dim3(LG_THREADS), 0, s, (const T*)d_logits, ld, V, temperature,
-                       (float)(1.0 / (double)temperature), d_ids, d_t_logp, t_dtype, K, d_weights, (float)(1.0 / N), tail, d_stats, d_g_loss, d_g_row,
-                       (T*)d_dlogits, ldd);
-    AG_LAUNCH_CHECK();
-    return AG_OK;
-}
-
-template <typename T>
-static int distill_fwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_ids, const void* d_t_logp, int t_dtype, int K,
-                       const float* d_weights, int tail, float* d_row_loss, float* d_stats, hipStream_t s) {
-    const float inv_t = (float)(1.0 / (double)temperature);
-    if (tail)
-        hipLaunchKernelGGL((topk_distill_kernel<T, true>), dim3(N), dim3(LG_THREADS), (size_t)((V + 31) / 32) * 4, s, (const T*)d_logits, ld, V, temperature,
-                           inv_t, d_ids, d_t_logp, t_dtype, K, d_weights, d_row_loss, d_stats);
-    else
-        hipLaunchKernelGGL((topk_distill_kernel<T, false>), dim3(N), dim3(LG_THREADS), 0, s, (const T*)d_logits, ld, V, temperature, inv_t, d_ids, d_t_logp,
-                           t_dtype, K, d_weights, d_row_loss, d_stats);
-    AG_LAUNCH_CHECK();
-    return AG_OK;
+    const LogprobsGrad q = {d_stats, d_entropy, d_g_logp, d_g_entropy, d_g_lse, d_g_top_logp, d_g_logp ? d_tokens : nullptr, d_top_ids,
+                            d_g_top_logp ? top_k : 0};
+    return (dtype == AG_BF16 ? logprobs_bwd<bf16_t> : logprobs_bwd<float>)(d_logits, ld, N, V, temperature, q, d_dlogits, ldd, (hipStream_t)stream);
 }
 
 extern "C" int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
                                const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, float* d_row_loss,
                                float* d_loss, float* d_stats, void* d_dlogits, int64_t ldd, void* stream) {
     if (int rc = check_rows("ag_topk_distill", d_logits, ld, N, V, dtype, temperature)) return rc;
-    if (int rc = check_teacher("ag_topk_distill", V, d_teacher_ids, d_teacher_logp, teacher_dtype, K, N)) return rc;
-    AG_REQUIRE(N >= 1 && d_row_loss && d_loss && d_stats, "ag_topk_distill: no rows or a null pointer");
+    if (int rc = check_teacher("ag_topk_distill", d_teacher_ids, d_teacher_logp, teacher_dtype, K, N)) return rc;
+    AG_REQUIRE(N >= 1 && d_row_loss && d_loss && (d_stats || d_dlogits), "ag_topk_distill: no rows or a null pointer");
     AG_REQUIRE(!d_dlogits || ldd >= V, "ag_topk_distill: gradient row stride %lld < %d logits", (long long)ldd, V);
     hipStream_t s = (hipStream_t)stream;
-    int rc = dtype == AG_BF16 ? distill_fwd<bf16_t>(d_logits, ld, N, V, temperature, d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, tail,
-                                                    d_row_loss, d_stats, s)
-                              : distill_fwd<float>(d_logits, ld, N, V, temperature, d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, tail,
-                                                   d_row_loss, d_stats, s);
-    if (rc) return rc;
-    hipLaunchKernelGGL(weighted_sum_kernel, dim3(1), dim3(1024), 0, s, d_row_loss, d_weights, (float)(1.0 / N), N, d_loss);
+    const Distill p = {d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, (float)(1.0 / N)};
+    const auto bf = tail ? (d_dlogits ? distill<bf16_t, true, true> : distill<bf16_t, true, false>)
+                         : (d_dlogits ? distill<bf16_t, false, true> : distill<bf16_t, false, false>);
+    const auto f = tail ? (d_dlogits ? distill<float, true, true> : distill<float, true, false>)
+                        : (d_dlogits ? distill<float, false, true> : distill<float, false, false>);
+    if (int rc = (dtype == AG_BF16 ? bf : f)(d_logits, ld, N, V, temperature, p, d_row_loss, d_stats, d_dlogits, ldd, s)) return rc;
+    hipLaunchKernelGGL(weighted_sum_kernel, dim3(1), dim3(1024), 0, s, d_row_loss, d_weights, p.weight0, N, d_loss);
     AG_LAUNCH_CHECK();
-    if (!d_dlogits) return AG_OK;
-    return ag_topk_distill_bwd(d_logits, ld, N, V, dtype, temperature, d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, tail, d_stats, nullptr,
-                               nullptr, d_dlogits, ldd, stream);
+    return AG_OK;
 }
 
 extern "C" int ag_topk_distill_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
                                    const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, const float* d_stats,
                                    const float* d_g_loss, const float* d_g_row_loss, void* d_dlogits, int64_t ldd, void* stream) {
     if (int rc = check_rows("ag_topk_distill_bwd", d_logits, ld, N, V, dtype, temperature)) return rc;
-    if (int rc = check_teacher("ag_topk_distill_bwd", V, d_teacher_ids, d_teacher_logp, teacher_dtype, K, N)) return rc;
+    if (int rc = check_teacher("ag_topk_distill_bwd", d_teacher_ids, d_teacher_logp, teacher_dtype, K, N)) return rc;
     AG_REQUIRE(N >= 1 && d_stats && d_dlogits, "ag_topk_distill_bwd: no rows or a null pointer");
     AG_REQUIRE(ldd >= V, "ag_topk_distill_bwd: gradient row stride %lld < %d logits", (long long)ldd, V);
-    hipStream_t s = (hipStream_t)stream;
-    return dtype == AG_BF16 ? distill_bwd<bf16_t>(d_logits, ld, N, V, temperature, d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, tail, d_stats,
-                                                  d_g_loss, d_g_row_loss, d_dlogits, ldd, s)
-                            : distill_bwd<float>(d_logits, ld, N, V, temperature, d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, tail, d_stats,
-                                                 d_g_loss, d_g_row_loss, d_dlogits, ldd, s);
+    const Distill p = {d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, (float)(1.0 / N)};
+    return (dtype == AG_BF16 ? distill_bwd<bf16_t> : distill_bwd<float>)(d_logits, ld, N, V, temperature, p, tail, d_stats, d_g_loss, d_g_row_loss,
+                                                                         d_dlogits, ldd, (hipStream_t)stream);
 }

@@ -40,40 +40,33 @@ template <> struct Chunk<bf16_t> {
     }
 };
 
-// a row as chunks: chunk c holds the logits [c E - sh, c E - sh + E) of [0, V)
+// A row as chunks: chunk c holds the logits [c E - sh, c E - sh + E); those in [first, end) lie inside the row and are aligned 16-byte
+// loads.  The up to E - 1 logits before the first and behind the last of them are the row's ends, one for each of 2 E lanes.  Nothing outside
+// the row is ever touched.
 template <typename T>
 struct Row {
     static constexpr int E = Chunk<T>::E;
     const T* z;
-    int V, sh, n;   // logits, those of the first chunk that lie before the row, chunks
+    int V, sh, first, end;
     __device__ __forceinline__ Row(const T* p, int v) : z(p), V(v) {
         sh = (int)(((uintptr_t)p & 15) / sizeof(T));
-        n = (v + sh + E - 1) / E;
+        first = sh ? 1 : 0;
+        end = max((v + sh) / E, first);
     }
-    // chunks 1 .. n - 2 lie inside the row
-    __device__ __forceinline__ uint4 inner(int c) const { return *reinterpret_cast<const uint4*>(z + (c * E - sh)); }
-    // any chunk; one that reaches over an end of the row is read element by element (nothing outside the row is touched), -inf outside
-    __device__ __forceinline__ uint4 load(int c) const {
-        const int lo = c * E - sh;
-        if (lo >= 0 && lo + E <= V) return *reinterpret_cast<const uint4*>(z + lo);
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = lo + e >= 0 && lo + e < V ? Store<T>::load(z + lo + e) : -INFINITY;
-        return Chunk<T>::pack(x);
+    __device__ __forceinline__ int full() const { return end - first; }
+    __device__ __forceinline__ uint4 load(int c) const { return *reinterpret_cast<const uint4*>(z + (c * E - sh)); }
+    // the logit at the row's ends that belongs to lane l of the row's threads (-1: none)
+    __device__ __forceinline__ int end_index(int l) const {
+        if (l < E) return sh && l < min(E - sh, V) ? l : -1;
+        const int i = max(end * E - sh, 0) + (l - E);
+        return l < 2 * E && i < V ? i : -1;
     }
-    // the chunk's place in another row of the same length (16-byte stores at the logits' alignment: the hardware takes any)
+    // the chunk's place in another row of the same length (at the logits' alignment: the hardware takes any)
     __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const {
         typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t any_uint4;
-        const int lo = c * E - sh;
         const uint4 r = Chunk<T>::pack(x);
-        if (lo >= 0 && lo + E <= V) {
-            const any_uint4 v = {r.x, r.y, r.z, r.w};
-            *reinterpret_cast<any_uint4*>(d + lo) = v;
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lo + e >= 0 && lo + e < V) Store<T>::store(d + lo + e, x[e]);
+        const any_uint4 v = {r.x, r.y, r.z, r.w};
+        *reinterpret_cast<any_uint4*>(d + (c * E - sh)) = v;
     }
 };
 
@@ -179,17 +172,27 @@ struct Sums {
         const float f = __builtin_amdgcn_exp2f(-ref.delta);
         return {ref.m, f * s, f * fmaf(-ref.delta, s, t)};
     }
+    __device__ __forceinline__ void refer(float to) {
+        const Acc a = rebase(acc(), to, c);
+        ref = Ref(to, c);
+        lim = to + slack;
+        zero = ref.far ? NAN : 0.f;
+        const float f = __builtin_amdgcn_exp2f(ref.delta);
+        s = f * a.s;
+        t = f * fmaf(ref.delta, a.s, a.t);
+    }
+    __device__ __forceinline__ void add_guarded(float x, float& cs, float& ct) const {
+        const float y = ref.y(x, c), p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y);
+        cs += p;
+        if (ENTROPY) ct += p == 0.f ? 0.f : p * y;
+    }
+    __device__ __forceinline__ void add_one(float x) {
+        if (x > lim) refer(x);
+        add_guarded(x, s, t);
+    }
     // x: the chunk's logits (-inf: none), cmax: the largest of them
     __device__ __forceinline__ void add(const float (&x)[E], float cmax) {
-        if (cmax > lim) {
-            const Acc a = rebase(acc(), cmax, c);
-            ref = Ref(cmax, c);
-            lim = cmax + slack;
-            zero = ref.far ? NAN : 0.f;
-            const float f = __builtin_amdgcn_exp2f(ref.delta);
-            s = f * a.s;
-            t = f * fmaf(ref.delta, a.s, a.t);
-        }
+        if (cmax > lim) refer(cmax);
         float cs = zero, ct = zero;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -202,11 +205,7 @@ struct Sums {
         if (bad != bad) {
             cs = 0.f; ct = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float y = ref.y(x[e], c), p = x[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y);
-                cs += p;
-                ct += p == 0.f ? 0.f : p * y;
-            }
+            for (int e = 0; e < E; ++e) add_guarded(x[e], cs, ct);
         }
         s += cs;
         t += ct;
@@ -356,7 +355,7 @@ template <int TH> __device__ __forceinline__ void write_top(TopLds& lds, int n, 
 }
 
 template <typename T>
-__device__ __forceinline__ void write_row(const Row<T>& row, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
+__device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
                                           float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats) {
     stats[r * 2] = a.m;
     stats[r * 2 + 1] = a.s;
@@ -365,8 +364,8 @@ __device__ __forceinline__ void write_row(const Row<T>& row, int64_t r, const Ac
     if (tokens) {
         const int64_t t = tokens[r];
         float v = 0.f;
-        if (t >= row.V) v = NAN;
-        else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(row.z + t) - a.m) * inv_t - log_s;
+        if (t >= V) v = NAN;
+        else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(z + t) - a.m) * inv_t - log_s;
         logp[r] = v;
     }
 }
@@ -381,28 +380,26 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
     const Row<T> row(z + r * ld, V);
     const int tid = threadIdx.x;
     Sums<T, true> sums(c);
-    float slot[LG_SLOTS], ends = -INFINITY;
+    float slot[LG_SLOTS];
 #pragma unroll
     for (int i = 0; i < LG_SLOTS; ++i) slot[i] = -INFINITY;
-    // the first and the last chunk (threads 0 and 1) reach over the row's ends; their loads are the first in flight
-    const int last = row.n - 1;
-    const bool has_end = tid == 0 || (tid == 1 && last > 0);
-    uint4 end_v = make_uint4(0, 0, 0, 0);
-    if (has_end) end_v = row.load(tid ? last : 0);
-    for (int c0 = 1; c0 < last; c0 += LG_SLOTS * TH) {
+    const int n = row.full(), ei = row.end_index(tid);
+    // the next U chunks are on their way while U are added up (loads without a condition: behind the row's end its last chunk again)
+    uint4 v[U], w[U];
+    const auto fetch = [&](uint4 (&to)[U], int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) to[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
+    };
+    fetch(v, 0);
+    const float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
+    for (int i0 = 0; i0 < n; i0 += LG_SLOTS * TH) {
 #pragma unroll
         for (int i = 0; i < LG_SLOTS; i += U) {
-            if (c0 + i * TH >= last) break;
-            uint4 v[U];
+            if (i0 + i * TH >= n) break;
+            fetch(w, i0 + (i + U) * TH);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int ch = c0 + (i + u) * TH + tid;
-                if (ch < last) v[u] = row.inner(ch);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int ch = c0 + (i + u) * TH + tid;
-                if (ch < last) {
+                if (i0 + (i + u) * TH + tid < n) {
                     float x[E];
                     Chunk<T>::unpack(v[u], x);
                     const float cmax = max_of(x);
@@ -410,22 +407,19 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
                     sums.add(x, cmax);
                 }
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = w[u];
         }
     }
-    if (has_end) {
-        float x[E];
-        Chunk<T>::unpack(end_v, x);
-        ends = max_of(x);
-        sums.add(x, ends);
-    }
+    if (ei >= 0) sums.add_one(end);
     const Acc a = team_join<TH>(sums.acc(), c, red);
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (tid == 0) write_row(row, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (tid == 0) write_row(row.z, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
     if (!TOP) return;
     __shared__ TopLds lds;
     if (tid == 0) { lds.n_list = 0; lds.n_cand = 0; }
-    float mine = ends;
+    float mine = end;
 #pragma unroll
     for (int i = 0; i < LG_SLOTS; ++i) mine = fmaxf(mine, slot[i]);
     const uint32_t kth = wave_kth<(E == 8 ? 16 : 0)>(order_key(mine), (k + TH / 64 - 1) / (TH / 64));
@@ -437,29 +431,29 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
     const float bound = key_value(least);
     bool whole = a.s != a.s;   // a NaN or +inf in the row
     if (!whole) {
-        const auto again = [&](int ch) {
-            const int at = atomicAdd(&lds.n_list, 1);
-            if (at < LG_CAND) lds.list[at] = ch;
+        const auto candidate = [&](float x, int i) {
+            const int at = atomicAdd(&lds.n_cand, 1);
+            if (at < LG_CAND) lds.cand[at] = order_key(x, i);
         };
-        if (has_end && ends >= bound) again(tid ? last : 0);
 #pragma unroll
         for (int i = 0; i < LG_SLOTS; ++i)
             if (slot[i] >= bound)
-                for (int ch = 1 + i * TH + tid; ch < last; ch += LG_SLOTS * TH) again(ch);
+                for (int ch = i * TH + tid; ch < n; ch += LG_SLOTS * TH) {
+                    const int at = atomicAdd(&lds.n_list, 1);
+                    if (at < LG_CAND) lds.list[at] = ch;
+                }
+        if (ei >= 0 && end >= bound) candidate(end, ei);
         __syncthreads();
         const int n_list = lds.n_list;
         whole = n_list > LG_CAND;
         if (!whole) {
             for (int q = tid; q < n_list; q += TH) {
-                const int ch = lds.list[q], lo = ch * E - row.sh;
+                const int ch = row.first + lds.list[q], lo = ch * E - row.sh;
                 float x[E];
                 Chunk<T>::unpack(row.load(ch), x);
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    if (x[e] >= bound && lo + e >= 0 && lo + e < V) {
-                        const int at = atomicAdd(&lds.n_cand, 1);
-                        if (at < LG_CAND) lds.cand[at] = order_key(x[e], lo + e);
-                    }
+                    if (x[e] >= bound) candidate(x[e], lo + e);
             }
             __syncthreads();
             whole = lds.n_cand > LG_CAND;
@@ -473,37 +467,55 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
 // Rows of up to 64 (W = 16 lanes a row) or 2041 / 2045 logits (W = 64): the whole row lives in registers, the maximum is found first.
 template <typename T, int W> struct Small;
 template <typename T> struct Small<T, 16> {   // element j of a lane: lane + 16 j
-    static constexpr int NE = 4, G = 1;
+    static constexpr int NE = 4;
     static __host__ __device__ constexpr int max_v() { return 16 * NE; }
     const T* z;
     int V, lane;
     __device__ __forceinline__ Small(const T* p, int v, int l) : z(p), V(v), lane(l) {}
     __device__ __forceinline__ int index(int j) const { return lane + 16 * j; }
-    __device__ __forceinline__ int groups() const { return NE; }
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int j = 0; j < NE; ++j) f(j);
+    }
     __device__ __forceinline__ void load(float (&x)[NE]) const {
 #pragma unroll
         for (int j = 0; j < NE; ++j) x[j] = index(j) < V ? Store<T>::load(z + index(j)) : -INFINITY;
     }
 };
-template <typename T> struct Small<T, 64> {   // chunks of a lane: lane + 64 i
-    static constexpr int E = Chunk<T>::E, NE = 32, G = E, NC = NE / E;
-    static __host__ __device__ constexpr int max_v() { return 64 * NE - E + 1; }
+template <typename T> struct Small<T, 64> {   // chunks of a lane: lane + 64 i, and (element NE - 1) one of the row's ends
+    static constexpr int E = Chunk<T>::E, NE = 32 + 1, NC = 32 / E;
+    static __host__ __device__ constexpr int max_v() { return 64 * 32; }
     Row<T> row;
-    int V, lane;
-    __device__ __forceinline__ Small(const T* p, int v, int l) : row(p, v), V(v), lane(l) {}
-    __device__ __forceinline__ int index(int j) const { return ((j / E) * 64 + lane) * E + j % E - row.sh; }
-    __device__ __forceinline__ int groups() const { return (row.n + 63) / 64; }
+    int V, lane, end;
+    __device__ __forceinline__ Small(const T* p, int v, int l) : row(p, v), V(v), lane(l) { end = row.end_index(l); }
+    // the place of element j in the row; of a place the row does not have: -1 or at least V
+    __device__ __forceinline__ int index(int j) const { return j == NE - 1 ? end : row_index((j / E) * 64 + lane, j % E); }
+    __device__ __forceinline__ int row_index(int i, int e) const { return i < row.full() ? (row.first + i) * E + e - row.sh : V; }
+    // f(j) for the lane's elements, chunk rounds that the row does not reach left out
+    template <typename F> __device__ __forceinline__ void each_chunk(F f) const {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (i * 64 >= row.full()) break;
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(i * E + e);
+        }
+    }
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        each_chunk(f);
+        f(NE - 1);
+    }
     __device__ __forceinline__ void load(float (&x)[NE]) const {
+        const int n = row.full();
         uint4 v[NC];
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (i * 64 + lane < row.n) v[i] = row.load(i * 64 + lane);
+        for (int i = 0; i < NC; ++i) v[i] = row.load(row.first + min(i * 64 + lane, n - 1));   // (more than 64 logits: n > 0)
+        x[NE - 1] = end >= 0 ? Store<T>::load(row.z + end) : -INFINITY;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float y[E];
             Chunk<T>::unpack(v[i], y);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[i * E + e] = i * 64 + lane < row.n ? y[e] : -INFINITY;
+            for (int e = 0; e < E; ++e) x[i * E + e] = i * 64 + lane < n ? y[e] : -INFINITY;
         }
     }
 };
@@ -514,7 +526,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
                                                              float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats,
                                                              int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
     using S = Small<T, W>;
-    constexpr int NE = S::NE, G = S::G, CAP = W == 16 ? 64 : 256;
+    constexpr int NE = S::NE, CAP = W == 16 ? 64 : 256;
     const int lane = threadIdx.x & (W - 1), team = threadIdx.x / W;
     const int64_t r = (int64_t)blockIdx.x * (256 / W) + team;
     if (r >= N) return;
@@ -522,105 +534,88 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
     const S row(zr, V, lane);
     float x[NE];
     row.load(x);
-    float m = x[0];
+    float m = LG_NEG;
 #pragma unroll
-    for (int j = 1; j < NE; ++j) m = fmaxf(m, x[j]);
-    m = fmaxf(lanes_join<W>(m, Max()), LG_NEG);
+    for (int j = 0; j < NE; ++j) m = fmaxf(m, x[j]);
+    m = lanes_join<W>(m, Max());
     Acc a = {m, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NE / G; ++g) {
-        if (g >= row.groups()) break;
-#pragma unroll
-        for (int j = g * G; j < g * G + G; ++j) {
-            const float y = (x[j] - m) * c, p = __builtin_amdgcn_exp2f(y);
-            const bool none = x[j] == -INFINITY;      // (m may be the type's lowest value: y = -inf, or NaN where m is +inf)
-            a.s += none ? 0.f : p;
-            a.t += p == 0.f || none ? 0.f : p * y;
-        }
-    }
+    row.each([&](int j) {
+        const float y = (x[j] - m) * c, p = x[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y);   // (m may be the type's lowest value)
+        a.s += p;
+        a.t += p == 0.f ? 0.f : p * y;
+    });
     a.s = lanes_join<W>(a.s, Add());
     a.t = lanes_join<W>(a.t, Add());
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (lane == 0) {
-        stats[r * 2] = a.m;
-        stats[r * 2 + 1] = a.s;
-        lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
-        entropy[r] = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
-        if (tokens) {
-            const int64_t t = tokens[r];
-            float v = 0.f;
-            if (t >= V) v = NAN;
-            else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(zr + t) - a.m) * inv_t - log_s;
-            logp[r] = v;
-        }
-    }
+    if (lane == 0) write_row(zr, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
     if (!TOP) return;
     __shared__ unsigned long long cand_lds[256 / W][CAP];
     unsigned long long* cand = cand_lds[team];
+    const auto packed = [&](uint32_t key, int i) { return ((unsigned long long)key << 32) | (0xFFFFFFFFu - (uint32_t)i); };
     int n;
-    if (W == 16) {   // every logit is a candidate
+    if constexpr (W == 16) {   // every logit is a candidate
         n = V;
-#pragma unroll
-        for (int j = 0; j < NE; ++j)
+        row.each([&](int j) {
             if (row.index(j) < V) cand[row.index(j)] = order_key(x[j], row.index(j));
+        });
     } else {
         // the k-th largest key from the top bit down, until at most `most` keys reach it (then those are the candidates) or it is exact
-        const auto valid = [&](int j) { return row.index(j) >= 0 && row.index(j) < V; };
         uint32_t key[NE];
 #pragma unroll
-        for (int j = 0; j < NE; ++j) key[j] = valid(j) ? order_key(x[j]) : 0u;
-        const int most = min(CAP, k + max(8, k >> 2)), ng = row.groups();
+        for (int j = 0; j < NE; ++j) key[j] = row.index(j) >= 0 && row.index(j) < V ? order_key(x[j]) : 0u;
+        const int most = min(CAP, k + max(8, k >> 2));
         uint32_t at = 0;
         n = V;
         for (int b = 31; b >= 0 && n > most; --b) {
             const uint32_t t = at | (1u << b);
             int cnt = 0;
-#pragma unroll
-            for (int g = 0; g < NE / G; ++g) {
-                if (g >= ng) break;
-#pragma unroll
-                for (int j = g * G; j < g * G + G; ++j) cnt += __popcll(__ballot(key[j] >= t));
-            }
+            row.each([&](int j) { cnt += __popcll(__ballot(key[j] >= t)); });
             if (cnt >= k) { at = t; n = cnt; }
         }
-        const uint32_t above = n <= CAP ? (at ? at - 1u : 0u) : at;   // (at = 0: every valid key, they are at least 1)
+        const uint32_t above = n <= CAP ? (at ? at - 1u : 0u) : at;   // (at = 0: every key of the row, they are at least 1)
         const unsigned long long lt = (1ull << lane) - 1ull;
-        int n_out = 0;
+        int out = 0;
+        row.each([&](int j) {
+            const unsigned long long on = __ballot(key[j] > above);
+            if (key[j] > above) cand[out + __popcll(on & lt)] = packed(key[j], row.index(j));
+            out += __popcll(on);
+        });
+        if (n > CAP) {   // many logits equal the k-th: the first of them in the row's order (its head, rounds of chunks by lane and element, its tail)
+            int left = k - out;
+            const auto take = [&](uint32_t q, int i, bool head) {
+                const bool mine = q == at && (lane < Chunk<T>::E) == head;
+                const unsigned long long on = __ballot(mine);
+                const int before = __popcll(on & lt);
+                if (mine && before < left) cand[out + before] = packed(q, i);
+                const int took = max(0, min(__popcll(on), left));
+                out += took;
+                left -= took;
+            };
+            take(key[NE - 1], row.index(NE - 1), true);
 #pragma unroll
-        for (int g = 0; g < NE / G; ++g) {
-            if (g >= ng) break;
-#pragma unroll
-            for (int j = g * G; j < g * G + G; ++j) {
-                const unsigned long long on = __ballot(key[j] > above);
-                if (key[j] > above) cand[n_out + __popcll(on & lt)] = ((unsigned long long)key[j] << 32) | (0xFFFFFFFFu - (uint32_t)row.index(j));
-                n_out += __popcll(on);
-            }
-        }
-        if (n > CAP) {   // many logits equal the k-th: the first of them in the row's order (rounds of chunks, lanes, elements)
-            int left = k - n_out;
-#pragma unroll
-            for (int g = 0; g < NE / G; ++g) {
-                if (g >= ng || left <= 0) break;
+            for (int i = 0; i < S::NC; ++i) {
+                if (left <= 0) break;
                 int before = 0, total = 0;
 #pragma unroll
-                for (int j = g * G; j < g * G + G; ++j) {
+                for (int j = i * S::E; j < i * S::E + S::E; ++j) {
                     const unsigned long long on = __ballot(key[j] == at);
                     before += __popcll(on & lt);
                     total += __popcll(on);
                 }
 #pragma unroll
-                for (int j = g * G; j < g * G + G; ++j)
+                for (int j = i * S::E; j < i * S::E + S::E; ++j)
                     if (key[j] == at) {
-                        if (before < left) cand[n_out + before] = ((unsigned long long)key[j] << 32) | (0xFFFFFFFFu - (uint32_t)row.index(j));
+                        if (before < left) cand[out + before] = packed(key[j], row.index(j));
                         ++before;
                     }
                 const int took = min(total, left);
-                n_out += took;
+                out += took;
                 left -= took;
             }
+            if (left > 0) take(key[NE - 1], row.index(NE - 1), false);
         }
-        n = n_out;
+        n = out;
     }
     Team<W>::sync();
     for (int q = lane; q < n; q += W) {
@@ -639,6 +634,27 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // exponent), and a few places (the given token, the listed ones) where something is added: those are written again once the row is done.
 // One read and one write of the row; a lane has U chunks in flight.
 
+// f(chunk, its 16 bytes) for the chunks inside the row, U of a lane at once (loads without a condition, so that all are in flight together:
+// behind the row's end its last chunk again)
+template <typename T, int TH, int U, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, F f) {
+    const int tid = Team<TH>::rank(), n = row.full();
+    for (int i0 = 0; i0 < n; i0 += U * TH) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * TH + tid < n) f(row.first + i0 + u * TH + tid, v[u]);
+    }
+}
+template <typename T, int TH> __device__ __forceinline__ void zero_row(const Row<T>& row, T* d) {
+    constexpr int E = Chunk<T>::E;
+    const float x[E] = {};
+    const int tid = Team<TH>::rank(), ei = row.end_index(tid);
+    if (ei >= 0) Store<T>::store(d + ei, 0.f);
+    for (int i = tid; i < row.full(); i += TH) row.store(d, row.first + i, x);
+}
+
 // dz_i = inv_t [ p_i (A + B ln p_i) + g_t 1[i = t] + sum_j g_j 1[i = id_j] ],  A = g_lse - g_t - sum_j g_j - g_H H,  B = -g_H
 struct LogprobsGrad {
     const float *stats, *entropy, *g_logp, *g_entropy, *g_lse, *g_top;
@@ -648,7 +664,7 @@ struct LogprobsGrad {
 template <typename T, int TH>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t, LogprobsGrad q,
                                                                            T* __restrict__ dz, int64_t ldd) {
-    constexpr int E = Chunk<T>::E, U = 4, PER = TH < 256 ? 256 / TH : 1;
+    constexpr int E = Chunk<T>::E, U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1;
     __shared__ float red[TH < 64 ? 1 : TH / 64];
     const int64_t r = (int64_t)blockIdx.x * PER + (PER > 1 ? threadIdx.x / TH : 0);
     if (PER > 1 && r >= N) return;
@@ -671,21 +687,15 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
         const float y = fmaxf(ref.y(x, c), -200.f);   // (a masked logit: e = 0, whatever c1 is)
         return __builtin_amdgcn_exp2f(y) * fmaf(c1, y, c0);
     };
-    for (int ch0 = tid; ch0 < row.n; ch0 += U * TH) {
-        uint4 v[U];
+    const int ei = row.end_index(tid);
+    if (ei >= 0) Store<T>::store(d + ei, one(Store<T>::load(row.z + ei)));
+    each_chunk<T, TH, U>(row, [&](int ch, const uint4& v) {
+        float x[E];
+        Chunk<T>::unpack(v, x);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (ch0 + u * TH < row.n) v[u] = row.load(ch0 + u * TH);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (ch0 + u * TH < row.n) {
-                float x[E];
-                Chunk<T>::unpack(v[u], x);
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = one(x[e]);
-                row.store(d, ch0 + u * TH, x);
-            }
-    }
+        for (int e = 0; e < E; ++e) x[e] = one(x[e]);
+        row.store(d, ch, x);
+    });
     if (empty) return;
     Team<TH>::sync();
     // (top ids are distinct; the given token may be one of them)
@@ -725,56 +735,59 @@ template <int TH> struct ListLds {
 
 struct Teacher { float Q, rest, qlogq; };
 
-template <int TH, bool TAIL>
-__device__ __forceinline__ Teacher read_list(const Distill& p, int64_t r, int V, int* sid, float* sq, float* red) {
-    constexpr int J = (AG_LOGITS_MAX_TOP + TH - 1) / TH;
-    const int tid = Team<TH>::rank();
+// the list of a row: loaded (before the row's own loads, so that those stay in flight while the list is worked on), then put into LDS
+template <int TH> struct List {
+    static constexpr int J = (AG_LOGITS_MAX_TOP + TH - 1) / TH;
     float lp[J];
-    float m = -INFINITY;
+    int id[J];
+    __device__ __forceinline__ void load(const Distill& p, int64_t r, int V) {
 #pragma unroll
-    for (int i = 0; i < J; ++i) {
-        const int j = tid + i * TH;
-        lp[i] = -INFINITY;
-        if (j >= p.K) continue;
-        const int64_t id = p.ids[r * p.K + j];
-        const float v = p.dtype == AG_BF16 ? bf16_to_f32(((const bf16_t*)p.logp)[r * p.K + j]) : ((const float*)p.logp)[r * p.K + j];
-        sid[j] = id < 0 ? -1 : id >= V ? V : (int)id;
-        lp[i] = id < 0 ? -INFINITY : id >= V ? NAN : v;
-        m = fmaxf(m, lp[i]);
+        for (int i = 0; i < J; ++i) {
+            const int j = min(Team<TH>::rank() + i * TH, p.K - 1);
+            const int64_t t = p.ids[r * p.K + j];
+            const float v = p.dtype == AG_BF16 ? bf16_to_f32(((const bf16_t*)p.logp)[r * p.K + j]) : ((const float*)p.logp)[r * p.K + j];
+            id[i] = t < 0 ? -1 : t >= V ? V : (int)t;
+            lp[i] = t < 0 || Team<TH>::rank() + i * TH >= p.K ? -INFINITY : t >= V ? NAN : v;
+        }
     }
-    m = Team<TH>::max(m, red);
-    if (!TAIL) {
-        float s = 0.f;
+    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int* sid, float* sq, float* red) {
+        const int tid = Team<TH>::rank();
+        float m = lp[0];
 #pragma unroll
-        for (int i = 0; i < J; ++i) s += lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
-        s = Team<TH>::sum(s, red);
-        const float ls = logf(s);
+        for (int i = 1; i < J; ++i) m = fmaxf(m, lp[i]);
+        m = Team<TH>::max(m, red);
+        if (!TAIL) {
+            float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < J; ++i) lp[i] = s == 0.f ? -INFINITY : (lp[i] - m) - ls;
-    }
-    Teacher t = {0.f, 0.f, 0.f};
-    float others = 0.f;   // the masses that are not the largest
-    int top = 0;          // slots that have the largest
+            for (int i = 0; i < J; ++i) s += lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
+            s = Team<TH>::sum(s, red);
+            const float ls = logf(s);
 #pragma unroll
-    for (int i = 0; i < J; ++i) {
-        const int j = tid + i * TH;
-        const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
-        if (j < p.K) sq[j] = q;
-        t.Q += q;
-        t.qlogq += q == 0.f ? 0.f : q * lp[i];
-        if (TAIL) { if (lp[i] == m) ++top; else others += q; }
+            for (int i = 0; i < J; ++i) lp[i] = s == 0.f ? -INFINITY : (lp[i] - m) - ls;
+        }
+        Teacher t = {0.f, 0.f, 0.f};
+        float others = 0.f, top = 0.f;   // the masses that are not the largest, and how many are
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+            const int j = tid + i * TH;
+            const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
+            if (j < p.K) { sid[j] = id[i]; sq[j] = q; }
+            t.Q += q;
+            t.qlogq += q == 0.f ? 0.f : q * lp[i];
+            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q; }
+        }
+        t.Q = Team<TH>::sum(t.Q, red);
+        t.qlogq = Team<TH>::sum(t.qlogq, red);
+        if (TAIL) {
+            // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
+            top = Team<TH>::sum(top, red);
+            others = Team<TH>::sum(others, red);
+            t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (top - 1.f) * expf(m) - others, 0.f);
+            if (t.Q != t.Q) t.rest = t.Q;
+        }
+        return t;
     }
-    t.Q = Team<TH>::sum(t.Q, red);
-    t.qlogq = Team<TH>::sum(t.qlogq, red);
-    if (TAIL) {
-        // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
-        const float n_top = Team<TH>::sum((float)top, red);
-        others = Team<TH>::sum(others, red);
-        t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (n_top - 1.f) * expf(m) - others, 0.f);
-        if (t.Q != t.Q) t.rest = t.Q;
-    }
-    return t;
-}
+};
 
 // what a row's gradient takes from the forward pass: g a exp2((z - m_off) c) off the list, g (on exp2((z - m) c) - q) on it
 struct GradOf { float m_off, a, m, on; };
@@ -796,20 +809,15 @@ template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T
     float x[E];
     Chunk<T>::unpack(v, x);
     if (!ref.far) {
+        const float gd = ga * __builtin_amdgcn_exp2f(-ref.delta);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = ga * __builtin_amdgcn_exp2f(fmaf(x[e], c, ref.nr));
+        for (int e = 0; e < E; ++e) x[e] = gd * __builtin_amdgcn_exp2f(fmaf(x[e], c, ref.nr));
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = ga * exp2_from(x[e], ref.m, c);
     }
     row.store(d, ch, x);
 }
-template <typename T, int TH> __device__ __forceinline__ void zero_row(const Row<T>& row, T* d) {
-    constexpr int E = Chunk<T>::E;
-    const float x[E] = {};
-    for (int ch = Team<TH>::rank(); ch < row.n; ch += TH) row.store(d, ch, x);
-}
-
 // words of LDS for a bit per logit of a row's chunks, whatever its alignment
 template <typename T> __host__ __device__ constexpr int bit_words(int V) { return (V + Chunk<T>::E - 1 + 31) / 32 + 1; }
 
@@ -827,6 +835,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
     const int64_t r = (int64_t)blockIdx.x * PER + team;
     if (PER > 1 && r >= N) return;
     const Row<T> row(z + r * ld, V);
+    const int n = row.full(), ei = row.end_index(tid);
     T* d = dz + r * ldd;
     const float w = p.weights ? p.weights[r] : p.weight0;
     if (w == 0.f) {   // the row takes no part
@@ -835,17 +844,23 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
         if (GRAD) zero_row<T, TH>(row, d);
         return;
     }
+    List<TH> mine;
+    mine.load(p, r, V);
+    const float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
     uint4 v[NC];
+    const auto fetch = [&](int i0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-        if (i * TH + tid < row.n) v[i] = row.load(i * TH + tid);
+        for (int i = 0; i < NC; ++i) v[i] = row.load(row.first + max(min(i0 + i * TH + tid, n - 1), 0));
+    };
+    if (n > 0) fetch(0);
     int* sid = list.id[team];
     float* sq = list.q[team];
-    Teacher tc = read_list<TH, TAIL>(p, r, V, sid, sq, red);
-    uint32_t* bits = bits_lds + (TAIL ? team * bit_words<T>(V) : 0);
+    Teacher tc = mine.template finish<TAIL>(p, sid, sq, red);
+    uint32_t* bits = bits_lds + (TAIL ? team * bit_words<T>(V) : 0);   // logit i: bit i + sh
+    if (TAIL)
+        for (int i = tid; i < bit_words<T>(V); i += TH) bits[i] = 0u;
+    Team<TH>::sync();
     if (TAIL) {
-        for (int i = tid; i < (row.n + BITS - 1) / BITS; i += TH) bits[i] = 0u;
-        Team<TH>::sync();
         float fresh = 0.f;
         for (int j = tid; j < p.K; j += TH) {
             if (sid[j] < 0 || sid[j] >= V) continue;
@@ -855,20 +870,18 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
         }
         if ((int)Team<TH>::sum(fresh, red) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
         Team<TH>::sync();
-    } else {
-        Team<TH>::sync();
     }
     Sums<T, false> sums(c);
-    for (int c0 = 0;;) {
+    for (int i0 = 0; i0 < n;) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int ch = c0 + i * TH + tid;
-            if (ch < row.n) {
+            if (i0 + i * TH + tid < n) {
+                const int ch = row.first + i0 + i * TH + tid;
                 float y[E];
                 Chunk<T>::unpack(v[i], y);
                 if (TAIL) {
-                    const uint32_t b = bits[ch / BITS] >> ((ch % BITS) * E);
-                    if (b & ((1u << E) - 1u)) {
+                    const uint32_t b = (bits[ch / BITS] >> ((ch % BITS) * E)) & ((1u << E) - 1u);
+                    if (b) {
 #pragma unroll
                         for (int e = 0; e < E; ++e)
                             if ((b >> e) & 1u) y[e] = -INFINITY;
@@ -877,21 +890,18 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
                 sums.add(y, max_of(y));
             }
         }
-        if (c0 + NC * TH >= row.n) break;
-        c0 += NC * TH;
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (c0 + i * TH + tid < row.n) v[i] = row.load(c0 + i * TH + tid);
+        i0 += NC * TH;
+        if (i0 < n) fetch(i0);
     }
+    if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(end);
     const Acc off = team_join<TH>(sums.acc(), c, red);
     // the listed tokens' logits: their part of the sums (with the tail), and of the loss
     Acc all = off;
-    float cross = 0.f, lm = LG_NEG;
-    for (int j = tid; j < p.K; j += TH)
-        if (sid[j] >= 0 && sid[j] < V) lm = fmaxf(lm, Store<T>::load(row.z + sid[j]));
     if (TAIL) {
+        float lm = LG_NEG, s = 0.f;
+        for (int j = tid; j < p.K; j += TH)
+            if (sid[j] >= 0 && sid[j] < V) lm = fmaxf(lm, Store<T>::load(row.z + sid[j]));
         all = rebase(off, fmaxf(off.m, Team<TH>::max(lm, red)), c);
-        float s = 0.f;
         for (int j = tid; j < p.K; j += TH) {
             if (sid[j] < 0 || sid[j] >= V) continue;
             bool first = true;
@@ -902,6 +912,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
     }
     const bool empty = all.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(all.s);
+    float cross = 0.f;
     for (int j = tid; j < p.K; j += TH) {
         const float q = sq[j];
         if (q == 0.f) continue;
@@ -922,15 +933,14 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* _
     if (!GRAD) return;
     if (empty) { zero_row<T, TH>(row, d); return; }
     const Ref ref(s.m_off, c);
-    const float g = tau * w, ga = g * s.a * __builtin_amdgcn_exp2f(-ref.delta);
-    for (int c0 = (row.n - 1) / (NC * TH) * (NC * TH);;) {   // the last round's chunks are still here
+    const float g = tau * w, ga = g * s.a;
+    if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(end, ref.m, c));
+    for (int i0 = (n - 1) / (NC * TH) * (NC * TH); i0 >= 0 && n > 0;) {   // the last round's chunks are still here
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-            if (c0 + i * TH + tid < row.n) gradient_chunk(row, c0 + i * TH + tid, v[i], c, ref, ga, d);
-        c0 -= NC * TH;
-        if (c0 < 0) break;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) v[i] = row.load(c0 + i * TH + tid);
+            if (i0 + i * TH + tid < n) gradient_chunk(row, row.first + i0 + i * TH + tid, v[i], c, ref, ga, d);
+        i0 -= NC * TH;
+        if (i0 >= 0) fetch(i0);
     }
     Team<TH>::sync();
     listed_gradients<T, TH>(row, sid, sq, p.K, s, g, c, d);
@@ -940,7 +950,7 @@ template <typename T, int TH, bool TAIL>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                                                                           const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
-    constexpr int U = 4, PER = TH < 256 ? 256 / TH : 1;
+    constexpr int U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1;
     __shared__ float red[TH < 64 ? 1 : TH / 64];
     __shared__ ListLds<TH> list;
     const int team = PER > 1 ? threadIdx.x / TH : 0, tid = Team<TH>::rank();
@@ -955,19 +965,15 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
         zero_row<T, TH>(row, d);
         return;
     }
+    List<TH> mine;
+    mine.load(p, r, V);
     const Ref ref(s.m_off, c);
     const float g = tau * (g_loss || g_row ? (g_loss ? w * g_loss[0] : 0.f) + (g_row ? g_row[r] : 0.f) : w);
-    const float ga = g * s.a * __builtin_amdgcn_exp2f(-ref.delta);
-    for (int ch0 = tid; ch0 < row.n; ch0 += U * TH) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (ch0 + u * TH < row.n) v[u] = row.load(ch0 + u * TH);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (ch0 + u * TH < row.n) gradient_chunk(row, ch0 + u * TH, v[u], c, ref, ga, d);
-    }
-    read_list<TH, TAIL>(p, r, V, list.id[team], list.q[team], red);
+    const float ga = g * s.a;
+    const int ei = row.end_index(tid);
+    if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
+    each_chunk<T, TH, U>(row, [&](int ch, const uint4& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
+    mine.template finish<TAIL>(p, list.id[team], list.q[team], red);
     Team<TH>::sync();
     listed_gradients<T, TH>(row, list.id[team], list.q[team], p.K, s, g, c, d);
 }
@@ -1065,7 +1071,7 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
             int64_t ldd, hipStream_t s) {
     constexpr int E = Chunk<T>::E;
 #define LG_CALL(TH)                                                                                                                                   \
-    constexpr int NC = TH == 16 ? (E == 8 ? 1 : 2) : TH == 64 ? (E == 8 ? 4 : 8) : GRAD ? 16 : 4;                                                     \
+    constexpr int NC = TH == 16 ? 64 / E / 16 + (E == 8) : TH == 64 ? 32 / E : GRAD ? 16 : 4;                                                          \
     const size_t lds = TAIL ? (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1) : 0;                                                                      \
     hipLaunchKernelGGL((distill_kernel<T, TH, NC, TAIL, GRAD>), team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), lds, s, (const T*)d_logits, ld, N, V,     \
                        temperature, log2e_over(temperature), one_over(temperature), p, d_row_loss, d_stats, (T*)d_dlogits, ldd)

@@ -24,6 +24,12 @@ template <> struct Chunk<float> {
     static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[4]) {
         x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
     }
+    static __device__ __forceinline__ float pick(const uint4& r, int e) {   // (selections, not an array in memory)
+        uint32_t a = r.x, b = r.y, c = r.z, d = r.w;
+        asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+        const uint32_t p = e & 1 ? b : a, q = e & 1 ? d : c;
+        return __uint_as_float(e & 2 ? q : p);
+    }
     static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
@@ -34,6 +40,12 @@ template <> struct Chunk<bf16_t> {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+    static __device__ __forceinline__ float pick(const uint4& r, int e) {
+        uint32_t a = r.x, b = r.y, c = r.z, d = r.w;
+        asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+        const uint32_t p = e & 2 ? b : a, q = e & 2 ? d : c, w = e & 4 ? q : p;
+        return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
     }
     static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
         return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
@@ -110,6 +122,10 @@ struct Team {
     }
     static __device__ __forceinline__ float sum(float v, float* red) { return join(v, Add(), red); }
     static __device__ __forceinline__ float max(float v, float* red) { return join(v, Max(), red); }
+};
+
+struct MaxBits {   // of the values' bits, as unsigned integers
+    __device__ __forceinline__ float operator()(float a, float b) const { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
 };
 
 struct Acc { float m, s, t; };   // reference (a logit), sum of exp2(y), sum of exp2(y) y,  y = (z - m) c,  c = log2(e) / temperature
@@ -242,37 +258,53 @@ __device__ __forceinline__ unsigned long long order_key(float x, int i) {
 // bound that at least k logits reach, and few others: the chunks of the slots that reach it (about two per alternative asked for) are read
 // again, their logits at or above the bound are the candidates, and every candidate's place is the number of candidates that beat it.
 // Rows with more candidates than fit (many equal logits) or a NaN take a radix selection over the whole row.
-constexpr int LG_SLOTS = 16, LG_CAND = 1024;
+constexpr int LG_SLOTS = 16;
 
-struct TopLds {
-    unsigned long long cand[LG_CAND];
-    int list[LG_CAND];      // chunks to read again; the radix selection's counters
-    int place[LG_CAND];
+template <int TH> struct TopLds {
+    static constexpr int CAP = TH == 64 ? 256 : 1024;
+    int list[CAP];          // slots to read again; the radix selection's counters
+    unsigned long long cand[CAP];
     uint32_t bound[16];
     int n_list, n_cand;
 };
 
-// count(keys of the wave >= result) >= j, from the top bit down; stops when it is j
-template <int LOW> __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int j) {
-    uint32_t r = 0;
-    for (int b = 31; b >= LOW; --b) {
-        const uint32_t t = r | (1u << b);
-        const int n = __popcll(__ballot(key >= t));
-        if (n < j) continue;
-        r = t;
-        if (n == j) break;
+// a key that at least j and (unless logits are equal) hardly more than j of the wave's G 64 values reach, by bisection between the least lane
+// maximum (or nothing) and the largest value.  SHIFT: low key bits that carry nothing (16 for bf16)
+template <int G, int SHIFT> __device__ __forceinline__ uint32_t wave_bound(const float (&v)[G], int j) {
+    float mine = v[0];
+#pragma unroll
+    for (int g = 1; g < G; ++g) mine = fmaxf(mine, v[g]);
+    const float most = lanes_join<64>(mine, Max());
+    uint32_t key[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) key[g] = order_key(v[g]) >> SHIFT;
+    uint32_t lo = j <= 64 ? order_key(-lanes_join<64>(-mine, Max())) >> SHIFT : 0u, hi = (order_key(most) >> SHIFT) + 1u;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    const int enough = j + (j >> 3) + (j > 4);
+    while (hi - lo > 1u) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        int n = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) n += __popcll(__ballot(key[g] >= mid));
+        if (n >= j) {
+            lo = mid;
+            if (n <= enough) break;
+        } else {
+            hi = mid;
+        }
     }
-    return r;
+    return lo << SHIFT;
 }
 
 // exact: the k-th largest key by radix (four digits of 8 bits over the row), then every larger logit and the first of the equal ones
-template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k, TopLds& lds) {
+template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k, TopLds<TH>& lds) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0;
     int left = k;                       // how many of the logits with the digits found so far are still wanted
     for (int d = 24; d >= 0; d -= 8) {
         for (int i = tid; i < 256; i += TH) lds.list[i] = 0;
-        __syncthreads();
+        Team<TH>::sync();
         for (int i = tid; i < row.V; i += TH) {
             const uint32_t key = order_key(Store<T>::load(row.z + i));
             if (d != 24 && (key >> (d + 8)) != prefix) continue;
@@ -285,7 +317,7 @@ template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k
                 atomicAdd(&lds.list[digit], 1);
             }
         }
-        __syncthreads();
+        Team<TH>::sync();
         int digit = 255, above = 0;
         for (; digit > 0; --digit) {                         // (every thread, the same broadcast reads)
             const int n = lds.list[digit];
@@ -294,11 +326,11 @@ template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k
         }
         left -= above;
         prefix = d == 24 ? (uint32_t)digit : (prefix << 8) | digit;
-        __syncthreads();
+        Team<TH>::sync();
     }
     // prefix is the k-th largest key; `left` of the logits equal to it belong to the top, the first ones
     if (tid == 0) { lds.n_cand = 0; lds.n_list = 0; }
-    __syncthreads();
+    Team<TH>::sync();
     for (int i0 = 0; i0 < row.V; i0 += TH) {
         const int i = i0 + tid;
         const uint32_t key = i < row.V ? order_key(Store<T>::load(row.z + i)) : 0u;
@@ -307,50 +339,114 @@ template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k
         const unsigned long long m = __ballot(eq);
         const int before = lds.n_list;                       // equal logits of the rounds so far
         if (before >= left) continue;                        // (uniform: all of them are found, only larger ones are still wanted)
-        __syncthreads();
-        if ((tid & 63) == 0) lds.place[tid >> 6] = __popcll(m);
-        __syncthreads();
+        Team<TH>::sync();
+        if ((tid & 63) == 0) lds.bound[tid >> 6] = __popcll(m);
+        Team<TH>::sync();
         int at = before;
-        for (int w = 0; w < (tid >> 6); ++w) at += lds.place[w];
+        for (int w = 0; w < (tid >> 6); ++w) at += (int)lds.bound[w];
         int total = before;
-        for (int w = 0; w < TH / 64; ++w) total += lds.place[w];
+        for (int w = 0; w < TH / 64; ++w) total += (int)lds.bound[w];
         at += __popcll(m & ((1ull << (tid & 63)) - 1ull));
         if (eq && at < left) lds.cand[atomicAdd(&lds.n_cand, 1)] = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (uint32_t)i);
-        __syncthreads();
+        Team<TH>::sync();
         if (tid == 0) lds.n_list = total;
-        __syncthreads();
+        Team<TH>::sync();
     }
-    __syncthreads();
+    Team<TH>::sync();
 }
 
-// candidates [0, n) of LDS (at least k, all different) -> their places; the first k are written
-template <int TH> __device__ __forceinline__ void write_top(TopLds& lds, int n, int k, const Acc& a, float inv_t, float log_s, bool empty,
-                                                            int64_t* __restrict__ ids, float* __restrict__ logp) {
-    const int tid = threadIdx.x;
-    // P threads share a candidate, each compares it with a part of the others
-    int cap = 64;
-    while (cap < n) cap <<= 1;
-    const int P = cap < TH ? TH / cap : 1, q0 = tid & (cap - 1), part = cap < TH ? tid / cap : 0;
-    if (P > 1) {
-        for (int i = tid; i < n; i += TH) lds.place[i] = 0;
-        __syncthreads();
+struct TopOut {
+    int64_t* ids;
+    float* logp;
+    int k;
+    float m, inv_t, log_s;
+    bool empty;
+    __device__ __forceinline__ void write(unsigned long long me, int place) const {
+        if (place >= k) return;
+        ids[place] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
+        logp[place] = empty ? -INFINITY : (key_value((uint32_t)(me >> 32)) - m) * inv_t - log_s;
     }
-    for (int q = cap < TH ? q0 : tid; q < n; q += cap < TH ? cap : TH) {
-        const unsigned long long me = lds.cand[q];
-        int r = 0;
-        const int lo = (int)((int64_t)n * part / P), hi = (int)((int64_t)n * (part + 1) / P);
-        for (int j = lo; j < hi; ++j) r += lds.cand[j] > me;
-        if (P > 1) atomicAdd(&lds.place[q], r);
-        else lds.place[q] = r;
+};
+
+// the value of lane ^ J
+template <int J> __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
+    else if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
+    else if constexpr (J < 32) return __builtin_amdgcn_ds_swizzle(v, (J << 10) | 0x1F);
+    else return __shfl_xor(v, J, 64);
+}
+template <int J> __device__ __forceinline__ unsigned long long lane_xor(unsigned long long v) {
+    return ((unsigned long long)lane_xor<J>((uint32_t)(v >> 32)) << 32) | lane_xor<J>((uint32_t)v);
+}
+// One wave sorts 64 R different keys in descending order, key 64 i + lane in q[i]: a bitonic network, step (S, J) compares keys J apart in
+// runs of S.  64 keys of 32 bits: 21 steps of one exchange, one comparison and one selection.
+template <int R, int S, int J, typename K> __device__ __forceinline__ void sort_steps(K (&q)[R]) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (J >= 64) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (i & (J / 64)) continue;
+            const K a = q[i], b = q[i | (J / 64)];
+            const bool swap = (a < b) == !((i * 64) & S);
+            q[i] = swap ? b : a;
+            q[i | (J / 64)] = swap ? a : b;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const K other = lane_xor<J>(q[i]);
+            const bool down = S < 64 ? !(lane & S) : !((i * 64) & S), larger = !(lane & J) == down;
+            q[i] = (other > q[i]) == larger ? other : q[i];
+        }
     }
-    __syncthreads();
-    for (int q = tid; q < n; q += TH) {
-        const int r = lds.place[q];
-        if (r >= k) continue;
+    if constexpr (J > 1) sort_steps<R, S, J / 2>(q);
+    else if constexpr (S < 64 * R) sort_steps<R, 2 * S, S>(q);
+}
+
+// One wave, candidates [0, n) of LDS with k <= n <= 256, all different -> the first k of them in order.  A bf16 candidate's 16 value and (up
+// to 65536 logits) 16 index bits are one 32-bit key.
+template <typename T, int R> __device__ __forceinline__ void place_sorted(const unsigned long long* cand, int n, int V, const TopOut& out) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long c[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) c[i] = lane + 64 * i < n ? cand[lane + 64 * i] : (unsigned long long)(uint32_t)(lane + 64 * i);   // (below every candidate)
+    if (Chunk<T>::E == 8 && V <= 65536) {
+        uint32_t q[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) q[i] = ((uint32_t)(c[i] >> 32) & 0xFFFF0000u) | ((uint32_t)c[i] & 0xFFFFu);
+        sort_steps<R, 2, 1>(q);
+        // (the low key bits that were dropped: 0 of a positive bf16 logit, ones of a negative one and of a NaN's key)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (lane + 64 * i < out.k) {
+                const uint32_t hi = q[i] & 0xFFFF0000u, full = hi & 0x80000000u && hi != 0xFFFF0000u ? hi : hi | 0xFFFFu;
+                out.write(((unsigned long long)full << 32) | 0xFFFF0000u | (q[i] & 0xFFFFu), lane + 64 * i);
+            }
+    } else {
+        sort_steps<R, 2, 1>(c);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (lane + 64 * i < out.k) out.write(c[i], lane + 64 * i);
+    }
+}
+template <typename T> __device__ __forceinline__ void place_wave(const unsigned long long* cand, int n, int V, const TopOut& out) {
+    if (n <= 64) place_sorted<T, 1>(cand, n, V, out);
+    else if (n <= 128) place_sorted<T, 2>(cand, n, V, out);
+    else place_sorted<T, 4>(cand, n, V, out);
+}
+
+// A workgroup's candidates: by its first wave, or where there are more than 256 by all threads
+template <typename T, int TH> __device__ __forceinline__ void place_all(TopLds<TH>& lds, int n, int V, const TopOut& out) {
+    if (n <= 256) {
+        if (threadIdx.x < 64) place_wave<T>(lds.cand, n, V, out);
+        return;
+    }
+    for (int q = threadIdx.x; q < n; q += TH) {
         const unsigned long long me = lds.cand[q];
-        const float x = key_value((uint32_t)(me >> 32));
-        ids[r] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
-        logp[r] = empty ? -INFINITY : (x - a.m) * inv_t - log_s;
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += lds.cand[j] > me;
+        out.write(me, place);
     }
 }
 
@@ -370,11 +466,29 @@ __device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_
     }
 }
 
+#ifndef LG_DB
+#define LG_DB 1
+#endif
+#ifndef LG_B0
+#define LG_B0 32
+#endif
+#ifndef LG_U
+#define LG_U 2
+#endif
+#ifndef LG_MINW
+#define LG_MINW 7
+#endif
+#ifndef LG_B1
+#define LG_B1 32
+#endif
+#ifndef LG_B2
+#define LG_B2 64
+#endif
 template <typename T, int TH, bool TOP>
-__global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
+__global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                          int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
                                                          float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
-    constexpr int E = Chunk<T>::E, U = 4;   // U chunks of a lane are in flight
+    constexpr int E = Chunk<T>::E, U = LG_U;   // U chunks of a lane are in flight
     __shared__ float red[3 * (TH / 64)];
     const int64_t r = blockIdx.x;
     const Row<T> row(z + r * ld, V);
@@ -390,13 +504,19 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
 #pragma unroll
         for (int u = 0; u < U; ++u) to[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
     };
+#if LG_DB
     fetch(v, 0);
+#endif
     const float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
     for (int i0 = 0; i0 < n; i0 += LG_SLOTS * TH) {
 #pragma unroll
         for (int i = 0; i < LG_SLOTS; i += U) {
             if (i0 + i * TH >= n) break;
+#if LG_DB
             fetch(w, i0 + (i + U) * TH);
+#else
+            fetch(v, i0 + i * TH);
+#endif
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (i0 + (i + u) * TH + tid < n) {
@@ -407,8 +527,10 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
                     sums.add(x, cmax);
                 }
             }
+#if LG_DB
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u] = w[u];
+#endif
         }
     }
     if (ei >= 0) sums.add_one(end);
@@ -417,51 +539,78 @@ __global__ __launch_bounds__(TH) void logprobs_wg_kernel(const T* __restrict__ z
     const float log_s = empty ? -INFINITY : logf(a.s);
     if (tid == 0) write_row(row.z, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
     if (!TOP) return;
-    __shared__ TopLds lds;
+    __shared__ TopLds<TH> lds;
+    constexpr int CAP = TopLds<TH>::CAP;
     if (tid == 0) { lds.n_list = 0; lds.n_cand = 0; }
-    float mine = end;
+    uint32_t least;
+    if constexpr (TH == 64) {
+        float group[4];
 #pragma unroll
-    for (int i = 0; i < LG_SLOTS; ++i) mine = fmaxf(mine, slot[i]);
-    const uint32_t kth = wave_kth<(E == 8 ? 16 : 0)>(order_key(mine), (k + TH / 64 - 1) / (TH / 64));
-    if ((tid & 63) == 0) lds.bound[tid >> 6] = kth;
-    __syncthreads();
-    uint32_t least = lds.bound[0];
+        for (int g = 0; g < 4; ++g) group[g] = g ? -INFINITY : end;
 #pragma unroll
-    for (int w = 1; w < TH / 64; ++w) least = min(least, lds.bound[w]);
+        for (int i = 0; i < LG_SLOTS; ++i) group[i & 3] = fmaxf(group[i & 3], slot[i]);
+        least = wave_bound<4, E == 8 ? 16 : 0>(group, k);
+    } else {
+        float mine[1] = {end};
+#pragma unroll
+        for (int i = 0; i < LG_SLOTS; ++i) mine[0] = fmaxf(mine[0], slot[i]);
+        const uint32_t b = wave_bound<1, E == 8 ? 16 : 0>(mine, (k + TH / 64 - 1) / (TH / 64));
+        if ((tid & 63) == 0) lds.bound[tid >> 6] = b;
+        __syncthreads();
+        least = lds.bound[0];
+#pragma unroll
+        for (int w = 1; w < TH / 64; ++w) least = min(least, lds.bound[w]);
+    }
     const float bound = key_value(least);
     bool whole = a.s != a.s;   // a NaN or +inf in the row
     if (!whole) {
-        const auto candidate = [&](float x, int i) {
-            const int at = atomicAdd(&lds.n_cand, 1);
-            if (at < LG_CAND) lds.cand[at] = order_key(x, i);
-        };
+        // (one addition to a counter per lane: its latency is what this part is made of)
+        uint32_t which = 0;
 #pragma unroll
-        for (int i = 0; i < LG_SLOTS; ++i)
-            if (slot[i] >= bound)
-                for (int ch = i * TH + tid; ch < n; ch += LG_SLOTS * TH) {
-                    const int at = atomicAdd(&lds.n_list, 1);
-                    if (at < LG_CAND) lds.list[at] = ch;
-                }
-        if (ei >= 0 && end >= bound) candidate(end, ei);
-        __syncthreads();
-        const int n_list = lds.n_list;
-        whole = n_list > LG_CAND;
-        if (!whole) {
-            for (int q = tid; q < n_list; q += TH) {
-                const int ch = row.first + lds.list[q], lo = ch * E - row.sh;
-                float x[E];
-                Chunk<T>::unpack(row.load(ch), x);
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (x[e] >= bound) candidate(x[e], lo + e);
-            }
-            __syncthreads();
-            whole = lds.n_cand > LG_CAND;
+        for (int i = 0; i < LG_SLOTS; ++i) which |= slot[i] >= bound ? 1u << i : 0u;
+        if (which) {
+            const int many = __popc(which);
+            int at = atomicAdd(&lds.n_list, many);
+            if (at + many <= CAP)
+                for (; which; which &= which - 1u) lds.list[at++] = (__ffs(which) - 1) * TH + tid;
         }
-        __syncthreads();
+        if (ei >= 0 && end >= bound) {
+            const int at = atomicAdd(&lds.n_cand, 1);
+            if (at < CAP) lds.cand[at] = order_key(end, ei);
+        }
+        Team<TH>::sync();
+        const int n_list = lds.n_list, rounds = (n + LG_SLOTS * TH - 1) / (LG_SLOTS * TH);
+        whole = n_list > CAP;
+        if (!whole) {
+            const auto sift = [&](int i, const uint4& v) {
+                const int lo = (row.first + i) * E - row.sh;
+                float x[E];
+                Chunk<T>::unpack(v, x);
+                uint32_t mine = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) mine |= x[e] >= bound ? 1u << e : 0u;
+                const int many = __popc(mine);
+                int at = many ? atomicAdd(&lds.n_cand, many) : 0;
+                if (at + many <= CAP)
+                    for (; mine; mine &= mine - 1u) {
+                        const int e = __ffs(mine) - 1;
+                        lds.cand[at++] = order_key(Chunk<T>::pick(v, e), lo + e);
+                    }
+            };
+            for (int j = 0; j < rounds; ++j)
+                for (int q = tid; q < n_list; q += 2 * TH) {
+                    const int i = lds.list[q] + j * (LG_SLOTS * TH), i2 = q + TH < n_list ? lds.list[q + TH] + j * (LG_SLOTS * TH) : n;
+                    const uint4 v = row.load(row.first + min(i, n - 1)), v2 = row.load(row.first + min(i2, n - 1));
+                    if (i < n) sift(i, v);
+                    if (i2 < n) sift(i2, v2);
+                }
+            Team<TH>::sync();
+            whole = lds.n_cand > CAP;
+        }
+        Team<TH>::sync();
     }
     if (whole) top_radix<T, TH>(row, k, lds);
-    write_top<TH>(lds, lds.n_cand, k, a, inv_t, log_s, empty, top_ids + r * k, top_logp + r * k);
+    place_all<T, TH>(lds, lds.n_cand, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
 }
 
 // Rows of up to 64 (W = 16 lanes a row) or 2041 / 2045 logits (W = 64): the whole row lives in registers, the maximum is found first.
@@ -560,18 +709,28 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
             if (row.index(j) < V) cand[row.index(j)] = order_key(x[j], row.index(j));
         });
     } else {
-        // the k-th largest key from the top bit down, until at most `most` keys reach it (then those are the candidates) or it is exact
         uint32_t key[NE];
 #pragma unroll
         for (int j = 0; j < NE; ++j) key[j] = row.index(j) >= 0 && row.index(j) < V ? order_key(x[j]) : 0u;
-        const int most = min(CAP, k + max(8, k >> 2));
         uint32_t at = 0;
         n = V;
-        for (int b = 31; b >= 0 && n > most; --b) {
-            const uint32_t t = at | (1u << b);
-            int cnt = 0;
-            row.each([&](int j) { cnt += __popcll(__ballot(key[j] >= t)); });
-            if (cnt >= k) { at = t; n = cnt; }
+        if (V > CAP || V > k + (k >> 1)) {   // (else every logit is a candidate)
+            float group[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) group[g] = g ? -INFINITY : x[NE - 1];
+            row.each_chunk([&](int j) { group[j & 3] = fmaxf(group[j & 3], x[j]); });
+            at = wave_bound<4, Chunk<T>::E == 8 ? 16 : 0>(group, k);
+            n = 0;
+            row.each([&](int j) { n += __popcll(__ballot(key[j] >= at)); });
+        }
+        if (n > CAP) {   // equal logits, or a short row's long list: the k-th largest key from the top bit down, until few enough reach it
+            at = 0;
+            for (int b = 31; b >= 0 && n > CAP; --b) {
+                const uint32_t t = at | (1u << b);
+                int cnt = 0;
+                row.each([&](int j) { cnt += __popcll(__ballot(key[j] >= t)); });
+                if (cnt >= k) { at = t; n = cnt; }
+            }
         }
         const uint32_t above = n <= CAP ? (at ? at - 1u : 0u) : at;   // (at = 0: every key of the row, they are at least 1)
         const unsigned long long lt = (1ull << lane) - 1ull;
@@ -618,13 +777,16 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
         n = out;
     }
     Team<W>::sync();
-    for (int q = lane; q < n; q += W) {
-        const unsigned long long me = cand[q];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += cand[j] > me;
-        if (place < k) {
-            top_ids[r * k + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
-            top_logp[r * k + place] = empty ? -INFINITY : (key_value((uint32_t)(me >> 32)) - a.m) * inv_t - log_s;
+    const TopOut result = {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty};
+    if constexpr (W == 64) {
+        place_wave<T>(cand, n, V, result);
+    } else {
+        for (int q = lane; q < n; q += W) {
+            const unsigned long long me = cand[q];
+            int place = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) place += cand[j] > me;
+            result.write(me, place);
         }
     }
 }
@@ -1043,13 +1205,14 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
                                        d_entropy, d_lse, d_stats, d_top_ids, d_top_logp)
 #define LG_WG(TH) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP>), dim3(N), dim3(TH), 0, s, z, ld, V, c, inv_t, d_tokens, k, d_logp, d_entropy, d_lse, \
                                      d_stats, d_top_ids, d_top_logp)
-    switch (team_of<T>(V, N)) {
-        case 16: LG_SMALL(16); break;
-        case 64: LG_SMALL(64); break;
-        case 256: LG_WG(256); break;
-        case 512: LG_WG(512); break;
-        default: LG_WG(1024); break;
-    }
+    const int chunks = V / Chunk<T>::E;
+    if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
+    else if (V <= Small<T, 64>::max_v() && !(chunks >= 128 && 64 * min(chunks / 64, 4) >= k + k / 2)) LG_SMALL(64);
+    else if (N <= 256 && V > Small<T, 64>::max_v()) LG_WG(1024);
+    else if (chunks <= LG_B0 * 64) LG_WG(64);
+    else if (chunks <= LG_B1 * 256) LG_WG(256);
+    else if (chunks <= LG_B2 * 512) LG_WG(512);
+    else LG_WG(1024);
 #undef LG_SMALL
 #undef LG_WG
     AG_LAUNCH_CHECK();

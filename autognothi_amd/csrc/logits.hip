@@ -108,6 +108,8 @@ template <int TH>
 struct Team {
     static constexpr int LANES = TH < 64 ? TH : 64, WAVES = TH / 64;
     static __device__ __forceinline__ int rank() { return TH >= 64 && TH < 256 ? threadIdx.x & 63 : threadIdx.x & (TH - 1); }
+    // which team of the workgroup this is (one number for the whole wave where a team is a wave: the row's own numbers are scalars then)
+    static __device__ __forceinline__ int index() { return TH >= 256 ? 0 : TH == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / TH; }
     static __device__ __forceinline__ void sync() {
         if (TH > 64) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the LDS and the loads / stores of one wave keep their order
@@ -828,7 +830,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
                                                                            T* __restrict__ dz, int64_t ldd) {
     constexpr int E = Chunk<T>::E, U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1;
     __shared__ float red[TH < 64 ? 1 : TH / 64];
-    const int64_t r = (int64_t)blockIdx.x * PER + (PER > 1 ? threadIdx.x / TH : 0);
+    const int64_t r = (int64_t)blockIdx.x * PER + Team<TH>::index();
     if (PER > 1 && r >= N) return;
     const int tid = Team<TH>::rank();
     const Row<T> row(z + r * ld, V);
@@ -887,42 +889,40 @@ struct Distill {
     float weight0;
 };
 
-// the list of a row in LDS: token (-1: empty slot, V: no token of the row), mass, and the mass of all slots that name the same token for the
-// first of them (-1 for the others)
-template <int TH> struct ListLds {
-    static constexpr int PER = TH < 256 ? 256 / TH : 1;
-    int id[PER][AG_LOGITS_MAX_TOP];
-    float q[PER][AG_LOGITS_MAX_TOP];
-};
-
 struct Teacher { float Q, rest, qlogq; };
 
-// the list of a row: loaded (before the row's own loads, so that those stay in flight while the list is worked on), then put into LDS
-template <int TH> struct List {
-    static constexpr int J = (AG_LOGITS_MAX_TOP + TH - 1) / TH;
-    float lp[J];
+// the list of a row, by W = 16 or 64 lanes: loaded (before the row's own loads, and not looked at yet, so that those stay in flight while
+// the list is worked on), then a token (-1: empty slot, V: no token of the row) and a mass for each of a lane's slots lane + W i
+template <int W> struct List {
+    static constexpr int J = (AG_LOGITS_MAX_TOP + W - 1) / W;
+    int64_t raw_id[J];
+    uint32_t raw_lp[J];
     int id[J];
-    __device__ __forceinline__ void load(const Distill& p, int64_t r, int V) {
+    float q[J];
+    static __device__ __forceinline__ int lane() { return threadIdx.x & (W - 1); }
+    __device__ __forceinline__ void load(const Distill& p, int64_t r) {
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-            const int j = min(Team<TH>::rank() + i * TH, p.K - 1);
-            const int64_t t = p.ids[r * p.K + j];
-            const float v = p.dtype == AG_BF16 ? bf16_to_f32(((const bf16_t*)p.logp)[r * p.K + j]) : ((const float*)p.logp)[r * p.K + j];
-            id[i] = t < 0 ? -1 : t >= V ? V : (int)t;
-            lp[i] = t < 0 || Team<TH>::rank() + i * TH >= p.K ? -INFINITY : t >= V ? NAN : v;
+            const int64_t j = r * p.K + min(lane() + i * W, p.K - 1);
+            raw_id[i] = p.ids[j];
+            raw_lp[i] = p.dtype == AG_BF16 ? ((const bf16_t*)p.logp)[j] : ((const uint32_t*)p.logp)[j];
         }
     }
-    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int* sid, float* sq, float* red) {
-        const int tid = Team<TH>::rank();
-        float m = lp[0];
+    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int V) {
+        float lp[J], m = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < J; ++i) m = fmaxf(m, lp[i]);
-        m = Team<TH>::max(m, red);
+        for (int i = 0; i < J; ++i) {
+            const bool there = raw_id[i] >= 0 && lane() + i * W < p.K;
+            id[i] = !there ? -1 : raw_id[i] >= V ? V : (int)raw_id[i];
+            lp[i] = !there ? -INFINITY : id[i] == V ? NAN : __uint_as_float(p.dtype == AG_BF16 ? raw_lp[i] << 16 : raw_lp[i]);
+            m = fmaxf(m, lp[i]);
+        }
+        m = lanes_join<W>(m, Max());
         if (!TAIL) {
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < J; ++i) s += lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
-            s = Team<TH>::sum(s, red);
+            s = lanes_join<W>(s, Add());
             const float ls = logf(s);
 #pragma unroll
             for (int i = 0; i < J; ++i) lp[i] = s == 0.f ? -INFINITY : (lp[i] - m) - ls;
@@ -931,19 +931,17 @@ template <int TH> struct List {
         float others = 0.f, top = 0.f;   // the masses that are not the largest, and how many are
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-            const int j = tid + i * TH;
-            const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
-            if (j < p.K) { sid[j] = id[i]; sq[j] = q; }
-            t.Q += q;
-            t.qlogq += q == 0.f ? 0.f : q * lp[i];
-            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q; }
+            q[i] = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
+            t.Q += q[i];
+            t.qlogq += q[i] == 0.f ? 0.f : q[i] * lp[i];
+            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q[i]; }
         }
-        t.Q = Team<TH>::sum(t.Q, red);
-        t.qlogq = Team<TH>::sum(t.qlogq, red);
+        t.Q = lanes_join<W>(t.Q, Add());
+        t.qlogq = lanes_join<W>(t.qlogq, Add());
         if (TAIL) {
             // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
-            top = Team<TH>::sum(top, red);
-            others = Team<TH>::sum(others, red);
+            top = lanes_join<W>(top, Add());
+            others = lanes_join<W>(others, Add());
             t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (top - 1.f) * expf(m) - others, 0.f);
             if (t.Q != t.Q) t.rest = t.Q;
         }
@@ -954,17 +952,40 @@ template <int TH> struct List {
 // what a row's gradient takes from the forward pass: g a exp2((z - m_off) c) off the list, g (on exp2((z - m) c) - q) on it
 struct GradOf { float m_off, a, m, on; };
 
-template <typename T, int TH>
-__device__ __forceinline__ void listed_gradients(const Row<T>& row, const int* sid, const float* sq, int K, const GradOf& s, float g, float c, T* d) {
-    for (int j = Team<TH>::rank(); j < K; j += TH) {
-        const int i = sid[j];
-        if (i < 0 || i >= row.V) continue;
-        float q = 0.f;
-        bool first = true;
-        for (int p = 0; p < K; ++p)
-            if (sid[p] == i) { q += sq[p]; first &= p >= j; }
-        if (first) Store<T>::store(d + i, g * (exp2_from(Store<T>::load(row.z + i), s.m, c) * s.on - q));
+// The gradients of the listed tokens (W lanes; gx: their logits; bit i of `first`: this lane's i-th slot is known to be the first that names
+// its token).  Where a token may be listed more than once its masses are added up: the slots find that out from each other in LDS.
+template <typename T, int W>
+__device__ __forceinline__ void listed_gradients(const Row<T>& row, const List<W>& l, const float* gx, int K, uint32_t first, const GradOf& s, float g,
+                                                 float c, int* sid, float* sq, T* d) {
+    constexpr int J = List<W>::J;
+    uint32_t is = 0;
+#pragma unroll
+    for (int i = 0; i < J; ++i) is |= l.id[i] >= 0 && l.id[i] < row.V ? 1u << i : 0u;
+    if (__any(is != first)) {
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+            const int j = l.lane() + i * W;
+            if (j < K) { sid[j] = l.id[i]; sq[j] = l.q[i]; }
+        }
+        Team<W>::sync();
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+            const int j = l.lane() + i * W, at = l.id[i];
+            if (!((is >> i) & 1u)) continue;
+            float q = 0.f;
+            bool one = true;
+#pragma unroll 4
+            for (int o = 0; o < K; ++o) {
+                q += sid[o] == at ? sq[o] : 0.f;
+                one &= sid[o] != at || o >= j;
+            }
+            if (one) Store<T>::store(d + at, g * (exp2_from(gx[i], s.m, c) * s.on - q));
+        }
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+        if ((is >> i) & 1u) Store<T>::store(d + l.id[i], g * (exp2_from(gx[i], s.m, c) * s.on - l.q[i]));
 }
 template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const uint4& v, float c, const Ref& ref, float ga, T* d) {
     constexpr int E = Chunk<T>::E;
@@ -983,139 +1004,291 @@ template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T
 // words of LDS for a bit per logit of a row's chunks, whatever its alignment
 template <typename T> __host__ __device__ constexpr int bit_words(int V) { return (V + Chunk<T>::E - 1 + 31) / 32 + 1; }
 
-// Loss, and (GRAD) its gradient from the same pass: a lane holds NC chunks of the row in registers between the sums and the gradient, so a
-// row of up to TH NC chunks is read once; a longer one takes several rounds and reads all but its last round again.
-template <typename T, int TH, int NC, bool TAIL, bool GRAD>
-__global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p,
-                                                                      float* __restrict__ row_loss, float* __restrict__ stats, T* __restrict__ dz,
-                                                                      int64_t ldd) {
-    constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1, BITS = 32 / E;   // chunks whose bits share a word
-    extern __shared__ uint32_t bits_lds[];
-    __shared__ float red[TH < 64 ? 1 : 3 * (TH / 64)];
-    __shared__ ListLds<TH> list;
-    const int team = PER > 1 ? threadIdx.x / TH : 0, tid = Team<TH>::rank();
-    const int64_t r = (int64_t)blockIdx.x * PER + team;
-    if (PER > 1 && r >= N) return;
-    const Row<T> row(z + r * ld, V);
-    const int n = row.full(), ei = row.end_index(tid);
-    T* d = dz + r * ldd;
-    const float w = p.weights ? p.weights[r] : p.weight0;
-    if (w == 0.f) {   // the row takes no part
-        if (tid == 0) row_loss[r] = 0.f;
-        if (!GRAD && tid < 4) stats[r * 4 + tid] = 0.f;
-        if (GRAD) zero_row<T, TH>(row, d);
-        return;
-    }
-    List<TH> mine;
-    mine.load(p, r, V);
-    const float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
-    uint4 v[NC];
-    const auto fetch = [&](int i0) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) v[i] = row.load(row.first + max(min(i0 + i * TH + tid, n - 1), 0));
-    };
-    if (n > 0) fetch(0);
-    int* sid = list.id[team];
-    float* sq = list.q[team];
-    Teacher tc = mine.template finish<TAIL>(p, sid, sq, red);
-    uint32_t* bits = bits_lds + (TAIL ? team * bit_words<T>(V) : 0);   // logit i: bit i + sh
-    if (TAIL)
-        for (int i = tid; i < bit_words<T>(V); i += TH) bits[i] = 0u;
-    Team<TH>::sync();
-    if (TAIL) {
-        float fresh = 0.f;
-        for (int j = tid; j < p.K; j += TH) {
-            if (sid[j] < 0 || sid[j] >= V) continue;
-            const int at = sid[j] + row.sh;
-            const uint32_t b = 1u << (at & 31);
-            fresh += atomicOr(&bits[at >> 5], b) & b ? 0.f : 1.f;
-        }
-        if ((int)Team<TH>::sum(fresh, red) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
-        Team<TH>::sync();
-    }
-    Sums<T, false> sums(c);
-    for (int i0 = 0; i0 < n;) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            if (i0 + i * TH + tid < n) {
-                const int ch = row.first + i0 + i * TH + tid;
-                float y[E];
-                Chunk<T>::unpack(v[i], y);
-                if (TAIL) {
-                    const uint32_t b = (bits[ch / BITS] >> ((ch % BITS) * E)) & ((1u << E) - 1u);
-                    if (b) {
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            if ((b >> e) & 1u) y[e] = -INFINITY;
-                    }
-                }
-                sums.add(y, max_of(y));
-            }
-        }
-        i0 += NC * TH;
-        if (i0 < n) fetch(i0);
-    }
-    if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(end);
-    const Acc off = team_join<TH>(sums.acc(), c, red);
-    // the listed tokens' logits: their part of the sums (with the tail), and of the loss
-    Acc all = off;
-    if (TAIL) {
-        float lm = LG_NEG, s = 0.f;
-        for (int j = tid; j < p.K; j += TH)
-            if (sid[j] >= 0 && sid[j] < V) lm = fmaxf(lm, Store<T>::load(row.z + sid[j]));
-        all = rebase(off, fmaxf(off.m, Team<TH>::max(lm, red)), c);
-        for (int j = tid; j < p.K; j += TH) {
-            if (sid[j] < 0 || sid[j] >= V) continue;
-            bool first = true;
-            for (int i = 0; i < j; ++i) first &= sid[i] != sid[j];
-            if (first) s += exp2_from(Store<T>::load(row.z + sid[j]), all.m, c);
-        }
-        all.s += Team<TH>::sum(s, red);
-    }
-    const bool empty = all.s == 0.f;
-    const float log_s = empty ? -INFINITY : logf(all.s);
-    float cross = 0.f;
-    for (int j = tid; j < p.K; j += TH) {
-        const float q = sq[j];
-        if (q == 0.f) continue;
-        cross += sid[j] >= V ? NAN : q * (empty ? INFINITY : log_s - (Store<T>::load(row.z + sid[j]) - all.m) * inv_t);
-    }
-    cross = Team<TH>::sum(cross, red);
+// the row's loss from its sums (off: over what the dense part of the gradient covers, all: over the row), and what its gradient takes from them
+template <bool TAIL> __device__ __forceinline__ GradOf row_gradient(const Teacher& tc, const Acc& off, const Acc& all, float c) {
     GradOf s;
+    const bool empty = all.s == 0.f;
     s.m_off = off.m;
     s.m = empty ? -INFINITY : all.m;
     s.on = empty ? 0.f : (tc.Q + tc.rest) / all.s;
     s.a = !TAIL ? s.on : off.s == 0.f ? 0.f : s.on * __builtin_amdgcn_exp2f((off.m - all.m) * c) - tc.rest / off.s;
-    if (tid == 0) {
-        float L = tc.qlogq + cross;
-        if (TAIL && tc.rest != 0.f) L += tc.rest * (logf(tc.rest) - (off.s == 0.f ? -INFINITY : (off.m - all.m) * inv_t + logf(off.s) - log_s));
-        row_loss[r] = tau * tau * L;
+    return s;
+}
+template <bool TAIL> __device__ __forceinline__ float row_loss_of(const Teacher& tc, float cross, const Acc& off, const Acc& all, float log_s, float tau, float inv_t) {
+    float L = tc.qlogq + cross;
+    if (TAIL && tc.rest != 0.f) L += tc.rest * (logf(tc.rest) - (off.s == 0.f ? -INFINITY : (off.m - all.m) * inv_t + logf(off.s) - log_s));
+    return tau * tau * L;
+}
+
+// Rows of up to 64 logits, 16 lanes a row: the row, the listed masses of its tokens and the gradient stay in registers.
+template <typename T, bool TAIL, bool GRAD>
+__global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p,
+                                                            float* __restrict__ row_loss, float* __restrict__ stats, T* __restrict__ dz, int64_t ldd) {
+    using S = Small<T, 16>;
+    using G = Team<16>;
+    constexpr int NE = S::NE;
+    __shared__ int sid_lds[16][AG_LOGITS_MAX_TOP];
+    __shared__ float sq_lds[16][AG_LOGITS_MAX_TOP];
+    const int team = threadIdx.x / 16, lane = G::rank();
+    const int64_t r = (int64_t)blockIdx.x * 16 + team;
+    if (r >= N) return;
+    T* d = dz + r * ldd;
+    const S row(z + r * ld, V, lane);
+    const float w = p.weights ? p.weights[r] : p.weight0;
+    const bool part = w != 0.f;
+    List<16> mine;
+    mine.load(p, r);
+    float x[NE];
+    if (part) row.load(x);
+    int* sid = sid_lds[team];
+    float* sq = sq_lds[team];
+    Teacher tc = mine.template finish<TAIL>(p, V);
+#pragma unroll
+    for (int i = 0; i < List<16>::J; ++i)
+        if (lane + 16 * i < p.K) { sid[lane + 16 * i] = mine.id[i]; sq[lane + 16 * i] = mine.q[i]; }
+    G::sync();
+    float q[NE] = {};
+    uint32_t listed = 0;     // bit j: element j is on the list
+    for (int j = 0; j < p.K; ++j) {
+        const int id = sid[j];
+        const float m = sq[j];
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+            if (id == row.index(e)) { q[e] += m; listed |= 1u << e; }
+    }
+    if (TAIL && (int)G::sum((float)__popc(listed), nullptr) >= V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
+    if (!part) {   // the row takes no part
+        if (lane == 0) row_loss[r] = 0.f;
+        if (!GRAD && lane < 4) stats[r * 4 + lane] = 0.f;
+        if (GRAD) row.each([&](int e) { if (row.index(e) < V) Store<T>::store(d + row.index(e), 0.f); });
+        return;
+    }
+    float lm = LG_NEG, om = LG_NEG;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        if (TAIL && !((listed >> e) & 1u)) om = fmaxf(om, x[e]);
+        lm = fmaxf(lm, x[e]);
+    }
+    Acc all = {G::max(lm, nullptr), 0.f, 0.f}, off = {TAIL ? G::max(om, nullptr) : all.m, 0.f, 0.f};
+    float ex[NE], so = 0.f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        const bool on = TAIL && ((listed >> e) & 1u);
+        ex[e] = exp2_from(x[e], on ? all.m : off.m, c);
+        if (on) all.s += ex[e]; else so += ex[e];
+    }
+    off.s = G::sum(so, nullptr);
+    all.s = TAIL ? G::sum(all.s, nullptr) + rebase(off, all.m, c).s : off.s;
+    const bool empty = all.s == 0.f;
+    const float log_s = empty ? -INFINITY : logf(all.s);
+    float cross = 0.f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) cross += q[e] == 0.f ? 0.f : q[e] * (empty ? INFINITY : log_s - (x[e] - all.m) * inv_t);
+    cross = G::sum(cross, nullptr);
+    const GradOf s = row_gradient<TAIL>(tc, off, all, c);
+    if (lane == 0) {
+        row_loss[r] = tc.Q != tc.Q ? tc.Q : row_loss_of<TAIL>(tc, cross, off, all, log_s, tau, inv_t);
         if (!GRAD) *reinterpret_cast<float4*>(stats + r * 4) = make_float4(s.m_off, s.a, s.m, s.on);
     }
     if (!GRAD) return;
-    if (empty) { zero_row<T, TH>(row, d); return; }
-    const Ref ref(s.m_off, c);
-    const float g = tau * w, ga = g * s.a;
-    if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(end, ref.m, c));
-    for (int i0 = (n - 1) / (NC * TH) * (NC * TH); i0 >= 0 && n > 0;) {   // the last round's chunks are still here
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (i0 + i * TH + tid < n) gradient_chunk(row, row.first + i0 + i * TH + tid, v[i], c, ref, ga, d);
-        i0 -= NC * TH;
-        if (i0 >= 0) fetch(i0);
-    }
+    const float g = tau * w;
+    row.each([&](int e) {
+        if (row.index(e) >= V) return;
+        const bool on = (listed >> e) & 1u;
+        Store<T>::store(d + row.index(e), empty ? 0.f : on ? g * (ex[e] * s.on - q[e]) : g * s.a * ex[e]);
+    });
+}
+
+// Loss, and (GRAD) its gradient from the same pass.  A lane holds NC chunks of the row in registers between the sums and the gradient, so a
+// row of up to TH NC chunks is read once (a longer one in several rounds, all but the last of them twice).  A row's sums and its gradient
+// are work of different kinds with a join between them, and few such rows fit a CU at once: the workgroups stay, and a chunk's registers take
+// the next round's or the next row's chunk as soon as the chunk is done with, so that memory is busy through all of it.
+// The list is the first wave's: it works on it while the row arrives, marks the listed tokens for the sums of all waves, adds their own part,
+// and writes the loss and the listed tokens' gradients.  MULTI: rows of several rounds.
+template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD>
+__global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
+    const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
+    T* __restrict__ dz, int64_t ldd) {
+    constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1, BITS = 32 / E;   // chunks whose bits share a word
+    constexpr int J = List<64>::J, ROUND = NC * TH;
+    extern __shared__ uint32_t bits_lds[];
+    __shared__ float red[3 * (TH / 64)];
+    __shared__ int sid_lds[PER][AG_LOGITS_MAX_TOP];
+    __shared__ float sq_lds[PER][AG_LOGITS_MAX_TOP];
+    __shared__ float said[PER][4];   // the first wave's word: mass on the list, the rest; the listed logits' largest, their exponentials' sum
+    const int team = Team<TH>::index(), tid = Team<TH>::rank();
+    const bool lead = TH == 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
+    const int64_t stride = (int64_t)gridDim.x * PER;
+    uint32_t* bits = bits_lds + team * bit_words<T>(V);   // logit i of the row: bit i + sh, set where it is listed
+    for (int i = tid; i < bit_words<T>(V); i += TH) bits[i] = 0u;
     Team<TH>::sync();
-    listed_gradients<T, TH>(row, sid, sq, p.K, s, g, c, d);
+    // the first row from r on that takes part (of those that do not: no loss, no gradient)
+    const auto next_row = [&](int64_t r) {
+        for (; r < N; r += stride) {
+            if (!p.weights || p.weights[r] != 0.f) break;
+            if (tid == 0) row_loss[r] = 0.f;
+            if (!GRAD && tid < 4) stats[r * 4 + tid] = 0.f;
+            if (GRAD) zero_row<T, TH>(Row<T>(z + r * ld, V), dz + r * ldd);
+        }
+        return r;
+    };
+    int64_t r = next_row((int64_t)blockIdx.x * PER + team);
+    if (r >= N) return;
+    List<64> mine;
+    uint4 v[NC];
+    if (lead) mine.load(p, r);
+    Row<T> row(z + r * ld, V);
+    int ei = row.end_index(tid);
+    float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
+    {
+        const int last = row.full() - 1;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = row.load(row.first + min(i * TH + tid, last));
+    }
+    for (;;) {
+        // (the places of a thread's chunks are worked out where they are used, from a number that the compiler cannot see through: kept over
+        // the loop, they are NC registers that the chunks themselves need)
+        int t0 = tid, t1 = tid;
+        asm volatile("" : "+v"(t0));
+        const int n = row.full();
+        T* d = dz + r * ldd;
+        const float w = p.weights ? p.weights[r] : p.weight0;
+        const int64_t r2 = next_row(r + stride);
+        const Row<T> row2(r2 < N ? z + r2 * ld : row.z, V);
+        const int last2 = r2 < N ? row2.full() - 1 : 0;   // (no next row: its loads are one chunk of this one, again and again)
+        const int ei2 = row2.end_index(tid);
+        Teacher tc = {0.f, 0.f, 0.f};
+        float gx[J];           // the logits of the slots' tokens
+        uint32_t first = 0;    // bit i: no earlier slot names the token of this lane's i-th
+        if (lead) {
+            tc = mine.template finish<TAIL>(p, V);
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+                const bool is = mine.id[i] >= 0 && mine.id[i] < V;
+                gx[i] = is ? Store<T>::load(row.z + mine.id[i]) : -INFINITY;
+                if (is) {
+                    const int at = mine.id[i] + row.sh;
+                    const uint32_t b = 1u << (at & 31);
+                    if (!(atomicOr(&bits[at >> 5], b) & b)) first |= 1u << i;
+                }
+            }
+            if (TAIL && TH == 64 && (int)lanes_join<64>((float)__popc(first), Add()) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
+            if (tid == 0) { said[team][0] = tc.Q; said[team][1] = tc.rest; }
+        }
+        if (TAIL) Team<TH>::sync();
+        Sums<T, false> sums(c);
+        const auto add_chunk = [&](int i, int ch) {
+            float y[E];
+            Chunk<T>::unpack(v[i], y);
+            if (TAIL) {
+                const uint32_t b = (bits[ch / BITS] >> ((ch % BITS) * E)) & ((1u << E) - 1u);
+                if (b) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if ((b >> e) & 1u) y[e] = -INFINITY;
+                }
+            }
+            sums.add(y, max_of(y));
+        };
+        const int lastr = MULTI ? (n - 1) / ROUND * ROUND : 0;
+        for (int i0 = 0; i0 < lastr; i0 += ROUND) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                add_chunk(i, row.first + i0 + i * TH + t0);
+                v[i] = row.load(row.first + min(i0 + ROUND + i * TH + t0, n - 1));
+            }
+        }
+        float end2 = -INFINITY;
+        List<64> next;
+        if (!GRAD) {
+            if (lead) next.load(p, r2 < N ? r2 : r);
+            if (ei2 >= 0) end2 = Store<T>::load(row2.z + ei2);
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (lastr + i * TH + t0 < n) add_chunk(i, row.first + lastr + i * TH + t0);
+            if (!GRAD) v[i] = row2.load(row2.first + min(i * TH + t0, last2));
+        }
+        if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(end);
+        if (TAIL && lead) {   // the listed tokens' part of the sums
+            float lm = LG_NEG, ls = 0.f;
+#pragma unroll
+            for (int i = 0; i < J; ++i) lm = fmaxf(lm, gx[i]);
+            lm = lanes_join<64>(lm, Max());
+#pragma unroll
+            for (int i = 0; i < J; ++i) ls += (first >> i) & 1u ? exp2_from(gx[i], lm, c) : 0.f;
+            ls = lanes_join<64>(ls, Add());
+            if (tid == 0) { said[team][2] = lm; said[team][3] = ls; }
+        }
+        const Acc off = team_join<TH>(sums.acc(), c, red);
+        if (TH == 64) Team<TH>::sync();
+        const float Q = said[team][0], rest = said[team][1];
+        Acc all = off;
+        if (TAIL) {
+            const Acc listed = {said[team][2], said[team][3], 0.f};
+            const float m = fmaxf(off.m, listed.m);
+            all = rebase(off, m, c);
+            all.s += rebase(listed, m, c).s;
+        }
+        const bool empty = all.s == 0.f;
+        const GradOf s = row_gradient<TAIL>({Q, rest, 0.f}, off, all, c);
+        if (lead) {
+            const float log_s = empty ? -INFINITY : logf(all.s);
+            float cross = 0.f;
+#pragma unroll
+            for (int i = 0; i < J; ++i) cross += mine.q[i] == 0.f ? 0.f : mine.q[i] * (empty ? INFINITY : log_s - (gx[i] - all.m) * inv_t);
+            cross = lanes_join<64>(cross, Add());
+            if (tid == 0) {
+                row_loss[r] = Q != Q ? Q : row_loss_of<TAIL>(tc, cross, off, all, log_s, tau, inv_t);   // (an id beyond the row)
+                if (!GRAD) *reinterpret_cast<float4*>(stats + r * 4) = make_float4(s.m_off, s.a, s.m, s.on);
+            }
+#pragma unroll
+            for (int i = 0; i < J; ++i)   // (every wave is done with them)
+                if (mine.id[i] >= 0 && mine.id[i] < V) bits[(mine.id[i] + row.sh) >> 5] = 0u;
+        }
+        if (GRAD) {
+            if (lead) next.load(p, r2 < N ? r2 : r);
+            if (ei2 >= 0) end2 = Store<T>::load(row2.z + ei2);
+            const Ref ref(s.m_off, c);
+            const float g = tau * w, ga = empty ? 0.f : g * s.a;
+            asm volatile("" : "+v"(t1));
+            if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(end, ref.m, c));
+            // the last round's chunks are still here; the rounds before it, then the next row's first round come in their places
+            const auto round = [&](int i0, bool again) {
+                const T* from = again ? row.z + ((row.first + i0 - ROUND) * E - row.sh) : row2.z + (row2.first * E - row2.sh);
+                const int to = again ? ROUND - 1 : last2;
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    if (i0 + i * TH + t1 < n) gradient_chunk(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
+                    v[i] = *reinterpret_cast<const uint4*>(from + min(i * TH + t1, to) * E);
+                }
+            };
+            if (!MULTI) round(0, false);
+            else
+                for (int i0 = lastr; i0 >= 0; i0 -= ROUND) round(i0, i0 > 0);
+            Team<TH>::sync();
+            if (lead && !empty) listed_gradients<T, 64>(row, mine, gx, p.K, first, s, g, c, sid_lds[team], sq_lds[team], d);
+        } else {
+            Team<TH>::sync();   // (the first wave's words are read)
+        }
+        if (r2 >= N) break;
+        mine = next;
+        r = r2;
+        row = row2;
+        ei = ei2;
+        end = end2;
+    }
 }
 
 template <typename T, int TH, bool TAIL>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                                                                           const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
-    constexpr int U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1;
-    __shared__ float red[TH < 64 ? 1 : TH / 64];
-    __shared__ ListLds<TH> list;
-    const int team = PER > 1 ? threadIdx.x / TH : 0, tid = Team<TH>::rank();
+    constexpr int U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1, W = TH < 64 ? TH : 64;
+    __shared__ int sid_lds[PER][AG_LOGITS_MAX_TOP];
+    __shared__ float sq_lds[PER][AG_LOGITS_MAX_TOP];
+    const int team = Team<TH>::index(), tid = Team<TH>::rank();
+    const bool lead = TH <= 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
     const int64_t r = (int64_t)blockIdx.x * PER + team;
     if (PER > 1 && r >= N) return;
     const Row<T> row(z + r * ld, V);
@@ -1127,17 +1300,22 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
         zero_row<T, TH>(row, d);
         return;
     }
-    List<TH> mine;
-    mine.load(p, r, V);
+    List<W> mine;
+    if (lead) mine.load(p, r);
     const Ref ref(s.m_off, c);
     const float g = tau * (g_loss || g_row ? (g_loss ? w * g_loss[0] : 0.f) + (g_row ? g_row[r] : 0.f) : w);
     const float ga = g * s.a;
     const int ei = row.end_index(tid);
     if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
     each_chunk<T, TH, U>(row, [&](int ch, const uint4& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
-    mine.template finish<TAIL>(p, list.id[team], list.q[team], red);
+    float gx[List<W>::J];
+    if (lead) {
+        mine.template finish<TAIL>(p, V);
+#pragma unroll
+        for (int i = 0; i < List<W>::J; ++i) gx[i] = mine.id[i] >= 0 && mine.id[i] < V ? Store<T>::load(row.z + mine.id[i]) : -INFINITY;
+    }
     Team<TH>::sync();
-    listed_gradients<T, TH>(row, list.id[team], list.q[team], p.K, s, g, c, d);
+    if (lead) listed_gradients<T, W>(row, mine, gx, p.K, 0u, s, g, c, sid_lds[team], sq_lds[team], d);
 }
 
 // sum_n w_n L_n in a fixed order
@@ -1232,13 +1410,31 @@ int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperatu
 template <typename T, bool TAIL, bool GRAD>
 int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, float* d_row_loss, float* d_stats, void* d_dlogits,
             int64_t ldd, hipStream_t s) {
-    constexpr int E = Chunk<T>::E;
-#define LG_CALL(TH)                                                                                                                                   \
-    constexpr int NC = TH == 16 ? 64 / E / 16 + (E == 8) : TH == 64 ? 32 / E : GRAD ? 16 : 4;                                                          \
-    const size_t lds = TAIL ? (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1) : 0;                                                                      \
-    hipLaunchKernelGGL((distill_kernel<T, TH, NC, TAIL, GRAD>), team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), lds, s, (const T*)d_logits, ld, N, V,     \
-                       temperature, log2e_over(temperature), one_over(temperature), p, d_row_loss, d_stats, (T*)d_dlogits, ldd)
-    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+    const T* z = (const T*)d_logits;
+    T* dz = (T*)d_dlogits;
+    const float c = log2e_over(temperature), inv_t = one_over(temperature);
+    const int chunks = V / Chunk<T>::E, cus = ag_device_cus() > 0 ? ag_device_cus() : 256;
+    if (V <= Small<T, 16>::max_v()) {
+        hipLaunchKernelGGL((distill_small_kernel<T, TAIL, GRAD>), dim3(ceil_div(N, 16)), dim3(256), 0, s, z, ld, N, V, temperature, c, inv_t, p, d_row_loss,
+                           d_stats, dz, ldd);
+        AG_LAUNCH_CHECK();
+        return AG_OK;
+    }
+#define LG_CALL(TH, NC, MULTI, PER_CU)                                                                                                                       \
+    hipLaunchKernelGGL((distill_kernel<T, TH, NC, MULTI, TAIL, GRAD>), dim3(min(ceil_div(N, TH < 256 ? 256 / TH : 1), cus * (PER_CU))), dim3(TH < 256 ? 256 : TH), \
+                       (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1), s, z, ld, N, V, temperature, c, inv_t, p, d_row_loss, d_stats, dz, ldd)
+    if constexpr (GRAD) {
+        if (chunks <= 4 * 64) LG_CALL(64, 4, false, 6);
+        else if (chunks <= 8 * 64) LG_CALL(64, 8, false, 5);
+        else if (chunks <= 8 * 256) LG_CALL(256, 8, false, 5);
+        else if (chunks <= 16 * 256) LG_CALL(256, 16, false, 4);
+        else if (chunks <= 16 * 512) LG_CALL(512, 16, false, 2);
+        else if (chunks <= 16 * 1024) LG_CALL(1024, 16, false, 1);
+        else LG_CALL(1024, 16, true, 1);
+    } else {
+        if (chunks <= 8 * 64) LG_CALL(64, 4, true, 6);
+        else LG_CALL(256, 4, true, 6);
+    }
 #undef LG_CALL
     AG_LAUNCH_CHECK();
     return AG_OK;

@@ -18,37 +18,41 @@ constexpr float LG_NEG = -3.402823466e38f;   // the reference of a row (or part 
 constexpr float LG_SLACK = 3.0f;
 constexpr float LG_LN2 = 0.69314718055994530942f;
 
-template <typename T> struct Chunk;   // E logits of 16 bytes
+typedef __attribute__((ext_vector_type(4))) uint32_t chunk_t;   // 16 bytes of a row
+
+template <typename T> struct Chunk;   // as E logits
 template <> struct Chunk<float> {
+    using Bits = uint32_t;
     static constexpr int E = 4;
-    static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[4]) {
+    static __device__ __forceinline__ void unpack(const chunk_t& r, float (&x)[4]) {
         x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
     }
-    static __device__ __forceinline__ float pick(const uint4& r, int e) {   // (selections, not an array in memory)
+    static __device__ __forceinline__ float pick(const chunk_t& r, int e) {   // (selections, not an array in memory)
         uint32_t a = r.x, b = r.y, c = r.z, d = r.w;
         asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
         const uint32_t p = e & 1 ? b : a, q = e & 1 ? d : c;
         return __uint_as_float(e & 2 ? q : p);
     }
-    static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    static __device__ __forceinline__ chunk_t pack(const float (&x)[4]) {
+        return chunk_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
     }
 };
 template <> struct Chunk<bf16_t> {
+    using Bits = bf16_t;
     static constexpr int E = 8;
-    static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
+    static __device__ __forceinline__ void unpack(const chunk_t& r, float (&x)[8]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
     }
-    static __device__ __forceinline__ float pick(const uint4& r, int e) {
+    static __device__ __forceinline__ float pick(const chunk_t& r, int e) {
         uint32_t a = r.x, b = r.y, c = r.z, d = r.w;
         asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
         const uint32_t p = e & 2 ? b : a, q = e & 2 ? d : c, w = e & 4 ? q : p;
         return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
     }
-    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-        return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    static __device__ __forceinline__ chunk_t pack(const float (&x)[8]) {
+        return chunk_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
     }
 };
 
@@ -66,7 +70,10 @@ struct Row {
         end = max((v + sh) / E, first);
     }
     __device__ __forceinline__ int full() const { return end - first; }
-    __device__ __forceinline__ uint4 load(int c) const { return *reinterpret_cast<const uint4*>(z + (c * E - sh)); }
+    __device__ __forceinline__ chunk_t load(int c) const { return *reinterpret_cast<const chunk_t*>(z + (c * E - sh)); }
+    // one logit's bits, to be made a number (`value`) where it is wanted: nothing waits for the load here
+    __device__ __forceinline__ uint32_t bits(int i) const { return reinterpret_cast<const typename Chunk<T>::Bits*>(z)[i]; }
+    static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(E == 8 ? b << 16 : b); }
     // the logit at the row's ends that belongs to lane l of the row's threads (-1: none)
     __device__ __forceinline__ int end_index(int l) const {
         if (l < E) return sh && l < min(E - sh, V) ? l : -1;
@@ -75,10 +82,8 @@ struct Row {
     }
     // the chunk's place in another row of the same length (at the logits' alignment: the hardware takes any)
     __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const {
-        typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t any_uint4;
-        const uint4 r = Chunk<T>::pack(x);
-        const any_uint4 v = {r.x, r.y, r.z, r.w};
-        *reinterpret_cast<any_uint4*>(d + (c * E - sh)) = v;
+        typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t any_chunk_t;
+        *reinterpret_cast<any_chunk_t*>(d + (c * E - sh)) = Chunk<T>::pack(x);
     }
 };
 
@@ -100,6 +105,12 @@ template <int W, typename F> __device__ __forceinline__ float lanes_join(float v
     }
     return v;
 }
+// one number that all lanes of a wave want, through the scalar cache (a vector load would queue behind every load of the row in flight)
+__device__ __forceinline__ float scalar_load(const float* p) {
+    typedef __attribute__((address_space(4))) const float constant_float;
+    return *(constant_float*)(uintptr_t)p;
+}
+
 struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
 struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 
@@ -167,6 +178,7 @@ template <int TH> __device__ __forceinline__ Acc team_join(Acc a, float c, float
 struct Ref {
     float m, nr, delta;
     bool far;
+    __device__ __forceinline__ Ref() : m(LG_NEG), nr(0.f), delta(0.f), far(true) {}   // of nothing yet
     __device__ __forceinline__ Ref(float m_, float c) : m(m_) {
         nr = -(m * c);
         far = !(fabsf(nr) < 1048576.f);
@@ -184,7 +196,7 @@ struct Sums {
     float lim = LG_NEG;   // what a logit must pass to move the reference
     float zero;           // 0, or NaN where the reference is `far`: every chunk then takes the guarded form below
     Ref ref;
-    __device__ __forceinline__ Sums(float c_) : c(c_), slack(LG_SLACK / c_), ref(LG_NEG, c_) { zero = NAN; }
+    __device__ __forceinline__ Sums(float c_) : c(c_), slack(LG_SLACK / c_) { zero = NAN; }
     // (s, t) without the reference's delta
     __device__ __forceinline__ Acc acc() const {
         const float f = __builtin_amdgcn_exp2f(-ref.delta);
@@ -501,8 +513,8 @@ __global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __res
     for (int i = 0; i < LG_SLOTS; ++i) slot[i] = -INFINITY;
     const int n = row.full(), ei = row.end_index(tid);
     // the next U chunks are on their way while U are added up (loads without a condition: behind the row's end its last chunk again)
-    uint4 v[U], w[U];
-    const auto fetch = [&](uint4 (&to)[U], int i0) {
+    chunk_t v[U], w[U];
+    const auto fetch = [&](chunk_t (&to)[U], int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) to[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
     };
@@ -584,7 +596,7 @@ __global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __res
         const int n_list = lds.n_list, rounds = (n + LG_SLOTS * TH - 1) / (LG_SLOTS * TH);
         whole = n_list > CAP;
         if (!whole) {
-            const auto sift = [&](int i, const uint4& v) {
+            const auto sift = [&](int i, const chunk_t& v) {
                 const int lo = (row.first + i) * E - row.sh;
                 float x[E];
                 Chunk<T>::unpack(v, x);
@@ -602,7 +614,7 @@ __global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __res
             for (int j = 0; j < rounds; ++j)
                 for (int q = tid; q < n_list; q += 2 * TH) {
                     const int i = lds.list[q] + j * (LG_SLOTS * TH), i2 = q + TH < n_list ? lds.list[q + TH] + j * (LG_SLOTS * TH) : n;
-                    const uint4 v = row.load(row.first + min(i, n - 1)), v2 = row.load(row.first + min(i2, n - 1));
+                    const chunk_t v = row.load(row.first + min(i, n - 1)), v2 = row.load(row.first + min(i2, n - 1));
                     if (i < n) sift(i, v);
                     if (i2 < n) sift(i2, v2);
                 }
@@ -657,7 +669,7 @@ template <typename T> struct Small<T, 64> {   // chunks of a lane: lane + 64 i, 
     }
     __device__ __forceinline__ void load(float (&x)[NE]) const {
         const int n = row.full();
-        uint4 v[NC];
+        chunk_t v[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) v[i] = row.load(row.first + min(i * 64 + lane, n - 1));   // (more than 64 logits: n > 0)
         x[NE - 1] = end >= 0 ? Store<T>::load(row.z + end) : -INFINITY;
@@ -803,7 +815,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 template <typename T, int TH, int U, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, F f) {
     const int tid = Team<TH>::rank(), n = row.full();
     for (int i0 = 0; i0 < n; i0 += U * TH) {
-        uint4 v[U];
+        chunk_t v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
 #pragma unroll
@@ -853,7 +865,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
     };
     const int ei = row.end_index(tid);
     if (ei >= 0) Store<T>::store(d + ei, one(Store<T>::load(row.z + ei)));
-    each_chunk<T, TH, U>(row, [&](int ch, const uint4& v) {
+    each_chunk<T, TH, U>(row, [&](int ch, const chunk_t& v) {
         float x[E];
         Chunk<T>::unpack(v, x);
 #pragma unroll
@@ -892,13 +904,12 @@ struct Distill {
 struct Teacher { float Q, rest, qlogq; };
 
 // the list of a row, by W = 16 or 64 lanes: loaded (before the row's own loads, and not looked at yet, so that those stay in flight while
-// the list is worked on), then a token (-1: empty slot, V: no token of the row) and a mass for each of a lane's slots lane + W i
+// the list is worked on), then in LDS a token (-1: empty
+// slot, V: no token of the row) and a mass for each slot
 template <int W> struct List {
     static constexpr int J = (AG_LOGITS_MAX_TOP + W - 1) / W;
     int64_t raw_id[J];
     uint32_t raw_lp[J];
-    int id[J];
-    float q[J];
     static __device__ __forceinline__ int lane() { return threadIdx.x & (W - 1); }
     __device__ __forceinline__ void load(const Distill& p, int64_t r) {
 #pragma unroll
@@ -908,13 +919,15 @@ template <int W> struct List {
             raw_lp[i] = p.dtype == AG_BF16 ? ((const bf16_t*)p.logp)[j] : ((const uint32_t*)p.logp)[j];
         }
     }
-    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int V) {
+    // -> LDS sid, sq
+    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int V, int* sid, float* sq) const {
         float lp[J], m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < J; ++i) {
             const bool there = raw_id[i] >= 0 && lane() + i * W < p.K;
-            id[i] = !there ? -1 : raw_id[i] >= V ? V : (int)raw_id[i];
-            lp[i] = !there ? -INFINITY : id[i] == V ? NAN : __uint_as_float(p.dtype == AG_BF16 ? raw_lp[i] << 16 : raw_lp[i]);
+            const int id = !there ? -1 : raw_id[i] >= V ? V : (int)raw_id[i];
+            if (lane() + i * W < p.K) sid[lane() + i * W] = id;
+            lp[i] = !there ? -INFINITY : id == V ? NAN : __uint_as_float(p.dtype == AG_BF16 ? raw_lp[i] << 16 : raw_lp[i]);
             m = fmaxf(m, lp[i]);
         }
         m = lanes_join<W>(m, Max());
@@ -931,10 +944,11 @@ template <int W> struct List {
         float others = 0.f, top = 0.f;   // the masses that are not the largest, and how many are
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-            q[i] = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
-            t.Q += q[i];
-            t.qlogq += q[i] == 0.f ? 0.f : q[i] * lp[i];
-            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q[i]; }
+            const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
+            if (lane() + i * W < p.K) sq[lane() + i * W] = q;
+            t.Q += q;
+            t.qlogq += q == 0.f ? 0.f : q * lp[i];
+            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q; }
         }
         t.Q = lanes_join<W>(t.Q, Add());
         t.qlogq = lanes_join<W>(t.qlogq, Add());
@@ -945,6 +959,7 @@ template <int W> struct List {
             t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (top - 1.f) * expf(m) - others, 0.f);
             if (t.Q != t.Q) t.rest = t.Q;
         }
+        Team<W>::sync();
         return t;
     }
 };
@@ -952,26 +967,22 @@ template <int W> struct List {
 // what a row's gradient takes from the forward pass: g a exp2((z - m_off) c) off the list, g (on exp2((z - m) c) - q) on it
 struct GradOf { float m_off, a, m, on; };
 
-// The gradients of the listed tokens (W lanes; gx: their logits; bit i of `first`: this lane's i-th slot is known to be the first that names
-// its token).  Where a token may be listed more than once its masses are added up: the slots find that out from each other in LDS.
+// The gradients of the listed tokens (W lanes, slots lane + W i; gx: their logits' bits; bit i of `first`: this lane's i-th slot is known to be
+// the first that names its token).  Where a token may be listed more than once its masses are added up.
 template <typename T, int W>
-__device__ __forceinline__ void listed_gradients(const Row<T>& row, const List<W>& l, const float* gx, int K, uint32_t first, const GradOf& s, float g,
-                                                 float c, int* sid, float* sq, T* d) {
+__device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32_t* gx, int K, uint32_t first, const GradOf& s, float g, float c,
+                                                 const int* sid, const float* sq, T* d) {
     constexpr int J = List<W>::J;
+    const int lane = threadIdx.x & (W - 1);
+    const auto store = [&](int i, int at, float q) { Store<T>::store(d + at, g * (exp2_from(Row<T>::value(gx[i]), s.m, c) * s.on - q)); };
     uint32_t is = 0;
 #pragma unroll
-    for (int i = 0; i < J; ++i) is |= l.id[i] >= 0 && l.id[i] < row.V ? 1u << i : 0u;
+    for (int i = 0; i < J; ++i) is |= lane + i * W < K && sid[lane + i * W] >= 0 && sid[lane + i * W] < row.V ? 1u << i : 0u;
     if (__any(is != first)) {
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-            const int j = l.lane() + i * W;
-            if (j < K) { sid[j] = l.id[i]; sq[j] = l.q[i]; }
-        }
-        Team<W>::sync();
-#pragma unroll
-        for (int i = 0; i < J; ++i) {
-            const int j = l.lane() + i * W, at = l.id[i];
             if (!((is >> i) & 1u)) continue;
+            const int j = lane + i * W, at = sid[j];
             float q = 0.f;
             bool one = true;
 #pragma unroll 4
@@ -979,15 +990,15 @@ __device__ __forceinline__ void listed_gradients(const Row<T>& row, const List<W
                 q += sid[o] == at ? sq[o] : 0.f;
                 one &= sid[o] != at || o >= j;
             }
-            if (one) Store<T>::store(d + at, g * (exp2_from(gx[i], s.m, c) * s.on - q));
+            if (one) store(i, at, q);
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < J; ++i)
-        if ((is >> i) & 1u) Store<T>::store(d + l.id[i], g * (exp2_from(gx[i], s.m, c) * s.on - l.q[i]));
+        if ((is >> i) & 1u) store(i, sid[lane + i * W], sq[lane + i * W]);
 }
-template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const uint4& v, float c, const Ref& ref, float ga, T* d) {
+template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const chunk_t& v, float c, const Ref& ref, float ga, T* d) {
     constexpr int E = Chunk<T>::E;
     float x[E];
     Chunk<T>::unpack(v, x);
@@ -1042,11 +1053,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     if (part) row.load(x);
     int* sid = sid_lds[team];
     float* sq = sq_lds[team];
-    Teacher tc = mine.template finish<TAIL>(p, V);
-#pragma unroll
-    for (int i = 0; i < List<16>::J; ++i)
-        if (lane + 16 * i < p.K) { sid[lane + 16 * i] = mine.id[i]; sq[lane + 16 * i] = mine.q[i]; }
-    G::sync();
+    Teacher tc = mine.template finish<TAIL>(p, V, sid, sq);
     float q[NE] = {};
     uint32_t listed = 0;     // bit j: element j is on the list
     for (int j = 0; j < p.K; ++j) {
@@ -1109,7 +1116,7 @@ template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
     const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
     T* __restrict__ dz, int64_t ldd) {
-    constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1, BITS = 32 / E;   // chunks whose bits share a word
+    constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1;
     constexpr int J = List<64>::J, ROUND = NC * TH;
     extern __shared__ uint32_t bits_lds[];
     __shared__ float red[3 * (TH / 64)];
@@ -1119,27 +1126,33 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
     const int team = Team<TH>::index(), tid = Team<TH>::rank();
     const bool lead = TH == 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
     const int64_t stride = (int64_t)gridDim.x * PER;
+    int* sid = sid_lds[team];
+    float* sq = sq_lds[team];
     uint32_t* bits = bits_lds + team * bit_words<T>(V);   // logit i of the row: bit i + sh, set where it is listed
     for (int i = tid; i < bit_words<T>(V); i += TH) bits[i] = 0u;
     Team<TH>::sync();
-    // the first row from r on that takes part (of those that do not: no loss, no gradient)
-    const auto next_row = [&](int64_t r) {
-        for (; r < N; r += stride) {
-            if (!p.weights || p.weights[r] != 0.f) break;
+    const auto weight = [&](int64_t r) { return p.weights ? scalar_load(p.weights + r) : p.weight0; };
+    // the first row from r on that takes part (of those that do not: no loss, no gradient); w: row r's weight, then that row's
+    const auto next_row = [&](int64_t r, float& w) {
+        for (; r < N && w == 0.f; w = weight(min(r += stride, (int64_t)N - 1))) {
             if (tid == 0) row_loss[r] = 0.f;
             if (!GRAD && tid < 4) stats[r * 4 + tid] = 0.f;
             if (GRAD) zero_row<T, TH>(Row<T>(z + r * ld, V), dz + r * ldd);
         }
         return r;
     };
-    int64_t r = next_row((int64_t)blockIdx.x * PER + team);
+    int64_t r = (int64_t)blockIdx.x * PER + team;
     if (r >= N) return;
+    float w = weight(r);
+    r = next_row(r, w);
+    if (r >= N) return;
+    float w2 = weight(min(r + stride, (int64_t)N - 1));
     List<64> mine;
-    uint4 v[NC];
+    chunk_t v[NC];
     if (lead) mine.load(p, r);
     Row<T> row(z + r * ld, V);
-    int ei = row.end_index(tid);
-    float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
+    // (of the logits at a row's ends: the bits, read whether the thread has one or not)
+    uint32_t end = row.bits(max(row.end_index(tid), 0));
     {
         const int last = row.full() - 1;
 #pragma unroll
@@ -1152,22 +1165,23 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
         asm volatile("" : "+v"(t0));
         const int n = row.full();
         T* d = dz + r * ldd;
-        const float w = p.weights ? p.weights[r] : p.weight0;
-        const int64_t r2 = next_row(r + stride);
+        const int64_t r2 = next_row(r + stride, w2);
+        const float w3 = weight(min(r2 + stride, (int64_t)N - 1));
         const Row<T> row2(r2 < N ? z + r2 * ld : row.z, V);
         const int last2 = r2 < N ? row2.full() - 1 : 0;   // (no next row: its loads are one chunk of this one, again and again)
-        const int ei2 = row2.end_index(tid);
         Teacher tc = {0.f, 0.f, 0.f};
-        float gx[J];           // the logits of the slots' tokens
-        uint32_t first = 0;    // bit i: no earlier slot names the token of this lane's i-th
+        uint32_t gx[J];   // the slots' tokens' logits
+        uint32_t first = 0;    // bit i: this lane's i-th slot names a token that no earlier one does
+#pragma unroll
+        for (int i = 0; i < J; ++i) asm volatile("" : "=v"(gx[i]));   // (a register each: packed into one, they would be waited for at once)
         if (lead) {
-            tc = mine.template finish<TAIL>(p, V);
+            tc = mine.template finish<TAIL>(p, V, sid, sq);
 #pragma unroll
             for (int i = 0; i < J; ++i) {
-                const bool is = mine.id[i] >= 0 && mine.id[i] < V;
-                gx[i] = is ? Store<T>::load(row.z + mine.id[i]) : -INFINITY;
-                if (is) {
-                    const int at = mine.id[i] + row.sh;
+                const int id = tid + i * 64 < p.K ? sid[tid + i * 64] : -1;
+                gx[i] = row.bits(min(max(id, 0), V - 1));
+                if (id >= 0 && id < V) {
+                    const int at = id + row.sh;
                     const uint32_t b = 1u << (at & 31);
                     if (!(atomicOr(&bits[at >> 5], b) & b)) first |= 1u << i;
                 }
@@ -1181,7 +1195,8 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
             float y[E];
             Chunk<T>::unpack(v[i], y);
             if (TAIL) {
-                const uint32_t b = (bits[ch / BITS] >> ((ch % BITS) * E)) & ((1u << E) - 1u);
+                const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
+                const uint32_t b = E == 8 ? byte[ch] : (byte[ch >> 1] >> ((ch & 1) * 4)) & 15u;
                 if (b) {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
@@ -1198,25 +1213,26 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
                 v[i] = row.load(row.first + min(i0 + ROUND + i * TH + t0, n - 1));
             }
         }
-        float end2 = -INFINITY;
-        List<64> next;
+        uint32_t end2 = 0;
         if (!GRAD) {
-            if (lead) next.load(p, r2 < N ? r2 : r);
-            if (ei2 >= 0) end2 = Store<T>::load(row2.z + ei2);
+            if (lead) mine.load(p, r2 < N ? r2 : r);
+            end2 = row2.bits(max(row2.end_index(tid), 0));
         }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
+            asm volatile("" : "+v"(v[i]));   // (waited for whether it is added or not: the compiler then knows that all have come in)
             if (lastr + i * TH + t0 < n) add_chunk(i, row.first + lastr + i * TH + t0);
             if (!GRAD) v[i] = row2.load(row2.first + min(i * TH + t0, last2));
         }
-        if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(end);
+        const int ei = row.end_index(tid);
+        if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(Row<T>::value(end));
         if (TAIL && lead) {   // the listed tokens' part of the sums
             float lm = LG_NEG, ls = 0.f;
 #pragma unroll
-            for (int i = 0; i < J; ++i) lm = fmaxf(lm, gx[i]);
+            for (int i = 0; i < J; ++i) lm = fmaxf(lm, (first >> i) & 1u ? Row<T>::value(gx[i]) : LG_NEG);
             lm = lanes_join<64>(lm, Max());
 #pragma unroll
-            for (int i = 0; i < J; ++i) ls += (first >> i) & 1u ? exp2_from(gx[i], lm, c) : 0.f;
+            for (int i = 0; i < J; ++i) ls += (first >> i) & 1u ? exp2_from(Row<T>::value(gx[i]), lm, c) : 0.f;
             ls = lanes_join<64>(ls, Add());
             if (tid == 0) { said[team][2] = lm; said[team][3] = ls; }
         }
@@ -1236,7 +1252,10 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
             const float log_s = empty ? -INFINITY : logf(all.s);
             float cross = 0.f;
 #pragma unroll
-            for (int i = 0; i < J; ++i) cross += mine.q[i] == 0.f ? 0.f : mine.q[i] * (empty ? INFINITY : log_s - (gx[i] - all.m) * inv_t);
+            for (int i = 0; i < J; ++i) {
+                const float q = tid + i * 64 < p.K ? sq[tid + i * 64] : 0.f;
+                cross += q == 0.f ? 0.f : q * (empty ? INFINITY : log_s - (Row<T>::value(gx[i]) - all.m) * inv_t);
+            }
             cross = lanes_join<64>(cross, Add());
             if (tid == 0) {
                 row_loss[r] = Q != Q ? Q : row_loss_of<TAIL>(tc, cross, off, all, log_s, tau, inv_t);   // (an id beyond the row)
@@ -1244,38 +1263,40 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
             }
 #pragma unroll
             for (int i = 0; i < J; ++i)   // (every wave is done with them)
-                if (mine.id[i] >= 0 && mine.id[i] < V) bits[(mine.id[i] + row.sh) >> 5] = 0u;
+                if (tid + i * 64 < p.K && sid[tid + i * 64] >= 0 && sid[tid + i * 64] < V) bits[(sid[tid + i * 64] + row.sh) >> 5] = 0u;
         }
         if (GRAD) {
-            if (lead) next.load(p, r2 < N ? r2 : r);
-            if (ei2 >= 0) end2 = Store<T>::load(row2.z + ei2);
+            if (lead) mine.load(p, r2 < N ? r2 : r);
+            end2 = row2.bits(max(row2.end_index(tid), 0));
             const Ref ref(s.m_off, c);
             const float g = tau * w, ga = empty ? 0.f : g * s.a;
             asm volatile("" : "+v"(t1));
-            if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(end, ref.m, c));
+            if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Row<T>::value(end), ref.m, c));
             // the last round's chunks are still here; the rounds before it, then the next row's first round come in their places
             const auto round = [&](int i0, bool again) {
                 const T* from = again ? row.z + ((row.first + i0 - ROUND) * E - row.sh) : row2.z + (row2.first * E - row2.sh);
                 const int to = again ? ROUND - 1 : last2;
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
+                    // (a new value for the compiler: else it keeps the sums' unpacked logits, twice the chunks' registers, for the gradient)
+                    asm volatile("" : "+v"(v[i]));
                     if (i0 + i * TH + t1 < n) gradient_chunk(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
-                    v[i] = *reinterpret_cast<const uint4*>(from + min(i * TH + t1, to) * E);
+                    v[i] = *reinterpret_cast<const chunk_t*>(from + min(i * TH + t1, to) * E);
                 }
             };
             if (!MULTI) round(0, false);
             else
                 for (int i0 = lastr; i0 >= 0; i0 -= ROUND) round(i0, i0 > 0);
             Team<TH>::sync();
-            if (lead && !empty) listed_gradients<T, 64>(row, mine, gx, p.K, first, s, g, c, sid_lds[team], sq_lds[team], d);
+            if (lead && !empty) listed_gradients<T, 64>(row, gx, p.K, first, s, g, c, sid, sq, d);
         } else {
             Team<TH>::sync();   // (the first wave's words are read)
         }
         if (r2 >= N) break;
-        mine = next;
         r = r2;
+        w = w2;
+        w2 = w3;
         row = row2;
-        ei = ei2;
         end = end2;
     }
 }
@@ -1307,15 +1328,17 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     const float ga = g * s.a;
     const int ei = row.end_index(tid);
     if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
-    each_chunk<T, TH, U>(row, [&](int ch, const uint4& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
-    float gx[List<W>::J];
+    each_chunk<T, TH, U>(row, [&](int ch, const chunk_t& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
+    uint32_t gx[List<W>::J];
+    int* sid = sid_lds[team];
+    float* sq = sq_lds[team];
     if (lead) {
-        mine.template finish<TAIL>(p, V);
+        mine.template finish<TAIL>(p, V, sid, sq);
 #pragma unroll
-        for (int i = 0; i < List<W>::J; ++i) gx[i] = mine.id[i] >= 0 && mine.id[i] < V ? Store<T>::load(row.z + mine.id[i]) : -INFINITY;
+        for (int i = 0; i < List<W>::J; ++i) gx[i] = row.bits(min(max(sid[min(tid + i * W, p.K - 1)], 0), V - 1));
     }
     Team<TH>::sync();
-    if (lead) listed_gradients<T, W>(row, mine, gx, p.K, 0u, s, g, c, sid_lds[team], sq_lds[team], d);
+    if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, sid, sq, d);
 }
 
 // sum_n w_n L_n in a fixed order

@@ -901,62 +901,73 @@ struct Distill {
     float weight0;
 };
 
-struct Teacher { float Q, rest, qlogq; };
+struct Teacher { float Q, rest; };   // the mass on the list, and (with the tail) off it
 
-// the list of a row, by W = 16 or 64 lanes: loaded (before the row's own loads, and not looked at yet, so that those stay in flight while
-// the list is worked on), then in LDS a token (-1: empty
-// slot, V: no token of the row) and a mass for each slot
+// a row's list in LDS: token (-1: empty slot, V: no token of the row), mass, its logarithm
+struct ListLds {
+    int id[AG_LOGITS_MAX_TOP];
+    float q[AG_LOGITS_MAX_TOP], lq[AG_LOGITS_MAX_TOP];
+};
+
+// The list of a row, by W = 16 or 64 lanes (slots lane + W i): loaded before the row's own loads, and not looked at yet, so that those stay in
+// flight while the list is worked on.
 template <int W> struct List {
     static constexpr int J = (AG_LOGITS_MAX_TOP + W - 1) / W;
     int64_t raw_id[J];
     uint32_t raw_lp[J];
     static __device__ __forceinline__ int lane() { return threadIdx.x & (W - 1); }
-    __device__ __forceinline__ void load(const Distill& p, int64_t r) {
+    // f(i) for the rounds of slots that a list of K has
+    template <typename F> static __device__ __forceinline__ void each(int K, F f) {
 #pragma unroll
-        for (int i = 0; i < J; ++i) {
+        for (int i = 0; i < J; ++i)
+            if (i == 0 || i * W < K) f(i);
+    }
+    __device__ __forceinline__ void load(const Distill& p, int64_t r) {
+        each(p.K, [&](int i) {
             const int64_t j = r * p.K + min(lane() + i * W, p.K - 1);
             raw_id[i] = p.ids[j];
             raw_lp[i] = p.dtype == AG_BF16 ? ((const bf16_t*)p.logp)[j] : ((const uint32_t*)p.logp)[j];
-        }
+        });
     }
-    // -> LDS sid, sq
-    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int V, int* sid, float* sq) const {
+    template <bool TAIL> __device__ __forceinline__ Teacher finish(const Distill& p, int V, ListLds& lds) const {
         float lp[J], m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < J; ++i) {
-            const bool there = raw_id[i] >= 0 && lane() + i * W < p.K;
+        each(p.K, [&](int i) {
+            const int j = lane() + i * W;
+            const bool there = raw_id[i] >= 0 && j < p.K;
             const int id = !there ? -1 : raw_id[i] >= V ? V : (int)raw_id[i];
-            if (lane() + i * W < p.K) sid[lane() + i * W] = id;
+            if (j < p.K) lds.id[j] = id;
             lp[i] = !there ? -INFINITY : id == V ? NAN : __uint_as_float(p.dtype == AG_BF16 ? raw_lp[i] << 16 : raw_lp[i]);
             m = fmaxf(m, lp[i]);
-        }
+        });
         m = lanes_join<W>(m, Max());
+        Teacher t = {0.f, 0.f};
         if (!TAIL) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < J; ++i) s += lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
+            float e[J], s = 0.f;
+            each(p.K, [&](int i) {
+                e[i] = lp[i] == -INFINITY ? 0.f : expf(lp[i] - m);
+                s += e[i];
+            });
             s = lanes_join<W>(s, Add());
-            const float ls = logf(s);
-#pragma unroll
-            for (int i = 0; i < J; ++i) lp[i] = s == 0.f ? -INFINITY : (lp[i] - m) - ls;
-        }
-        Teacher t = {0.f, 0.f, 0.f};
-        float others = 0.f, top = 0.f;   // the masses that are not the largest, and how many are
-#pragma unroll
-        for (int i = 0; i < J; ++i) {
-            const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
-            if (lane() + i * W < p.K) sq[lane() + i * W] = q;
-            t.Q += q;
-            t.qlogq += q == 0.f ? 0.f : q * lp[i];
-            if (TAIL) { if (lp[i] == m) top += 1.f; else others += q; }
-        }
-        t.Q = lanes_join<W>(t.Q, Add());
-        t.qlogq = lanes_join<W>(t.qlogq, Add());
-        if (TAIL) {
-            // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
+            const float ls = logf(s), is = s == 0.f ? 0.f : 1.f / s;
+            each(p.K, [&](int i) {
+                const int j = lane() + i * W;
+                if (j < p.K) { lds.q[j] = e[i] * is; lds.lq[j] = (lp[i] - m) - ls; }
+            });
+            t.Q = s == 0.f ? 0.f : s * is;   // (1, or NaN)
+        } else {
+            float others = 0.f, top = 0.f;   // the masses that are not the largest, and how many are
+            each(p.K, [&](int i) {
+                const int j = lane() + i * W;
+                const float q = lp[i] == -INFINITY ? 0.f : expf(lp[i]);
+                if (j < p.K) { lds.q[j] = q; lds.lq[j] = lp[i]; }
+                if (lp[i] == m) top += 1.f; else others += q;
+            });
             top = lanes_join<W>(top, Add());
             others = lanes_join<W>(others, Add());
-            t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (top - 1.f) * expf(m) - others, 0.f);
+            const float q = m == -INFINITY ? 0.f : expf(m);
+            t.Q = m == -INFINITY ? others : fmaf(top, q, others);
+            // 1 - sum q without the cancellation against its largest term: -expm1 of that one, minus all the others
+            t.rest = m == -INFINITY ? 1.f : fmaxf(-expm1f(m) - (top - 1.f) * q - others, 0.f);
             if (t.Q != t.Q) t.rest = t.Q;
         }
         Team<W>::sync();
@@ -971,32 +982,29 @@ struct GradOf { float m_off, a, m, on; };
 // the first that names its token).  Where a token may be listed more than once its masses are added up.
 template <typename T, int W>
 __device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32_t* gx, int K, uint32_t first, const GradOf& s, float g, float c,
-                                                 const int* sid, const float* sq, T* d) {
-    constexpr int J = List<W>::J;
-    const int lane = threadIdx.x & (W - 1);
+                                                 const ListLds& l, T* d) {
+    const int lane = List<W>::lane();
     const auto store = [&](int i, int at, float q) { Store<T>::store(d + at, g * (exp2_from(Row<T>::value(gx[i]), s.m, c) * s.on - q)); };
     uint32_t is = 0;
-#pragma unroll
-    for (int i = 0; i < J; ++i) is |= lane + i * W < K && sid[lane + i * W] >= 0 && sid[lane + i * W] < row.V ? 1u << i : 0u;
+    List<W>::each(K, [&](int i) { is |= lane + i * W < K && l.id[lane + i * W] >= 0 && l.id[lane + i * W] < row.V ? 1u << i : 0u; });
     if (__any(is != first)) {
-#pragma unroll
-        for (int i = 0; i < J; ++i) {
-            if (!((is >> i) & 1u)) continue;
-            const int j = lane + i * W, at = sid[j];
+        List<W>::each(K, [&](int i) {
+            if (!((is >> i) & 1u)) return;
+            const int j = lane + i * W, at = l.id[j];
             float q = 0.f;
             bool one = true;
 #pragma unroll 4
             for (int o = 0; o < K; ++o) {
-                q += sid[o] == at ? sq[o] : 0.f;
-                one &= sid[o] != at || o >= j;
+                q += l.id[o] == at ? l.q[o] : 0.f;
+                one &= l.id[o] != at || o >= j;
             }
             if (one) store(i, at, q);
-        }
+        });
         return;
     }
-#pragma unroll
-    for (int i = 0; i < J; ++i)
-        if ((is >> i) & 1u) store(i, sid[lane + i * W], sq[lane + i * W]);
+    List<W>::each(K, [&](int i) {
+        if ((is >> i) & 1u) store(i, l.id[lane + i * W], l.q[lane + i * W]);
+    });
 }
 template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const chunk_t& v, float c, const Ref& ref, float ga, T* d) {
     constexpr int E = Chunk<T>::E;
@@ -1025,8 +1033,9 @@ template <bool TAIL> __device__ __forceinline__ GradOf row_gradient(const Teache
     s.a = !TAIL ? s.on : off.s == 0.f ? 0.f : s.on * __builtin_amdgcn_exp2f((off.m - all.m) * c) - tc.rest / off.s;
     return s;
 }
-template <bool TAIL> __device__ __forceinline__ float row_loss_of(const Teacher& tc, float cross, const Acc& off, const Acc& all, float log_s, float tau, float inv_t) {
-    float L = tc.qlogq + cross;
+// kl: the listed tokens' sum of q (ln q - ln p)
+template <bool TAIL> __device__ __forceinline__ float row_loss_of(const Teacher& tc, float kl, const Acc& off, const Acc& all, float log_s, float tau, float inv_t) {
+    float L = tc.Q != tc.Q ? tc.Q : kl;   // (an id beyond the row)
     if (TAIL && tc.rest != 0.f) L += tc.rest * (logf(tc.rest) - (off.s == 0.f ? -INFINITY : (off.m - all.m) * inv_t + logf(off.s) - log_s));
     return tau * tau * L;
 }
@@ -1038,8 +1047,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     using S = Small<T, 16>;
     using G = Team<16>;
     constexpr int NE = S::NE;
-    __shared__ int sid_lds[16][AG_LOGITS_MAX_TOP];
-    __shared__ float sq_lds[16][AG_LOGITS_MAX_TOP];
+    __shared__ ListLds list_lds[16];
     const int team = threadIdx.x / 16, lane = G::rank();
     const int64_t r = (int64_t)blockIdx.x * 16 + team;
     if (r >= N) return;
@@ -1051,17 +1059,16 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     mine.load(p, r);
     float x[NE];
     if (part) row.load(x);
-    int* sid = sid_lds[team];
-    float* sq = sq_lds[team];
-    Teacher tc = mine.template finish<TAIL>(p, V, sid, sq);
-    float q[NE] = {};
+    const ListLds& l = list_lds[team];
+    Teacher tc = mine.template finish<TAIL>(p, V, list_lds[team]);
+    float q[NE] = {}, qlq = 0.f;   // the masses of the lane's tokens, and of their slots the sum of q ln q
     uint32_t listed = 0;     // bit j: element j is on the list
     for (int j = 0; j < p.K; ++j) {
-        const int id = sid[j];
-        const float m = sq[j];
+        const int id = l.id[j];
+        const float m = l.q[j], lm = m == 0.f ? 0.f : m * l.lq[j];
 #pragma unroll
         for (int e = 0; e < NE; ++e)
-            if (id == row.index(e)) { q[e] += m; listed |= 1u << e; }
+            if (id == row.index(e)) { q[e] += m; qlq += lm; listed |= 1u << e; }
     }
     if (TAIL && (int)G::sum((float)__popc(listed), nullptr) >= V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
     if (!part) {   // the row takes no part
@@ -1088,13 +1095,13 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     all.s = TAIL ? G::sum(all.s, nullptr) + rebase(off, all.m, c).s : off.s;
     const bool empty = all.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(all.s);
-    float cross = 0.f;
+    float kl = qlq;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) cross += q[e] == 0.f ? 0.f : q[e] * (empty ? INFINITY : log_s - (x[e] - all.m) * inv_t);
-    cross = G::sum(cross, nullptr);
+    for (int e = 0; e < NE; ++e) kl += q[e] == 0.f ? 0.f : q[e] * (empty ? INFINITY : log_s - (x[e] - all.m) * inv_t);
+    kl = G::sum(kl, nullptr);
     const GradOf s = row_gradient<TAIL>(tc, off, all, c);
     if (lane == 0) {
-        row_loss[r] = tc.Q != tc.Q ? tc.Q : row_loss_of<TAIL>(tc, cross, off, all, log_s, tau, inv_t);
+        row_loss[r] = row_loss_of<TAIL>(tc, kl, off, all, log_s, tau, inv_t);
         if (!GRAD) *reinterpret_cast<float4*>(stats + r * 4) = make_float4(s.m_off, s.a, s.m, s.on);
     }
     if (!GRAD) return;
@@ -1120,14 +1127,12 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
     constexpr int J = List<64>::J, ROUND = NC * TH;
     extern __shared__ uint32_t bits_lds[];
     __shared__ float red[3 * (TH / 64)];
-    __shared__ int sid_lds[PER][AG_LOGITS_MAX_TOP];
-    __shared__ float sq_lds[PER][AG_LOGITS_MAX_TOP];
+    __shared__ ListLds list_lds[PER];
     __shared__ float said[PER][4];   // the first wave's word: mass on the list, the rest; the listed logits' largest, their exponentials' sum
     const int team = Team<TH>::index(), tid = Team<TH>::rank();
     const bool lead = TH == 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
     const int64_t stride = (int64_t)gridDim.x * PER;
-    int* sid = sid_lds[team];
-    float* sq = sq_lds[team];
+    ListLds& l = list_lds[team];
     uint32_t* bits = bits_lds + team * bit_words<T>(V);   // logit i of the row: bit i + sh, set where it is listed
     for (int i = tid; i < bit_words<T>(V); i += TH) bits[i] = 0u;
     Team<TH>::sync();
@@ -1169,26 +1174,23 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
         const float w3 = weight(min(r2 + stride, (int64_t)N - 1));
         const Row<T> row2(r2 < N ? z + r2 * ld : row.z, V);
         const int last2 = r2 < N ? row2.full() - 1 : 0;   // (no next row: its loads are one chunk of this one, again and again)
-        Teacher tc = {0.f, 0.f, 0.f};
+        Teacher tc = {0.f, 0.f};
         uint32_t gx[J];   // the slots' tokens' logits
         uint32_t first = 0;    // bit i: this lane's i-th slot names a token that no earlier one does
-#pragma unroll
-        for (int i = 0; i < J; ++i) asm volatile("" : "=v"(gx[i]));   // (a register each: packed into one, they would be waited for at once)
+        int at[J] = {};
         if (lead) {
-            tc = mine.template finish<TAIL>(p, V, sid, sq);
-#pragma unroll
-            for (int i = 0; i < J; ++i) {
-                const int id = tid + i * 64 < p.K ? sid[tid + i * 64] : -1;
-                gx[i] = row.bits(min(max(id, 0), V - 1));
-                if (id >= 0 && id < V) {
-                    const int at = id + row.sh;
-                    const uint32_t b = 1u << (at & 31);
-                    if (!(atomicOr(&bits[at >> 5], b) & b)) first |= 1u << i;
-                }
-            }
+            tc = mine.template finish<TAIL>(p, V, l);
+            List<64>::each(p.K, [&](int i) {
+                const int id = tid + i * 64 < p.K ? l.id[tid + i * 64] : -1;
+                if (id < 0 || id >= V) return;
+                at[i] = id;
+                const uint32_t b = 1u << ((id + row.sh) & 31);
+                if (!(atomicOr(&bits[(id + row.sh) >> 5], b) & b)) first |= 1u << i;
+            });
             if (TAIL && TH == 64 && (int)lanes_join<64>((float)__popc(first), Add()) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
-            if (tid == 0) { said[team][0] = tc.Q; said[team][1] = tc.rest; }
+            if (TH > 64 && tid == 0) { said[team][0] = tc.Q; said[team][1] = tc.rest; }
         }
+        List<64>::each(p.K, [&](int i) { gx[i] = row.bits(at[i]); });   // (by all waves: a load that nothing waits for)
         if (TAIL) Team<TH>::sync();
         Sums<T, false> sums(c);
         const auto add_chunk = [&](int i, int ch) {
@@ -1226,44 +1228,41 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
         }
         const int ei = row.end_index(tid);
         if (ei >= 0 && !(TAIL && (bits[(ei + row.sh) >> 5] >> ((ei + row.sh) & 31) & 1u))) sums.add_one(Row<T>::value(end));
+        Acc listed = {LG_NEG, 0.f, 0.f};
         if (TAIL && lead) {   // the listed tokens' part of the sums
-            float lm = LG_NEG, ls = 0.f;
-#pragma unroll
-            for (int i = 0; i < J; ++i) lm = fmaxf(lm, (first >> i) & 1u ? Row<T>::value(gx[i]) : LG_NEG);
-            lm = lanes_join<64>(lm, Max());
-#pragma unroll
-            for (int i = 0; i < J; ++i) ls += (first >> i) & 1u ? exp2_from(Row<T>::value(gx[i]), lm, c) : 0.f;
-            ls = lanes_join<64>(ls, Add());
-            if (tid == 0) { said[team][2] = lm; said[team][3] = ls; }
+            List<64>::each(p.K, [&](int i) { listed.m = fmaxf(listed.m, (first >> i) & 1u ? Row<T>::value(gx[i]) : LG_NEG); });
+            listed.m = lanes_join<64>(listed.m, Max());
+            List<64>::each(p.K, [&](int i) { listed.s += (first >> i) & 1u ? exp2_from(Row<T>::value(gx[i]), listed.m, c) : 0.f; });
+            listed.s = lanes_join<64>(listed.s, Add());
+            if (TH > 64 && tid == 0) { said[team][2] = listed.m; said[team][3] = listed.s; }
         }
         const Acc off = team_join<TH>(sums.acc(), c, red);
-        if (TH == 64) Team<TH>::sync();
-        const float Q = said[team][0], rest = said[team][1];
+        if (TH > 64) {
+            tc = {said[team][0], said[team][1]};
+            if (TAIL) listed = {said[team][2], said[team][3], 0.f};
+        }
         Acc all = off;
         if (TAIL) {
-            const Acc listed = {said[team][2], said[team][3], 0.f};
             const float m = fmaxf(off.m, listed.m);
             all = rebase(off, m, c);
             all.s += rebase(listed, m, c).s;
         }
         const bool empty = all.s == 0.f;
-        const GradOf s = row_gradient<TAIL>({Q, rest, 0.f}, off, all, c);
+        const GradOf s = row_gradient<TAIL>(tc, off, all, c);
         if (lead) {
             const float log_s = empty ? -INFINITY : logf(all.s);
-            float cross = 0.f;
-#pragma unroll
-            for (int i = 0; i < J; ++i) {
-                const float q = tid + i * 64 < p.K ? sq[tid + i * 64] : 0.f;
-                cross += q == 0.f ? 0.f : q * (empty ? INFINITY : log_s - (Row<T>::value(gx[i]) - all.m) * inv_t);
-            }
-            cross = lanes_join<64>(cross, Add());
+            float kl = 0.f;
+            List<64>::each(p.K, [&](int i) {
+                const int j = tid + i * 64;
+                const float q = j < p.K ? l.q[j] : 0.f;
+                kl += q == 0.f ? 0.f : q * (empty ? INFINITY : l.lq[j] + log_s - (Row<T>::value(gx[i]) - all.m) * inv_t);
+                if (j < p.K && l.id[j] >= 0 && l.id[j] < V) bits[(l.id[j] + row.sh) >> 5] = 0u;   // (every wave is done with them)
+            });
+            kl = lanes_join<64>(kl, Add());
             if (tid == 0) {
-                row_loss[r] = Q != Q ? Q : row_loss_of<TAIL>(tc, cross, off, all, log_s, tau, inv_t);   // (an id beyond the row)
+                row_loss[r] = row_loss_of<TAIL>(tc, kl, off, all, log_s, tau, inv_t);
                 if (!GRAD) *reinterpret_cast<float4*>(stats + r * 4) = make_float4(s.m_off, s.a, s.m, s.on);
             }
-#pragma unroll
-            for (int i = 0; i < J; ++i)   // (every wave is done with them)
-                if (tid + i * 64 < p.K && sid[tid + i * 64] >= 0 && sid[tid + i * 64] < V) bits[(sid[tid + i * 64] + row.sh) >> 5] = 0u;
         }
         if (GRAD) {
             if (lead) mine.load(p, r2 < N ? r2 : r);
@@ -1288,7 +1287,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6
             else
                 for (int i0 = lastr; i0 >= 0; i0 -= ROUND) round(i0, i0 > 0);
             Team<TH>::sync();
-            if (lead && !empty) listed_gradients<T, 64>(row, gx, p.K, first, s, g, c, sid, sq, d);
+            if (lead && !empty) listed_gradients<T, 64>(row, gx, p.K, first, s, g, c, l, d);
         } else {
             Team<TH>::sync();   // (the first wave's words are read)
         }
@@ -1306,8 +1305,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                                                                           const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
     constexpr int U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1, W = TH < 64 ? TH : 64;
-    __shared__ int sid_lds[PER][AG_LOGITS_MAX_TOP];
-    __shared__ float sq_lds[PER][AG_LOGITS_MAX_TOP];
+    __shared__ ListLds list_lds[PER];
     const int team = Team<TH>::index(), tid = Team<TH>::rank();
     const bool lead = TH <= 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
     const int64_t r = (int64_t)blockIdx.x * PER + team;
@@ -1330,15 +1328,12 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
     each_chunk<T, TH, U>(row, [&](int ch, const chunk_t& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
     uint32_t gx[List<W>::J];
-    int* sid = sid_lds[team];
-    float* sq = sq_lds[team];
     if (lead) {
-        mine.template finish<TAIL>(p, V, sid, sq);
-#pragma unroll
-        for (int i = 0; i < List<W>::J; ++i) gx[i] = row.bits(min(max(sid[min(tid + i * W, p.K - 1)], 0), V - 1));
+        mine.template finish<TAIL>(p, V, list_lds[team]);
+        List<W>::each(p.K, [&](int i) { gx[i] = row.bits(min(max(list_lds[team].id[min(tid + i * W, p.K - 1)], 0), V - 1)); });
     }
     Team<TH>::sync();
-    if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, sid, sq, d);
+    if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, list_lds[team], d);
 }
 
 // sum_n w_n L_n in a fixed order
@@ -1346,9 +1341,17 @@ __global__ __launch_bounds__(1024) void weighted_sum_kernel(const float* __restr
                                                             float* __restrict__ loss) {
     __shared__ double red[16];
     double acc = 0.0;
-    for (int i = threadIdx.x; i < N; i += 1024) {
-        const float w = weights ? weights[i] : weight0;
-        if (w != 0.f) acc += (double)w * (double)row_loss[i];
+    for (int i0 = threadIdx.x; i0 < N; i0 += 8 * 1024) {   // (eight loads of each array in flight)
+        float w[8], v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = min(i0 + u * 1024, N - 1);
+            w[u] = weights ? weights[i] : weight0;
+            v[u] = row_loss[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * 1024 < N && w[u] != 0.f) acc += (double)w[u] * (double)v[u];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);

@@ -465,10 +465,10 @@ template <typename T, int TH> __device__ __forceinline__ void place_all(TopLds<T
 }
 
 template <typename T>
-__device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
+__device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, int64_t N, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
                                           float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats) {
-    stats[r * 2] = a.m;
-    stats[r * 2 + 1] = a.s;
+    stats[r] = a.m;
+    stats[N + r] = a.s;
     lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
     entropy[r] = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
     if (tokens) {
@@ -480,29 +480,11 @@ __device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_
     }
 }
 
-#ifndef LG_DB
-#define LG_DB 1
-#endif
-#ifndef LG_B0
-#define LG_B0 32
-#endif
-#ifndef LG_U
-#define LG_U 2
-#endif
-#ifndef LG_MINW
-#define LG_MINW 7
-#endif
-#ifndef LG_B1
-#define LG_B1 32
-#endif
-#ifndef LG_B2
-#define LG_B2 64
-#endif
 template <typename T, int TH, bool TOP>
-__global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
+__global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                          int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
                                                          float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
-    constexpr int E = Chunk<T>::E, U = LG_U;   // U chunks of a lane are in flight
+    constexpr int E = Chunk<T>::E, U = 2;   // 2 U chunks of a lane are in flight
     __shared__ float red[3 * (TH / 64)];
     const int64_t r = blockIdx.x;
     const Row<T> row(z + r * ld, V);
@@ -518,19 +500,13 @@ __global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __res
 #pragma unroll
         for (int u = 0; u < U; ++u) to[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
     };
-#if LG_DB
     fetch(v, 0);
-#endif
     const float end = ei >= 0 ? Store<T>::load(row.z + ei) : -INFINITY;
     for (int i0 = 0; i0 < n; i0 += LG_SLOTS * TH) {
 #pragma unroll
         for (int i = 0; i < LG_SLOTS; i += U) {
             if (i0 + i * TH >= n) break;
-#if LG_DB
             fetch(w, i0 + (i + U) * TH);
-#else
-            fetch(v, i0 + i * TH);
-#endif
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (i0 + (i + u) * TH + tid < n) {
@@ -541,17 +517,15 @@ __global__ __launch_bounds__(TH, LG_MINW) void logprobs_wg_kernel(const T* __res
                     sums.add(x, cmax);
                 }
             }
-#if LG_DB
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u] = w[u];
-#endif
         }
     }
     if (ei >= 0) sums.add_one(end);
     const Acc a = team_join<TH>(sums.acc(), c, red);
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (tid == 0) write_row(row.z, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (tid == 0) write_row(row.z, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
     if (!TOP) return;
     __shared__ TopLds<TH> lds;
     constexpr int CAP = TopLds<TH>::CAP;
@@ -711,7 +685,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
     a.t = lanes_join<W>(a.t, Add());
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (lane == 0) write_row(zr, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (lane == 0) write_row(zr, V, r, N, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
     if (!TOP) return;
     __shared__ unsigned long long cand_lds[256 / W][CAP];
     unsigned long long* cand = cand_lds[team];
@@ -847,7 +821,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
     const int tid = Team<TH>::rank();
     const Row<T> row(z + r * ld, V);
     T* d = dz + r * ldd;
-    const Acc a = {q.stats[r * 2], q.stats[r * 2 + 1], 0.f};
+    const Acc a = {q.stats[r], q.stats[N + r], 0.f};
     const int64_t t = q.tokens ? q.tokens[r] : -1;
     const float gt = t < 0 ? 0.f : t < V ? q.g_logp[r] : NAN, gh = q.g_entropy ? q.g_entropy[r] : 0.f;
     float gs = 0.f;
@@ -1120,7 +1094,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 // The list is the first wave's: it works on it while the row arrives, marks the listed tokens for the sums of all waves, adds their own part,
 // and writes the loss and the listed tokens' gradients.  MULTI: rows of several rounds.
 template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD>
-__global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
+__global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
     const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
     T* __restrict__ dz, int64_t ldd) {
     constexpr int E = Chunk<T>::E, PER = TH < 256 ? 256 / TH : 1;
@@ -1411,11 +1385,11 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
                                      d_stats, d_top_ids, d_top_logp)
     const int chunks = V / Chunk<T>::E;
     if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
-    else if (V <= Small<T, 64>::max_v() && !(chunks >= 128 && 64 * min(chunks / 64, 4) >= k + k / 2)) LG_SMALL(64);
-    else if (N <= 256 && V > Small<T, 64>::max_v()) LG_WG(1024);
-    else if (chunks <= LG_B0 * 64) LG_WG(64);
-    else if (chunks <= LG_B1 * 256) LG_WG(256);
-    else if (chunks <= LG_B2 * 512) LG_WG(512);
+    else if (V <= Small<T, 64>::max_v() && (chunks < 16 || min(chunks, 64 * min(max(chunks / 64, 1), 4)) < k + k / 2)) LG_SMALL(64);
+    else if (N <= 256 && chunks >= 2048) LG_WG(1024);
+    else if (chunks <= 2048) LG_WG(64);
+    else if (chunks <= 8192) LG_WG(256);
+    else if (chunks <= 32768) LG_WG(512);
     else LG_WG(1024);
 #undef LG_SMALL
 #undef LG_WG
@@ -1459,6 +1433,7 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
         else LG_CALL(1024, 16, true, 1);
     } else {
         if (chunks <= 8 * 64) LG_CALL(64, 4, true, 6);
+        else if (N <= 256 && chunks >= 4096) LG_CALL(1024, 8, true, 1);
         else LG_CALL(256, 4, true, 6);
     }
 #undef LG_CALL

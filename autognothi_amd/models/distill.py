@@ -35,7 +35,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature):
         r = ops.token_logprobs(logits, tokens, top_k, temperature)
-        ctx.save_for_backward(logits, tokens, r.stats, r.entropy, r.top_ids)
+        ctx.save_for_backward(logits, tokens, r.stats, r.top_ids)
         ctx.temperature = r.temperature
         ctx.set_materialize_grads(False)
         if r.top_ids is not None:
@@ -47,8 +47,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, g_lse, _g_ids, g_top):
         if g_logp is None and g_entropy is None and g_lse is None and g_top is None:
             return None, None, None, None
-        logits, tokens, stats, entropy, top_ids = ctx.saved_tensors
-        fwd = ops.TokenLogprobs(None, entropy, None, top_ids, None, stats, ctx.temperature)
+        logits, tokens, stats, top_ids = ctx.saved_tensors
+        fwd = ops.TokenLogprobs(None, None, None, top_ids, None, stats, ctx.temperature)
         return ops.token_logprobs_bwd(logits, fwd, tokens, g_logp, g_entropy, g_lse, g_top), None, None, None
 
 

@@ -756,7 +756,7 @@ class TokenLogprobs(NamedTuple):
     lse: Tensor                   # [N] ln sum exp(logits / temperature)
     top_ids: Optional[Tensor]     # [N, top_k] int64, descending, ties by the lower index (None: top_k = 0)
     top_logp: Optional[Tensor]    # [N, top_k]
-    stats: Tensor                 # [N, 2]
+    stats: Tensor                 # [5, N]: logp, entropy, lse and two rows of its own
     temperature: float
 
 
@@ -764,7 +764,7 @@ class TopkDistill(NamedTuple):
     loss: Tensor                  # [1] sum of weights * row_loss
     row_loss: Tensor              # [N]
     dlogits: Optional[Tensor]     # [N, V] in the logits' dtype: d loss / d logits (None: not asked for)
-    stats: Tensor                 # [N, 4], what topk_distill_bwd reads
+    stats: Optional[Tensor]       # [N, 4], what topk_distill_bwd reads (None: the gradient is already here)
 
 
 def _logit_rows(who: str, logits: Tensor) -> Tuple[Tensor, int, int, int, int]:
@@ -816,15 +816,15 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
     dev = logits.device
     tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
     L.require_gpu(logits)
-    logp = torch.empty(n, dtype=torch.float32, device=dev) if tokens is not None else None
-    entropy, lse = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    stats = torch.empty((5, n), dtype=torch.float32, device=dev)      # (one allocation: at one row the host's time is the call's)
+    logp, entropy, lse, _, _ = stats.unbind(0)
+    at = stats.data_ptr()
     ids = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
     top = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
     with L.on(dev):
-        L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, L.ptr(logp), L.ptr(entropy),
-                                          L.ptr(lse), L.ptr(stats), L.ptr(ids), L.ptr(top), L.stream()))
-    return TokenLogprobs(logp, entropy, lse, ids, top, stats, temperature)
+        L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
+                                          L.ptr(ids), L.ptr(top), L.stream()))
+    return TokenLogprobs(None if tokens is None else logp, entropy, lse, ids, top, stats, temperature)
 
 
 def token_logprobs_bwd(logits: Tensor, fwd: TokenLogprobs, tokens: Optional[Tensor] = None, d_logp: Optional[Tensor] = None,
@@ -841,14 +841,15 @@ def token_logprobs_bwd(logits: Tensor, fwd: TokenLogprobs, tokens: Optional[Tens
     if d_top_logp is not None and k == 0:
         raise ValueError(f"{who}: d_top_logp without alternatives in the forward call")
     tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
-    stats, entropy = _row_arg(who, "stats", fwd.stats, (n, 2), f32, dev), _row_arg(who, "entropy", fwd.entropy, (n,), f32, dev)
+    stats = _row_arg(who, "stats", fwd.stats, (5, n), f32, dev)
+    at = stats.data_ptr()
     d_logp, d_entropy = _row_arg(who, "d_logp", d_logp, (n,), f32, dev), _row_arg(who, "d_entropy", d_entropy, (n,), f32, dev)
     d_lse, d_top = _row_arg(who, "d_lse", d_lse, (n,), f32, dev), _row_arg(who, "d_top_logp", d_top_logp, (n, k), f32, dev)
     ids = _row_arg(who, "top_ids", fwd.top_ids, (n, k), torch.int64, dev) if k else None
     L.require_gpu(logits)
     out = torch.empty((n, v), dtype=logits.dtype, device=dev)
     with L.on(dev):
-        L.check(L.lib().ag_token_logprobs_bwd(L.ptr(logits), ld, n, v, dtype, fwd.temperature, L.ptr(stats), L.ptr(entropy), L.ptr(tokens),
+        L.check(L.lib().ag_token_logprobs_bwd(L.ptr(logits), ld, n, v, dtype, fwd.temperature, at + 12 * n, at + 4 * n, L.ptr(tokens),
                                               L.ptr(d_logp), L.ptr(d_entropy), L.ptr(d_lse), k, L.ptr(ids), L.ptr(d_top), L.ptr(out), v,
                                               L.stream()))
     return out
@@ -881,7 +882,7 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
     L.require_gpu(logits)
     row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.float32, device=dev)
-    stats = torch.empty((n, 4), dtype=torch.float32, device=dev)
+    stats = None if want_grad else torch.empty((n, 4), dtype=torch.float32, device=dev)
     out = torch.empty((n, v), dtype=logits.dtype, device=dev) if want_grad else None
     with L.on(dev):
         L.check(L.lib().ag_topk_distill(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w), 1 if tail else 0,
@@ -892,7 +893,7 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
 def topk_distill_bwd(logits: Tensor, fwd: TopkDistill, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor] = None,
                      temperature: float = 1.0, tail: bool = False, d_loss: Optional[Tensor] = None, d_row_loss: Optional[Tensor] = None) -> Tensor:
     """the gradient apart from the loss: of d_loss [1] * loss + sum(d_row_loss [N] * row_loss) (both None: of the loss) -> [N, V] in the
-    logits' dtype; the other arguments as topk_distill had them."""
+    logits' dtype; ``fwd`` is of a call with want_grad=False, the other arguments as it had them."""
     who = "topk_distill_bwd"
     logits, n, v, ld, dtype = _logit_rows(who, logits)
     temperature = _check_temperature(who, temperature)
@@ -900,6 +901,8 @@ def topk_distill_bwd(logits: Tensor, fwd: TopkDistill, teacher_ids: Tensor, teac
     if n == 0:
         raise ValueError(f"{who}: no rows")
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
+    if fwd.stats is None:
+        raise ValueError(f"{who}: the forward call has computed the gradient (want_grad=True)")
     stats = _row_arg(who, "stats", fwd.stats, (n, 4), torch.float32, dev)
     d_loss = _row_arg(who, "d_loss", d_loss, (1,), torch.float32, dev)
     d_row = _row_arg(who, "d_row_loss", d_row_loss, (n,), torch.float32, dev)

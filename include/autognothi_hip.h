@@ -512,7 +512,7 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
 #define AG_LOGITS_MAX_TOP 128
 /* d_lse [N] = ln sum exp x;  d_entropy [N] = -sum p ln p;  d_logp [N] = ln p of d_tokens[n] (NULL: not asked for; a token < 0 is ignored: 0;
  * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
- * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0. */
+ * all), and their ln p;  d_stats [2, N]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0. */
 int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
                       float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp, void* stream);
 /* dlogits [N, V] (dtype, row stride ldd >= V) = the gradient of sum(d_g_logp . logp + d_g_entropy . entropy + d_g_lse . lse + d_g_top_logp . top_logp)
@@ -528,7 +528,8 @@ int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dt
  * tail != 0: the masses are taken as they are and rest = max(0, 1 - sum q_j) is a class of its own against p_off, the student's mass off the
  * list:  L_n = temperature^2 [ sum_j q_j (ln q_j - ln p_id_j) + rest (ln rest - ln p_off) ]   (rest = 0 if the list names every token).
  * d_loss [1] = sum_n w_n L_n with w = d_weights [N] (NULL: 1 / N); a row of weight 0 takes no part: its logits are not read, L_n and its
- * gradient are 0.  d_dlogits (optional): d loss / d logits in `dtype`.  d_stats [N, 4]: what ag_topk_distill_bwd reads.  A student row of
+ * gradient are 0.  d_dlogits (optional): d loss / d logits in `dtype`.  d_stats [N, 4]: what
+ * ag_topk_distill_bwd reads, written where d_dlogits is NULL.  A student row of
  * -inf: L = +inf where the teacher has mass, gradient 0. */
 int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
                     const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, float* d_row_loss, float* d_loss,

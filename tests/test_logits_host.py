@@ -64,11 +64,13 @@ def _call(fn, **kw):
     if fn == "token_logprobs":
         return ops.token_logprobs(**{**dict(logits=z, tokens=torch.zeros(3, dtype=torch.int64)), **kw})
     if fn == "token_logprobs_bwd":
-        fwd = ops.TokenLogprobs(None, torch.zeros(3), torch.zeros(3), None, None, torch.zeros(3, 2), 1.0)
+        fwd = ops.TokenLogprobs(None, torch.zeros(3), torch.zeros(3), None, None, torch.zeros(5, 3), 1.0)
         return ops.token_logprobs_bwd(**{**dict(logits=z, fwd=fwd, tokens=torch.zeros(3, dtype=torch.int64), d_logp=torch.zeros(3)), **kw})
     base = dict(logits=z, teacher_ids=torch.zeros(3, 2, dtype=torch.int64), teacher_logp=torch.zeros(3, 2))
     if fn == "topk_distill_bwd":
         base["fwd"] = ops.TopkDistill(None, None, None, torch.zeros(3, 4))
+    if isinstance(kw.get("fwd"), tuple):
+        kw = {**kw, "fwd": ops.TopkDistill(*kw["fwd"])}
     return getattr(ops, fn)(**{**base, **kw})
 
 
@@ -110,6 +112,7 @@ def test_refused_logits(fn, logits, exc, text):
     ("topk_distill", dict(teacher_logp=torch.zeros(3, 3)), ValueError, "teacher_logp must be"),
     ("topk_distill", dict(weights=torch.zeros(3, 1)), ValueError, "weights must be"),
     ("topk_distill", dict(logits=torch.zeros(0, 11), teacher_ids=torch.zeros(0, 2, dtype=torch.int64), teacher_logp=torch.zeros(0, 2)), ValueError, "no rows"),
+    ("topk_distill_bwd", dict(fwd=(None, None, None, None)), ValueError, "has computed the gradient"),
     ("topk_distill_bwd", dict(d_loss=torch.zeros(3)), ValueError, "d_loss must be"),
     ("topk_distill_bwd", dict(d_row_loss=torch.zeros(2)), ValueError, "d_row_loss must be")])
 def test_refused_arguments(fn, kw, exc, text):

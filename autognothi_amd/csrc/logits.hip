@@ -1152,6 +1152,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
         uint32_t gx[J];   // the slots' tokens' logits
         uint32_t first = 0;    // bit i: this lane's i-th slot names a token that no earlier one does
         int at[J] = {};
+        uint32_t again = 0;
         if (lead) {
             tc = mine.template finish<TAIL>(p, V, l);
             List<64>::each(p.K, [&](int i) {
@@ -1160,7 +1161,17 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
                 at[i] = id;
                 const uint32_t b = 1u << ((id + row.sh) & 31);
                 if (!(atomicOr(&bits[(id + row.sh) >> 5], b) & b)) first |= 1u << i;
+                else again = 1u;
             });
+            if (__any(again)) {   // a token listed twice: its first slot is the lower one, whichever came first just now
+                first = 0;
+                List<64>::each(p.K, [&](int i) {
+                    const int j = tid + i * 64, id = j < p.K ? l.id[j] : -1;
+                    bool is = id >= 0 && id < V;
+                    for (int o = 0; o < p.K; ++o) is &= l.id[o] != id || o >= j;
+                    if (is) first |= 1u << i;
+                });
+            }
             if (TAIL && TH == 64 && (int)lanes_join<64>((float)__popc(first), Add()) == V && tc.rest == tc.rest) tc.rest = 0.f;   // no token is off the list
             if (TH > 64 && tid == 0) { said[team][0] = tc.Q; said[team][1] = tc.rest; }
         }
@@ -1344,7 +1355,7 @@ int check_rows(const char* who, const void* d_logits, int64_t ld, int N, int V, 
     AG_REQUIRE(d_logits || N == 0, "%s: null pointer", who);
     AG_REQUIRE(dtype == AG_F32 || dtype == AG_BF16, "%s: dtype %d (AG_F32 or AG_BF16)", who, dtype);
     AG_REQUIRE(ld >= 0, "%s: row stride %lld", who, (long long)ld);
-    AG_REQUIRE(temperature > 0.f && temperature <= 3.0e38f, "%s: temperature %g (a positive number)", who, (double)temperature);
+    AG_REQUIRE(temperature >= 0x1p-20f && temperature <= 0x1p20f, "%s: temperature %g (2^-20 to 2^20)", who, (double)temperature);
     return AG_OK;
 }
 int check_teacher(const char* who, const void* ids, const void* t_logp, int t_dtype, int K, int N) {

@@ -52,12 +52,23 @@ class _TokenLogprobs(torch.autograd.Function):
         return ops.token_logprobs_bwd(logits, fwd, tokens, g_logp, g_entropy, g_lse, g_top), None, None, None
 
 
+def _rows(t: Optional[Tensor], dims: int) -> Optional[Tensor]:
+    """``t`` with its leading dimensions as one (``dims``: 2 for rows, 1 for a number per row); as it is where it has that form (a view would be a
+    node of the autograd graph)"""
+    if t is None or t.dim() == dims:
+        return t
+    return t.reshape(-1, t.shape[-1]) if dims == 2 else t.reshape(-1)
+
+
+def _back(t: Optional[Tensor], lead) -> Optional[Tensor]:
+    return t if t is None or len(lead) == 1 else t.view(*lead, *t.shape[1:])
+
+
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int = 0, temperature: float = 1.0) -> Logprobs:
     """``ops.token_logprobs`` on logits [..., V] and tokens [...] int64; every output but the ids is differentiable with respect to the logits."""
-    lead, v = logits.shape[:-1], logits.shape[-1]
-    logp, entropy, lse, ids, top = _TokenLogprobs.apply(logits.reshape(-1, v), None if tokens is None else tokens.reshape(-1), top_k, temperature)
-    return Logprobs(None if logp is None else logp.view(lead), entropy.view(lead), lse.view(lead), None if ids is None else ids.view(*lead, top_k),
-                    None if top is None else top.view(*lead, top_k))
+    lead = logits.shape[:-1]
+    out = _TokenLogprobs.apply(_rows(logits, 2), _rows(tokens, 1), top_k, temperature)
+    return Logprobs(*(_back(t, lead) for t in out))
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -84,7 +95,5 @@ def loss_topk_distillation(logits: Tensor, teacher_ids: Tensor, teacher_logp: Te
                            tail: bool = False) -> Tuple[Tensor, Tensor]:
     """``ops.topk_distill`` on logits [..., V], teacher_ids / teacher_logp [..., K] and weights [...] -> (loss, row losses [...]), both
     differentiable with respect to the logits (the teacher's record and the weights get no gradient)."""
-    lead, v, k = logits.shape[:-1], logits.shape[-1], teacher_ids.shape[-1]
-    loss, row = _TopkDistill.apply(logits.reshape(-1, v), teacher_ids.reshape(-1, k), teacher_logp.detach().reshape(-1, k),
-                                   None if weights is None else weights.detach().reshape(-1), temperature, tail)
-    return loss, row.view(lead)
+    loss, row = _TopkDistill.apply(_rows(logits, 2), _rows(teacher_ids, 2), _rows(teacher_logp, 2), _rows(weights, 1), temperature, tail)
+    return loss, _back(row, logits.shape[:-1])

@@ -800,8 +800,8 @@ def _row_arg(who: str, name: str, t: Optional[Tensor], shape: Tuple[int, ...], d
 
 def _check_temperature(who: str, temperature: float) -> float:
     t = float(temperature)
-    if not 0.0 < t < 3.0e38:
-        raise ValueError(f"{who}: temperature must be a positive number; got {temperature}")
+    if not 2.0 ** -20 <= t <= 2.0 ** 20:
+        raise ValueError(f"{who}: temperature must be between 2^-20 and 2^20; got {temperature}")
     return t
 
 

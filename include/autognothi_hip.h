@@ -504,8 +504,8 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
  * Wide rows of logits (csrc/logits.hip): log-probabilities of given tokens, and distillation from a teacher's top log-probabilities.
  * No counterpart in the reference, whose distillation (models/shapley.py:96-106, scripts/train_surrogate.py:133-147) compares the full
  * probability vectors of a handful of classes: these are the same quantities for a vocabulary, where the teacher is recorded as a list.
- * d_logits [N, V] in `dtype`, row stride ld elements (any alignment; 0 = one row for all), 1 <= V <= AG_LOGITS_MAX_V; x = z / temperature,
- * p = softmax(x), every sum in fp32.  A logit of -inf has probability 0; a row of nothing but -inf has no distribution (below); a NaN or
+ * d_logits [N, V] in `dtype`, row stride ld elements (any alignment; 0 = one row for all), 1 <= V <= AG_LOGITS_MAX_V; x = z / temperature
+ * (2^-20 to 2^20), p = softmax(x), every sum in fp32.  A logit of -inf has probability 0; a row of nothing but -inf has no distribution (below); a NaN or
  * +inf makes its row's results NaN.  Nothing is read back to the host; all calls can be captured.  Outputs must not alias inputs.
  * ---------------------------------------------------------------------------------------------- */
 #define AG_LOGITS_MAX_V 524288

@@ -177,6 +177,21 @@ def test_nan_and_inf_stay_in_their_row(cuda_device, dtype, v):
     assert np.isnan(dz[bad]).any(axis=1).all() and np.isfinite(dz[ok]).all()
 
 
+@pytest.mark.parametrize("tau", [1e-6, 1e-2, 100.0, 1e6])
+def test_temperatures_far_from_one(cuda_device, tau):
+    """x = z / tau reaches 1e7, where a product m / tau rounds to units and more, and 1e-5, where every row is nearly uniform"""
+    g = np.random.default_rng(17)
+    for n, v in ((4, 40), (3, 900), (3, 5000), (2, 40000)):
+        z, z64 = _logits(g, n, v, F32, cuda_device)
+        tokens = z64.argmax(axis=1)                       # (at 1e-6 every other token's probability is 0)
+        tau32 = float(np.float32(tau))
+        r = _check_forward(z, z64, tokens, 3, tau32)
+        _check_backward(z, z64, r, tokens, tau32, g)
+        if tau > 1e-3:
+            ids, lp, lp64 = _teacher(g, n, v, 5, 0.8, False, F32)
+            _check_distill(z, z64, ids, lp, lp64, tau32, True, None)
+
+
 def test_tokens_outside_the_row_are_nan_and_read_nothing(cuda_device):
     from autognothi_amd import ops
     z = torch.randn(4, 50, device=cuda_device)
@@ -425,17 +440,88 @@ def test_captured_replayed_and_repeated(cuda_device, v):
                 assert torch.equal(x, y)
 
 
+def test_captured_autograd(cuda_device):
+    """loss and gradient of the autograd forms in one graph, replayed on new logits with eager work between"""
+    from autognothi_amd import ops
+    from autognothi_amd.models import distill
+    n, v, k = 9, 5000, 12
+    gen = torch.Generator(cuda_device).manual_seed(1)
+    z = torch.randn(n, v, device=cuda_device, generator=gen).requires_grad_(True)
+    tokens = torch.randint(0, v, (n,), device=cuda_device, generator=gen)
+    rec = ops.token_logprobs(torch.randn(n, v, device=cuda_device, generator=gen), top_k=k)
+
+    def step(x):
+        loss, _ = distill.loss_topk_distillation(x, rec.top_ids, rec.top_logp, tail=True)
+        total = loss - 0.1 * distill.token_logprobs(x, tokens).logp.mean()
+        return total.detach(), torch.autograd.grad(total, x)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(z)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(z)
+    for _ in range(3):
+        new = torch.randn(n, v, device=cuda_device, generator=gen)
+        want = [t.clone() for t in step(new.clone().requires_grad_(True))]
+        with torch.no_grad():
+            z.copy_(new)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [20, 1000, 9000])
+def test_c_entries_write_their_rows_alone(cuda_device, dtype, v):
+    """gradient rows further apart than they are long, and results one row short of their buffers: nothing else is touched"""
+    from autognothi_amd import _lib as L, ops
+    lib, n, k, ldd = L.lib(), 5, 4, v + 9
+    T = L.AG_F32 if dtype == F32 else L.AG_BF16
+    z = torch.randn(n, v, device=cuda_device).to(dtype)
+    tok = torch.zeros(n, dtype=torch.int64, device=cuda_device)
+    r = ops.token_logprobs(z, tok, k)
+    ids = torch.full(((n + 1) * k,), 77, dtype=torch.int64, device=cuda_device)
+    top, st = torch.full(((n + 1) * k,), 7.0, device=cuda_device), torch.full((5 * n + 1,), 7.0, device=cuda_device)
+    a, s = st.data_ptr(), L.stream()
+    L.check(lib.ag_token_logprobs(z.data_ptr(), v, n, v, T, 1.0, tok.data_ptr(), k, a, a + 4 * n, a + 8 * n, a + 12 * n, ids.data_ptr(), top.data_ptr(), s))
+    assert torch.equal(st[: 5 * n].view(5, n), r.stats) and st[-1] == 7 and (ids[n * k:] == 77).all() and (top[n * k:] == 7).all()
+    want = ops.token_logprobs_bwd(z, r, tok, d_logp=torch.ones(n, device=cuda_device))
+    g = torch.ones(n, device=cuda_device)
+    d = torch.full((n, ldd), 7.0, device=cuda_device).to(dtype)
+    L.check(lib.ag_token_logprobs_bwd(z.data_ptr(), v, n, v, T, 1.0, a + 12 * n, a + 4 * n, tok.data_ptr(), g.data_ptr(), None, None, 0, None, None,
+                                      d.data_ptr(), ldd, s))
+    assert torch.equal(d[:, :v], want) and (d[:, v:] == 7).all()
+    lp = torch.log_softmax(torch.randn(n, k, device=cuda_device), 1)
+    w = torch.tensor([1.0, 0.0, 0.5, 1.0, 0.0], device=cuda_device)
+    row, loss = torch.full((n + 1,), 7.0, device=cuda_device), torch.full((2,), 7.0, device=cuda_device)
+    for tail in (0, 1):
+        want = ops.topk_distill(z, r.top_ids, lp, w, tail=bool(tail))
+        d.fill_(7.0)
+        L.check(lib.ag_topk_distill(z.data_ptr(), v, n, v, T, 1.0, r.top_ids.data_ptr(), lp.data_ptr(), 0, k, w.data_ptr(), tail, row.data_ptr(),
+                                    loss.data_ptr(), None, d.data_ptr(), ldd, s))
+        assert torch.equal(d[:, :v], want.dlogits) and (d[:, v:] == 7).all()
+        assert torch.equal(row[:n], want.row_loss) and row[n] == 7 and torch.equal(loss[:1], want.loss) and loss[1] == 7
+
+
 def test_other_streams_and_repeats_give_the_same_bits(cuda_device):
     from autognothi_amd import ops
     gen = torch.Generator(cuda_device).manual_seed(5)
     z = torch.randn(300, 20011, device=cuda_device, generator=gen).to(BF16)
     rec = ops.token_logprobs(z, top_k=50)
+    rec.top_ids[::3, 20:30] = rec.top_ids[::3, 40:50]      # (tokens listed twice)
     base = ops.topk_distill(z, rec.top_ids, rec.top_logp, tail=True)
     torch.cuda.synchronize()
     for _ in range(3):
         s = torch.cuda.Stream()
         with torch.cuda.stream(s):
             again, rep = ops.topk_distill(z, rec.top_ids, rec.top_logp, tail=True), ops.token_logprobs(z, top_k=50)
+            rep.top_ids[::3, 20:30] = rep.top_ids[::3, 40:50]
         s.synchronize()
         for x, y in zip((*again[:3], rep.top_ids, rep.top_logp, rep.lse), (*base[:3], rec.top_ids, rec.top_logp, rec.lse)):
             assert torch.equal(x, y)

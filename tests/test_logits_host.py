@@ -99,6 +99,7 @@ def test_refused_logits(fn, logits, exc, text):
     ("token_logprobs", dict(top_k=-1), ValueError, "top_k"), ("token_logprobs", dict(top_k=12), ValueError, "top_k"),
     ("token_logprobs", dict(logits=torch.zeros(3, 500), top_k=129), ValueError, "top_k"),
     ("token_logprobs", dict(temperature=0.0), ValueError, "temperature"), ("token_logprobs", dict(temperature=-1.0), ValueError, "temperature"),
+    ("token_logprobs", dict(temperature=1e-7), ValueError, "temperature"), ("topk_distill", dict(temperature=2e6), ValueError, "temperature"),
     ("token_logprobs", dict(temperature=float("nan")), ValueError, "temperature"), ("topk_distill", dict(temperature=float("inf")), ValueError, "temperature"),
     ("token_logprobs_bwd", dict(tokens=None), ValueError, "without tokens"),
     ("token_logprobs_bwd", dict(d_top_logp=torch.zeros(3, 2)), ValueError, "without alternatives"),

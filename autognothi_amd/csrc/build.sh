@@ -6,8 +6,8 @@ OUT=../lib
 mkdir -p "$OUT"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-variable"
-# no packed fp32 instructions in the sources compiled with these flags on top (scalar forms: the same bits)
-NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
+# no packed fp32 instructions (the scalar forms have the same bits; the host pass does not know the feature and says so)
+FLAGS="$FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops"
 OBJS=()
 PIDS=()
 for src in gemm.hip gemm_tn.hip gemm_big.hip side_mlp.hip probe.hip attention.hip cls_last.hip sampler.hip elementwise.hip shapley.hip logits.hip train.hip train_fused.hip encoder.cpp capi.cpp; do
@@ -15,8 +15,7 @@ for src in gemm.hip gemm_tn.hip gemm_big.hip side_mlp.hip probe.hip attention.hi
   if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ common.h -nt "$obj" ] || [ ../../include/autognothi_hip.h -nt "$obj" ]; then
     echo "hipcc $src"
     rm -f "$obj"          # a failed compile must not leave a stale object behind
-    case "$src" in logits.hip) MORE="$NOPK" ;; *) MORE="" ;; esac
-    $HIPCC $FLAGS $MORE -x hip -c "$src" -o "$obj" &
+    $HIPCC $FLAGS -x hip -c "$src" -o "$obj" &
     PIDS+=($!)
   fi
   OBJS+=("$obj")

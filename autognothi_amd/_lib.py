@@ -222,7 +222,7 @@ _BACKGROUND = {}     # device index -> the device's background stream, created A
 
 def background_stream(index: int):
     """The device's second stream for work that runs BESIDE the caller's (the two-stream training epoch: scripts/common.TrainPartition):
-    a torch high-priority stream that is created and given one trivial kernel at the library's FIRST launch on the device, and kept.
+    a torch stream of default priority (as all of this library) that is created and given one trivial kernel at the library's FIRST launch on the device, and kept.
     Measured (profiles/HISTORY.md §10): a HIP stream takes its hardware queue at its first submission, and a second stream that does
     so after the process has captured hipGraphs / made its other streams runs its kernels behind the caller's instead of beside them
     (the same two-stream schedule: 420 instead of 635 images/s, against 550 on one stream); one that did so first never does."""
@@ -230,7 +230,7 @@ def background_stream(index: int):
     st = _BACKGROUND.get(index)
     if st is None:
         dev = torch.device("cuda", index)
-        st = _BACKGROUND[index] = torch.cuda.Stream(dev, priority=-1)
+        st = _BACKGROUND[index] = torch.cuda.Stream(dev)
         with torch.cuda.stream(st):
             torch.zeros(1, device=dev).add_(1)
         st.synchronize()

@@ -182,7 +182,7 @@ class TrainPartition:
             ok = L.streams_overlap(main, self.fwd)
             tries = 0
             while not ok and tries < 6:
-                cand = torch.cuda.Stream(self.device, priority=-1)
+                cand = torch.cuda.Stream(self.device)
                 ok = L.streams_overlap(main, cand)
                 if ok:
                     self.fwd = cand

@@ -9,6 +9,7 @@
 // every whole chunk is one aligned load whatever the row stride is.  Sums are fp32 in a fixed order, no atomics: results are
 // bit-reproducible.
 #include "common.h"
+#include <algorithm>
 
 namespace {
 
@@ -375,8 +376,11 @@ struct TopOut {
     int k;
     float m, inv_t, log_s;
     bool empty;
+    unsigned long long* keys = nullptr;   // of a part of a row that starts at logit `base`: the keys instead, for the whole row
+    int base = 0;
     __device__ __forceinline__ void write(unsigned long long me, int place) const {
         if (place >= k) return;
+        if (keys) { keys[place] = me - (unsigned long long)base; return; }   // (the key's low half counts down)
         ids[place] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
         logp[place] = empty ? -INFINITY : (key_value((uint32_t)(me >> 32)) - m) * inv_t - log_s;
     }
@@ -480,14 +484,24 @@ __device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_
     }
 }
 
-template <typename T, int TH, bool TOP>
+// parts of rows, for few long ones: `count` workgroups a row, `length` logits each, that leave (m, s, t, -) and k keys to logprobs_join_kernel
+struct Parts {
+    int count, length;
+    float4* acc;
+    unsigned long long* keys;
+};
+
+template <typename T, int TH, bool TOP, bool PART>
 __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                          int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
-                                                         float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+                                                         float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp,
+                                                         Parts parts) {
     constexpr int E = Chunk<T>::E, U = 2;   // 2 U chunks of a lane are in flight
     __shared__ float red[3 * (TH / 64)];
-    const int64_t r = blockIdx.x;
-    const Row<T> row(z + r * ld, V);
+    const int64_t r = PART ? blockIdx.x / parts.count : blockIdx.x;
+    const int base = PART ? blockIdx.x % parts.count * parts.length : 0;
+    if (PART) V = min(parts.length, V - base);
+    const Row<T> row(z + r * ld + base, V);
     const int tid = threadIdx.x;
     Sums<T, true> sums(c);
     float slot[LG_SLOTS];
@@ -525,7 +539,11 @@ __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict_
     const Acc a = team_join<TH>(sums.acc(), c, red);
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (tid == 0) write_row(row.z, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (PART) {
+        if (tid == 0) parts.acc[blockIdx.x] = make_float4(a.m, a.s, a.t, 0.f);
+    } else if (tid == 0) {
+        write_row(row.z, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    }
     if (!TOP) return;
     __shared__ TopLds<TH> lds;
     constexpr int CAP = TopLds<TH>::CAP;
@@ -598,7 +616,29 @@ __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict_
         Team<TH>::sync();
     }
     if (whole) top_radix<T, TH>(row, k, lds);
-    place_all<T, TH>(lds, lds.n_cand, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
+    if (PART) place_all<T, TH>(lds, lds.n_cand, V, {nullptr, nullptr, k, 0.f, 0.f, 0.f, false, parts.keys + (int64_t)blockIdx.x * k, base});
+    else place_all<T, TH>(lds, lds.n_cand, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
+}
+
+// One wave a row: its parts' sums (at most 64) and keys (at most 256)
+template <typename T, bool TOP>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
+                                                           int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
+                                                           float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp,
+                                                           Parts parts) {
+    __shared__ unsigned long long cand[256];
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x, n = parts.count * k;
+    if (TOP)
+        for (int i = lane; i < n; i += 64) cand[i] = parts.keys[r * n + i];
+    const float4 p = parts.acc[r * parts.count + min(lane, parts.count - 1)];
+    const Acc mine = {lane < parts.count ? p.x : LG_NEG, lane < parts.count ? p.y : 0.f, lane < parts.count ? p.z : 0.f};
+    const Acc a = lanes_join<64>(mine, c);
+    const bool empty = a.s == 0.f;
+    const float log_s = empty ? -INFINITY : logf(a.s);
+    if (lane == 0) write_row(z + r * ld, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    Team<64>::sync();
+    if (TOP) place_wave<T>(cand, n, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
 }
 
 // Rows of up to 64 (W = 16 lanes a row) or 2041 / 2045 logits (W = 64): the whole row lives in registers, the maximum is found first.
@@ -1385,23 +1425,39 @@ template <typename T> int team_of(int V, int N) {
     }
 template <int TH> dim3 team_grid(int N) { return dim3(TH < 256 ? ceil_div(N, 256 / TH) : N); }
 
+// How many workgroups share a row: for few rows, of 32768 chunks and more, as many as the join takes (64 sums, 256 keys) and leave each 1024
+// chunks (256 threads, four rounds).  One row, 4 alternatives, kernels alone: 524288 fp32 logits 50.5 -> 13.6 us, 262144 fp32 31.2 -> 13.4,
+// 262144 bf16 23.9 -> 11.3, 131072 bf16 16.2 -> 10.4; the second launch and the workspace cost the host 5 us, so shorter rows stay whole.
+Parts parts_of(int N, int V, int dtype, int k) {
+    const int chunks = V / (dtype == AG_BF16 ? 8 : 4);
+    int count = std::min(std::min(64, chunks / 1024), std::min(k ? 256 / k : 64, 512 / std::max(N, 1)));
+    if (N < 1 || N > 64 || chunks < 32768 || count < 2) return {0, 0, nullptr, nullptr};
+    const int length = (ceil_div(V, count) + 63) / 64 * 64;
+    return {ceil_div(V, length), length, nullptr, nullptr};
+}
+
 template <typename T, bool TOP>
 int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_tokens, int k, float* d_logp, float* d_entropy, float* d_lse,
-             float* d_stats, int64_t* d_top_ids, float* d_top_logp, hipStream_t s) {
+             float* d_stats, int64_t* d_top_ids, float* d_top_logp, Parts parts, hipStream_t s) {
     const float c = log2e_over(temperature), inv_t = one_over(temperature);
     const T* z = (const T*)d_logits;
 #define LG_SMALL(W) hipLaunchKernelGGL((logprobs_small_kernel<T, W, TOP>), team_grid<W>(N), dim3(256), 0, s, z, ld, N, V, c, inv_t, d_tokens, k, d_logp, \
                                        d_entropy, d_lse, d_stats, d_top_ids, d_top_logp)
-#define LG_WG(TH) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP>), dim3(N), dim3(TH), 0, s, z, ld, V, c, inv_t, d_tokens, k, d_logp, d_entropy, d_lse, \
-                                     d_stats, d_top_ids, d_top_logp)
+#define LG_WG(TH, PART) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP, PART>), dim3(N * (PART ? parts.count : 1)), dim3(TH), 0, s, z, ld, V, c, inv_t, \
+                                           d_tokens, k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, parts)
     const int chunks = V / Chunk<T>::E;
-    if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
+    if (parts.count) {
+        LG_WG(256, true);
+        AG_LAUNCH_CHECK();
+        hipLaunchKernelGGL((logprobs_join_kernel<T, TOP>), dim3(N), dim3(64), 0, s, z, ld, V, c, inv_t, d_tokens, k, d_logp, d_entropy, d_lse, d_stats,
+                           d_top_ids, d_top_logp, parts);
+    } else if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
     else if (V <= Small<T, 64>::max_v() && (chunks < 16 || min(chunks, 64 * min(max(chunks / 64, 1), 4)) < k + k / 2)) LG_SMALL(64);
-    else if (N <= 256 && chunks >= 2048) LG_WG(1024);
-    else if (chunks <= 2048) LG_WG(64);
-    else if (chunks <= 8192) LG_WG(256);
-    else if (chunks <= 32768) LG_WG(512);
-    else LG_WG(1024);
+    else if (N <= 256 && chunks >= 2048) LG_WG(1024, false);
+    else if (chunks <= 2048) LG_WG(64, false);
+    else if (chunks <= 8192) LG_WG(256, false);
+    else if (chunks <= 32768) LG_WG(512, false);
+    else LG_WG(1024, false);
 #undef LG_SMALL
 #undef LG_WG
     AG_LAUNCH_CHECK();
@@ -1467,16 +1523,30 @@ int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperatur
 
 }  // namespace
 
+extern "C" size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int top_k) {
+    const Parts p = parts_of(N, V, dtype, top_k);
+    return (size_t)std::max(N, 0) * p.count * (sizeof(float4) + (size_t)std::max(top_k, 0) * sizeof(unsigned long long));
+}
+
 extern "C" int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
                                  float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp,
-                                 void* stream) {
+                                 void* d_workspace, size_t workspace_bytes, void* stream) {
     if (int rc = check_rows("ag_token_logprobs", d_logits, ld, N, V, dtype, temperature)) return rc;
     AG_REQUIRE(top_k >= 0 && top_k <= AG_LOGITS_MAX_TOP && top_k <= V, "ag_token_logprobs: top_k = %d (0 to min(%d, %d logits))", top_k,
                AG_LOGITS_MAX_TOP, V);
     if (N == 0) return AG_OK;
     AG_REQUIRE(d_entropy && d_lse && d_stats && (!d_tokens || d_logp) && (top_k == 0 || (d_top_ids && d_top_logp)), "ag_token_logprobs: null pointer");
+    const size_t need = ag_token_logprobs_workspace_bytes(N, V, dtype, top_k);
+    AG_REQUIRE(!d_workspace || (workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0), "ag_token_logprobs: workspace of %zu bytes (16-byte aligned, %zu needed)",
+               workspace_bytes, need);
+    Parts parts = {0, 0, nullptr, nullptr};
+    if (d_workspace && need) {
+        parts = parts_of(N, V, dtype, top_k);
+        parts.acc = (float4*)d_workspace;
+        parts.keys = (unsigned long long*)(parts.acc + (size_t)N * parts.count);
+    }
     const auto run = dtype == AG_BF16 ? (top_k ? logprobs<bf16_t, true> : logprobs<bf16_t, false>) : (top_k ? logprobs<float, true> : logprobs<float, false>);
-    return run(d_logits, ld, N, V, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, (hipStream_t)stream);
+    return run(d_logits, ld, N, V, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, parts, (hipStream_t)stream);
 }
 
 extern "C" int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const float* d_stats,

@@ -822,8 +822,10 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
     ids = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
     top = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
     with L.on(dev):
+        need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 64 else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
-                                          L.ptr(ids), L.ptr(top), L.stream()))
+                                          L.ptr(ids), L.ptr(top), L.ptr(ws), need, L.stream()))
     return TokenLogprobs(None if tokens is None else logp, entropy, lse, ids, top, stats, temperature)
 
 

@@ -126,8 +126,8 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
     lib = L.lib()
     x = 0x1000    # never read: every call below is refused on the host
 
-    def tl(n=1, v=8, dtype=0, ld=8, tau=1.0, k=0, z=x, ent=x, ids=None):
-        return lib.ag_token_logprobs(z, ld, n, v, dtype, tau, None, k, None, ent, x, x, ids, ids, None)
+    def tl(n=1, v=8, dtype=0, ld=8, tau=1.0, k=0, z=x, ent=x, ids=None, ws=None, have=0):
+        return lib.ag_token_logprobs(z, ld, n, v, dtype, tau, None, k, None, ent, x, x, ids, ids, ws, have, None)
 
     def bw(ldd=8, st=x, g=None):
         return lib.ag_token_logprobs_bwd(x, 8, 1, 8, 0, 1.0, st, x, None, g, None, None, 0, None, None, x, ldd, None)
@@ -139,7 +139,8 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
         return lib.ag_topk_distill_bwd(x, 8, n, 8, 0, 1.0, x, x, 0, k, None, 0, st, None, None, dz, ldd, None)
 
     for rc in (tl(n=-1), tl(v=0), tl(v=524289), tl(dtype=2), tl(ld=-1), tl(tau=0.0), tl(tau=float("nan")), tl(k=9), tl(k=-1), tl(z=None), tl(ent=None),
-               tl(k=2, ids=None), bw(ldd=7), bw(st=None), bw(g=x), di(n=0), di(k=0), di(k=129), di(ids=None), di(tdt=5), di(ldd=7), di(loss=None),
+               tl(k=2, ids=None),
+               tl(v=200000, ld=200000, ws=x, have=lib.ag_token_logprobs_workspace_bytes(1, 200000, 0, 0) - 1), tl(ws=x + 4), bw(ldd=7), bw(st=None), bw(g=x), di(n=0), di(k=0), di(k=129), di(ids=None), di(tdt=5), di(ldd=7), di(loss=None),
                di(tau=-1.0), db(n=0), db(k=0), db(st=None), db(ldd=7), db(dz=None)):
         assert rc < 0 and lib.ag_last_error()
     assert tl(n=0) == 0    # no rows: nothing to do

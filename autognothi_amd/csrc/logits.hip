@@ -824,17 +824,36 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // exponent), and a few places (the given token, the listed ones) where something is added: those are written again once the row is done.
 // One read and one write of the row; a lane has U chunks in flight.
 
-// f(chunk, its 16 bytes) for the chunks inside the row, U of a lane at once (loads without a condition, so that all are in flight together:
-// behind the row's end its last chunk again)
-template <typename T, int TH, int U, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, F f) {
-    const int tid = Team<TH>::rank(), n = row.full();
-    for (int i0 = 0; i0 < n; i0 += U * TH) {
+// What one of gridDim.y workgroups of a row writes of its gradient: a run of chunks, and the row's ends with the first and the last run.
+template <typename T> struct Share {
+    int lo, hi;   // chunks of the row, counted from the first whole one
+    bool head, tail;
+    int per, n, to_first;
+    __device__ __forceinline__ Share(const Row<T>& row) {
+        n = row.full();
+        per = (n + (int)gridDim.y - 1) / (int)gridDim.y;
+        lo = min((int)blockIdx.y * per, n);
+        hi = min(lo + per, n);
+        head = blockIdx.y == 0;
+        tail = blockIdx.y == gridDim.y - 1;
+        to_first = row.first * Row<T>::E - row.sh;
+    }
+    __device__ __forceinline__ bool has(int i) const {   // logit i of the row
+        const int e = i - to_first;
+        return e < 0 ? head : e >= n * Row<T>::E ? tail : e >= lo * Row<T>::E && e < hi * Row<T>::E;
+    }
+};
+// f(chunk, its 16 bytes) for a run of the row's chunks, U of a lane at once (loads without a condition, so that all are in flight together:
+// behind the run's end its last chunk again)
+template <typename T, int TH, int U, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, int lo, int hi, F f) {
+    const int tid = Team<TH>::rank();
+    for (int i0 = lo; i0 < hi; i0 += U * TH) {
         chunk_t v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = row.load(row.first + min(i0 + u * TH + tid, n - 1));
+        for (int u = 0; u < U; ++u) v[u] = row.load(row.first + min(i0 + u * TH + tid, hi - 1));
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + u * TH + tid < n) f(row.first + i0 + u * TH + tid, v[u]);
+            if (i0 + u * TH + tid < hi) f(row.first + i0 + u * TH + tid, v[u]);
     }
 }
 template <typename T, int TH> __device__ __forceinline__ void zero_row(const Row<T>& row, T* d) {
@@ -877,9 +896,10 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
         const float y = fmaxf(ref.y(x, c), -200.f);   // (a masked logit: e = 0, whatever c1 is)
         return __builtin_amdgcn_exp2f(y) * fmaf(c1, y, c0);
     };
+    const Share<T> share(row);
     const int ei = row.end_index(tid);
-    if (ei >= 0) Store<T>::store(d + ei, one(Store<T>::load(row.z + ei)));
-    each_chunk<T, TH, U>(row, [&](int ch, const chunk_t& v) {
+    if (ei >= 0 && share.has(ei)) Store<T>::store(d + ei, one(Store<T>::load(row.z + ei)));
+    each_chunk<T, TH, U>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) {
         float x[E];
         Chunk<T>::unpack(v, x);
 #pragma unroll
@@ -892,7 +912,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
     for (int j = tid; j <= q.k; j += TH) {
         const bool is_token = j == q.k;
         const int64_t i = is_token ? t : q.top_ids[r * q.k + j];
-        if (i < 0 || i >= V) continue;
+        if (i < 0 || i >= V || !share.has((int)i)) continue;
         float g = is_token ? gt : q.g_top[r * q.k + j];
         if (!is_token && i == t) g += gt;
         bool again = false;
@@ -993,10 +1013,10 @@ template <int W> struct List {
 struct GradOf { float m_off, a, m, on; };
 
 // The gradients of the listed tokens (W lanes, slots lane + W i; gx: their logits' bits; bit i of `first`: this lane's i-th slot is known to be
-// the first that names its token).  Where a token may be listed more than once its masses are added up.
-template <typename T, int W>
+// the first that names its token; mine(i): logit i is this workgroup's).  Where a token may be listed more than once its masses are added up.
+template <typename T, int W, typename F>
 __device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32_t* gx, int K, uint32_t first, const GradOf& s, float g, float c,
-                                                 const ListLds& l, T* d) {
+                                                 const ListLds& l, T* d, F mine) {
     const int lane = List<W>::lane();
     const auto store = [&](int i, int at, float q) { Store<T>::store(d + at, g * (exp2_from(Row<T>::value(gx[i]), s.m, c) * s.on - q)); };
     uint32_t is = 0;
@@ -1012,12 +1032,12 @@ __device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32
                 q += l.id[o] == at ? l.q[o] : 0.f;
                 one &= l.id[o] != at || o >= j;
             }
-            if (one) store(i, at, q);
+            if (one && mine(at)) store(i, at, q);
         });
         return;
     }
     List<W>::each(K, [&](int i) {
-        if ((is >> i) & 1u) store(i, l.id[lane + i * W], l.q[lane + i * W]);
+        if ((is >> i) & 1u && mine(l.id[lane + i * W])) store(i, l.id[lane + i * W], l.q[lane + i * W]);
     });
 }
 template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const chunk_t& v, float c, const Ref& ref, float ga, T* d) {
@@ -1312,7 +1332,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
             else
                 for (int i0 = lastr; i0 >= 0; i0 -= ROUND) round(i0, i0 > 0);
             Team<TH>::sync();
-            if (lead && !empty) listed_gradients<T, 64>(row, gx, p.K, first, s, g, c, l, d);
+            if (lead && !empty) listed_gradients<T, 64>(row, gx, p.K, first, s, g, c, l, d, [](int) { return true; });
         } else {
             Team<TH>::sync();   // (the first wave's words are read)
         }
@@ -1340,8 +1360,9 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     const float w = p.weights ? p.weights[r] : p.weight0;
     const float4 st = *reinterpret_cast<const float4*>(stats + r * 4);
     const GradOf s = {st.x, st.y, st.z, st.w};
+    const Share<T> share(row);
     if (w == 0.f || s.m == -INFINITY) {   // the row takes no part, or none of its logits is above -inf
-        zero_row<T, TH>(row, d);
+        if (share.head) zero_row<T, TH>(row, d);
         return;
     }
     List<W> mine;
@@ -1350,15 +1371,15 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     const float g = tau * (g_loss || g_row ? (g_loss ? w * g_loss[0] : 0.f) + (g_row ? g_row[r] : 0.f) : w);
     const float ga = g * s.a;
     const int ei = row.end_index(tid);
-    if (ei >= 0) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
-    each_chunk<T, TH, U>(row, [&](int ch, const chunk_t& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
+    if (ei >= 0 && share.has(ei)) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
+    each_chunk<T, TH, U>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
     uint32_t gx[List<W>::J];
     if (lead) {
         mine.template finish<TAIL>(p, V, list_lds[team]);
         List<W>::each(p.K, [&](int i) { gx[i] = row.bits(min(max(list_lds[team].id[min(tid + i * W, p.K - 1)], 0), V - 1)); });
     }
     Team<TH>::sync();
-    if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, list_lds[team], d);
+    if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, list_lds[team], d, [&](int i) { return share.has(i); });
 }
 
 // sum_n w_n L_n in a fixed order
@@ -1407,23 +1428,17 @@ int check_teacher(const char* who, const void* ids, const void* t_logp, int t_dt
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 float one_over(float temperature) { return (float)(1.0 / (double)temperature); }
 
-// threads that own a row of V logits
-template <typename T> int team_of(int V, int N) {
-    if (V <= Small<T, 16>::max_v()) return 16;
-    if (V <= Small<T, 64>::max_v()) return 64;
-    const int chunks = (V + Chunk<T>::E - 1) / Chunk<T>::E;
-    if (N <= 256) return 1024;
-    return chunks <= 16 * 256 ? 256 : chunks <= 16 * 512 ? 512 : 1024;
-}
-#define AG_TEAM_SWITCH(th, CALL)                   \
-    switch (th) {                                  \
-        case 16: { CALL(16); break; }              \
-        case 64: { CALL(64); break; }              \
-        case 256: { CALL(256); break; }            \
-        case 512: { CALL(512); break; }            \
-        default: { CALL(1024); break; }            \
-    }
-template <int TH> dim3 team_grid(int N) { return dim3(TH < 256 ? ceil_div(N, 256 / TH) : N); }
+// The gradients' launches: 16 or 64 lanes a row up to 64 / 2048 logits; of longer rows few (up to 128) are shared by several workgroups of 256
+// threads (at least 1024 chunks each: 262144 fp32 logits of one row 22.1 -> 5.0 us), many get one workgroup each, of the size that reads its
+// row in a few rounds (2048 rows of 65537 bf16: 1024 threads 88 us, 256 threads 101 us).
+#define LG_GRADIENT(V, N, CALL)                                                                                                    \
+    const int row_chunks = (V) / Chunk<T>::E;                                                                                      \
+    if ((V) <= 64) { CALL(16, 1); }                                                                                                \
+    else if ((V) <= 2048) { CALL(64, 1); }                                                                                         \
+    else if ((N) <= 128) { CALL(256, std::max(1, std::min(512 / (N), row_chunks / 1024))); }                                       \
+    else if (row_chunks <= 16 * 256) { CALL(256, 1); }                                                                             \
+    else { CALL(1024, 1); }
+template <int TH> dim3 team_grid(int N, int y = 1) { return dim3(TH < 256 ? ceil_div(N, 256 / TH) : N, y); }
 
 // How many workgroups share a row: for few rows, of 32768 chunks and more, as many as the join takes (64 sums, 256 keys) and leave each 1024
 // chunks (256 threads, four rounds).  One row, 4 alternatives, kernels alone: 524288 fp32 logits 50.5 -> 13.6 us, 262144 fp32 31.2 -> 13.4,
@@ -1466,9 +1481,9 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
 
 template <typename T>
 int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const LogprobsGrad& q, void* d_dlogits, int64_t ldd, hipStream_t s) {
-#define LG_CALL(TH) hipLaunchKernelGGL((logprobs_bwd_kernel<T, TH>), team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, \
+#define LG_CALL(TH, Y) hipLaunchKernelGGL((logprobs_bwd_kernel<T, TH>), team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, \
                                        log2e_over(temperature), one_over(temperature), q, (T*)d_dlogits, ldd)
-    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+    LG_GRADIENT(V, N, LG_CALL)
 #undef LG_CALL
     AG_LAUNCH_CHECK();
     return AG_OK;
@@ -1511,11 +1526,11 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
 template <typename T>
 int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, int tail, const float* d_stats, const float* d_g_loss,
                 const float* d_g_row, void* d_dlogits, int64_t ldd, hipStream_t s) {
-#define LG_CALL(TH)                                                                                                                                   \
+#define LG_CALL(TH, Y)                                                                                                                                \
     const auto kernel = tail ? distill_bwd_kernel<T, TH, true> : distill_bwd_kernel<T, TH, false>;                                                    \
-    hipLaunchKernelGGL(kernel, team_grid<TH>(N), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, temperature, log2e_over(temperature), p, \
-                       d_stats, d_g_loss, d_g_row, (T*)d_dlogits, ldd)
-    AG_TEAM_SWITCH(team_of<T>(V, N), LG_CALL)
+    hipLaunchKernelGGL(kernel, team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, temperature, log2e_over(temperature), p, d_stats, \
+                       d_g_loss, d_g_row, (T*)d_dlogits, ldd)
+    LG_GRADIENT(V, N, LG_CALL)
 #undef LG_CALL
     AG_LAUNCH_CHECK();
     return AG_OK;
@@ -1573,14 +1588,17 @@ extern "C" int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, i
     AG_REQUIRE(!d_dlogits || ldd >= V, "ag_topk_distill: gradient row stride %lld < %d logits", (long long)ldd, V);
     hipStream_t s = (hipStream_t)stream;
     const Distill p = {d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, (float)(1.0 / N)};
-    const auto bf = tail ? (d_dlogits ? distill<bf16_t, true, true> : distill<bf16_t, true, false>)
-                         : (d_dlogits ? distill<bf16_t, false, true> : distill<bf16_t, false, false>);
-    const auto f = tail ? (d_dlogits ? distill<float, true, true> : distill<float, true, false>)
-                        : (d_dlogits ? distill<float, false, true> : distill<float, false, false>);
+    // few rows too long for a workgroup's registers: the loss, then the gradient by several workgroups a row (one row of 262144 fp32: 45 -> 32 us)
+    const bool apart = d_dlogits && d_stats && N <= 32 && V / (dtype == AG_BF16 ? 8 : 4) > 16 * 1024, grad = d_dlogits && !apart;
+    const auto bf = tail ? (grad ? distill<bf16_t, true, true> : distill<bf16_t, true, false>)
+                         : (grad ? distill<bf16_t, false, true> : distill<bf16_t, false, false>);
+    const auto f = tail ? (grad ? distill<float, true, true> : distill<float, true, false>)
+                        : (grad ? distill<float, false, true> : distill<float, false, false>);
     if (int rc = (dtype == AG_BF16 ? bf : f)(d_logits, ld, N, V, temperature, p, d_row_loss, d_stats, d_dlogits, ldd, s)) return rc;
     hipLaunchKernelGGL(weighted_sum_kernel, dim3(1), dim3(1024), 0, s, d_row_loss, d_weights, p.weight0, N, d_loss);
     AG_LAUNCH_CHECK();
-    return AG_OK;
+    if (!apart) return AG_OK;
+    return (dtype == AG_BF16 ? distill_bwd<bf16_t> : distill_bwd<float>)(d_logits, ld, N, V, temperature, p, tail, d_stats, nullptr, nullptr, d_dlogits, ldd, s);
 }
 
 extern "C" int ag_topk_distill_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,

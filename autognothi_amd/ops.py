@@ -884,12 +884,12 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
     L.require_gpu(logits)
     row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.float32, device=dev)
-    stats = None if want_grad else torch.empty((n, 4), dtype=torch.float32, device=dev)
+    stats = None if want_grad and (n > 32 or v <= 65536) else torch.empty((n, 4), dtype=torch.float32, device=dev)   # (few long rows are done in two steps)
     out = torch.empty((n, v), dtype=logits.dtype, device=dev) if want_grad else None
     with L.on(dev):
         L.check(L.lib().ag_topk_distill(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w), 1 if tail else 0,
                                         L.ptr(row), L.ptr(loss), L.ptr(stats), L.ptr(out), v, L.stream()))
-    return TopkDistill(loss, row, out, stats)
+    return TopkDistill(loss, row, out, None if want_grad else stats)
 
 
 def topk_distill_bwd(logits: Tensor, fwd: TopkDistill, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor] = None,

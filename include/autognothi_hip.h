@@ -533,8 +533,8 @@ int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dt
  * list:  L_n = temperature^2 [ sum_j q_j (ln q_j - ln p_id_j) + rest (ln rest - ln p_off) ]   (rest = 0 if the list names every token).
  * d_loss [1] = sum_n w_n L_n with w = d_weights [N] (NULL: 1 / N); a row of weight 0 takes no part: its logits are not read, L_n and its
  * gradient are 0.  d_dlogits (optional): d loss / d logits in `dtype`.  d_stats [N, 4]: what
- * ag_topk_distill_bwd reads, written where d_dlogits is NULL.  A student row of
- * -inf: L = +inf where the teacher has mass, gradient 0. */
+ * ag_topk_distill_bwd reads, written where d_dlogits is NULL; with d_dlogits it may be NULL, and where it is not a few long rows are
+ * done in two steps that use it.  A student row of -inf: L = +inf where the teacher has mass, gradient 0. */
 int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
                     const void* d_teacher_logp, int teacher_dtype, int K, const float* d_weights, int tail, float* d_row_loss, float* d_loss,
                     float* d_stats, void* d_dlogits, int64_t ldd, void* stream);

@@ -138,10 +138,6 @@ struct Team {
     static __device__ __forceinline__ float max(float v, float* red) { return join(v, Max(), red); }
 };
 
-struct MaxBits {   // of the values' bits, as unsigned integers
-    __device__ __forceinline__ float operator()(float a, float b) const { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
-};
-
 struct Acc { float m, s, t; };   // reference (a logit), sum of exp2(y), sum of exp2(y) y,  y = (z - m) c,  c = log2(e) / temperature
 
 // the same sums with respect to the reference `to` >= m (or equal); an empty one stays empty, a NaN a NaN
@@ -296,7 +292,7 @@ template <int G, int SHIFT> __device__ __forceinline__ uint32_t wave_bound(const
     uint32_t lo = j <= 64 ? order_key(-lanes_join<64>(-mine, Max())) >> SHIFT : 0u, hi = (order_key(most) >> SHIFT) + 1u;
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    const int enough = j + (j >> 3) + (j > 4);
+    const int enough = j + min(j >> 3, 4) + (j > 4);
     while (hi - lo > 1u) {
         const uint32_t mid = lo + ((hi - lo) >> 1);
         int n = 0;
@@ -873,7 +869,7 @@ struct LogprobsGrad {
 template <typename T, int TH>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t, LogprobsGrad q,
                                                                            T* __restrict__ dz, int64_t ldd) {
-    constexpr int E = Chunk<T>::E, U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1;
+    constexpr int E = Chunk<T>::E, U = TH < 64 ? 2 : 4, PER = TH < 256 ? 256 / TH : 1;
     __shared__ float red[TH < 64 ? 1 : TH / 64];
     const int64_t r = (int64_t)blockIdx.x * PER + Team<TH>::index();
     if (PER > 1 && r >= N) return;
@@ -1349,7 +1345,7 @@ template <typename T, int TH, bool TAIL>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                                                                           const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
-    constexpr int U = TH < 64 ? 1 : 4, PER = TH < 256 ? 256 / TH : 1, W = TH < 64 ? TH : 64;
+    constexpr int U = TH < 64 ? 2 : 4, PER = TH < 256 ? 256 / TH : 1, W = TH < 64 ? TH : 64;
     __shared__ ListLds list_lds[PER];
     const int team = Team<TH>::index(), tid = Team<TH>::rank();
     const bool lead = TH <= 64 || __builtin_amdgcn_readfirstlane(tid) < 64;
@@ -1417,6 +1413,10 @@ int check_rows(const char* who, const void* d_logits, int64_t ld, int N, int V, 
     AG_REQUIRE(dtype == AG_F32 || dtype == AG_BF16, "%s: dtype %d (AG_F32 or AG_BF16)", who, dtype);
     AG_REQUIRE(ld >= 0, "%s: row stride %lld", who, (long long)ld);
     AG_REQUIRE(temperature >= 0x1p-20f && temperature <= 0x1p20f, "%s: temperature %g (2^-20 to 2^20)", who, (double)temperature);
+    // (a launch holds less than 2^32 threads; at most this many belong to a row)
+    const int chunks = V / (dtype == AG_BF16 ? 8 : 4), threads = V <= 64 ? 16 : chunks <= 320 ? 64 : chunks <= 2048 ? 256 : 1024;
+    AG_REQUIRE((int64_t)N * threads < (int64_t)1 << 32, "%s: %d rows of %d logits in one call (fewer than %lld)", who, N, V,
+               ((long long)1 << 32) / threads);
     return AG_OK;
 }
 int check_teacher(const char* who, const void* ids, const void* t_logp, int t_dtype, int K, int N) {
@@ -1428,29 +1428,45 @@ int check_teacher(const char* who, const void* ids, const void* t_logp, int t_dt
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 float one_over(float temperature) { return (float)(1.0 / (double)temperature); }
 
-// The gradients' launches: 16 or 64 lanes a row up to 64 / 2048 logits; of longer rows few (up to 128) are shared by several workgroups of 256
-// threads (at least 1024 chunks each: 262144 fp32 logits of one row 22.1 -> 5.0 us), many get one workgroup each, of the size that reads its
-// row in a few rounds (2048 rows of 65537 bf16: 1024 threads 88 us, 256 threads 101 us).
+// The gradients' launches, by the row's 16-byte pieces and by the rows a CU gets (log-probabilities' gradient, fp32, both sides of each bound):
+//   up to 32: 16 lanes a row          131072 rows of 128: 23.6 us, 64 lanes 53.6; of 300: 68.0 / 76.8 (with a list of 50: 168.8 / 146.1)
+//   up to 320: 64 lanes               65536 rows of 1200: 124 us, 256 threads 137; of 1600: 159 / 151
+//   up to one row a CU, longer: several workgroups of 256 threads a row, at least 1024 pieces each
+//                                     one row of 262144: 5.0 us, one workgroup 22.1; 256 rows of 131072: 41 / 44
+//   up to 2048: 256 threads           16384 rows of 6000: 151 us, 1024 threads 160; of 8192: 199 / 192; 8192 of 16384: 207 / 188
+//   longer: 1024 threads
 #define LG_GRADIENT(V, N, CALL)                                                                                                    \
     const int row_chunks = (V) / Chunk<T>::E;                                                                                      \
-    if ((V) <= 64) { CALL(16, 1); }                                                                                                \
-    else if ((V) <= 2048) { CALL(64, 1); }                                                                                         \
-    else if ((N) <= 128) { CALL(256, std::max(1, std::min(512 / (N), row_chunks / 1024))); }                                       \
-    else if (row_chunks <= 16 * 256) { CALL(256, 1); }                                                                             \
+    if (row_chunks <= 32) { CALL(16, 1); }                                                                                         \
+    else if (row_chunks <= 320) { CALL(64, 1); }                                                                                   \
+    else if ((N) <= cu_count()) { CALL(256, std::max(1, std::min(8 * cu_count() / (N), row_chunks / 1024))); }                     \
+    else if (row_chunks <= 2048) { CALL(256, 1); }                                                                                 \
     else { CALL(1024, 1); }
+int cu_count() { return ag_device_cus() > 0 ? ag_device_cus() : 256; }
 template <int TH> dim3 team_grid(int N, int y = 1) { return dim3(TH < 256 ? ceil_div(N, 256 / TH) : N, y); }
 
-// How many workgroups share a row: for few rows, of 32768 chunks and more, as many as the join takes (64 sums, 256 keys) and leave each 1024
-// chunks (256 threads, four rounds).  One row, 4 alternatives, kernels alone: 524288 fp32 logits 50.5 -> 13.6 us, 262144 fp32 31.2 -> 13.4,
-// 262144 bf16 23.9 -> 11.3, 131072 bf16 16.2 -> 10.4; the second launch and the workspace cost the host 5 us, so shorter rows stay whole.
+// How many workgroups share a row: up to 128 rows of 32768 chunks and more, as many as the join takes (64 sums, 256 keys), as give each CU two
+// and leave each 1024 chunks (256 threads, four rounds).  Kernels alone, N x V fp32, k alternatives, shared / one workgroup a row: 1 x 131072,
+// k 0: 8.5 / 13.0 us, k 16: 13.8 / 20.2; 1 x 524288, k 4: 13.6 / 50.5; 128 x 131072, k 16: 20.9 / 23.6.  Not for more than 32 alternatives,
+// which leave the join few parts (1 x 131072, k 64: 20.9 / 22.0, k 128: 29.7 / 22.5) nor for shorter rows (1 x 65536, k 16: 14.3 / 14.3): the
+// second launch and the workspace cost the host 5 us.
+// (The last part has what the rounding up to 64 logits leaves it: at least 4096 - 63 * 64 logits, and at least k.)
 Parts parts_of(int N, int V, int dtype, int k) {
     const int chunks = V / (dtype == AG_BF16 ? 8 : 4);
-    int count = std::min(std::min(64, chunks / 1024), std::min(k ? 256 / k : 64, 512 / std::max(N, 1)));
-    if (N < 1 || N > 64 || chunks < 32768 || count < 2) return {0, 0, nullptr, nullptr};
+    if (N < 1 || N > 128 || chunks < 32768 || k > 32) return {0, 0, nullptr, nullptr};
+    const int count = std::min(std::min(64, chunks / 1024), std::min(k ? 256 / k : 64, 512 / N));
     const int length = (ceil_div(V, count) + 63) / 64 * 64;
     return {ceil_div(V, length), length, nullptr, nullptr};
 }
 
+// Threads of a row, by its chunks and the rows a CU gets (N rows of V logits, k alternatives, both sides of each bound):
+//   V <= 64: 16 lanes                        262144 x 64 fp32, k 3: 123 us, 64 lanes 282
+//   up to 2048 chunks: 64 lanes              16384 x 6000 fp32, k 20: 78 us, 256 threads 90; x 8192: 109 / 104 (bf16 x 16384: 111 / 118)
+//       four rows a CU or fewer: up to 512   512 x 4096 bf16, k 50: 11.0 / 9.7 us; 64 x 16384: 17.1 / 10.5; 1024 x 2080: 10.1 / 11.4
+//   up to 8192: 256 threads                  8192 x 32768 bf16, k 20: 103 us, 512 threads 132; 2048 x 65536 fp32, k 100: 112 / 107
+//       one row a CU or fewer: up to 4096    1 x 32000 fp32, k 16: 12.2 / 9.8 us; 256 x 16000: 10.3 / 10.5
+//   longer: 512 threads
+//       one row a CU or fewer, longer than 16384: 1024 threads      64 x 240000 fp32, k 128: 35.7 us, 512 threads 42.0; x 65536: 20.3 / 20.1
 template <typename T, bool TOP>
 int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_tokens, int k, float* d_logp, float* d_entropy, float* d_lse,
              float* d_stats, int64_t* d_top_ids, float* d_top_logp, Parts parts, hipStream_t s) {
@@ -1460,7 +1476,7 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
                                        d_entropy, d_lse, d_stats, d_top_ids, d_top_logp)
 #define LG_WG(TH, PART) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP, PART>), dim3(N * (PART ? parts.count : 1)), dim3(TH), 0, s, z, ld, V, c, inv_t, \
                                            d_tokens, k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, parts)
-    const int chunks = V / Chunk<T>::E;
+    const int chunks = V / Chunk<T>::E, cus = cu_count();
     if (parts.count) {
         LG_WG(256, true);
         AG_LAUNCH_CHECK();
@@ -1468,11 +1484,10 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
                            d_top_ids, d_top_logp, parts);
     } else if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
     else if (V <= Small<T, 64>::max_v() && (chunks < 16 || min(chunks, 64 * min(max(chunks / 64, 1), 4)) < k + k / 2)) LG_SMALL(64);
-    else if (N <= 256 && chunks >= 2048) LG_WG(1024, false);
-    else if (chunks <= 2048) LG_WG(64, false);
-    else if (chunks <= 8192) LG_WG(256, false);
-    else if (chunks <= 32768) LG_WG(512, false);
-    else LG_WG(1024, false);
+    else if (chunks <= (N <= 4 * cus ? 512 : 2048)) LG_WG(64, false);
+    else if (chunks <= (N <= cus ? 4096 : 8192)) LG_WG(256, false);
+    else if (N <= cus && chunks > 16384) LG_WG(1024, false);
+    else LG_WG(512, false);
 #undef LG_SMALL
 #undef LG_WG
     AG_LAUNCH_CHECK();
@@ -1489,13 +1504,20 @@ int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperatu
     return AG_OK;
 }
 
+// Threads of a row and chunks of a thread: the fewest threads whose registers hold the row.  With the gradient, 16384 rows fp32, list of 50,
+// the choice against its neighbour: V 1000: (64, 4) 43.6 us, (64, 8) 50.0; 2040: (64, 8) 80.8, (256, 8) 118.6; 2400: (64, 16) 90, (256, 8) 118;
+// 4000: 141 / 143; 8160: (256, 8) 248, (256, 16) 254; 11184 x 12000: (256, 16) 248, (512, 16) 258; 5592 x 24000: (512, 16) 233, (1024, 16) 274;
+// 2048 x 65520: one round of (1024, 16) 245, rounds of (256, 8) 293.  Four rows a CU or fewer are a matter of latency: 512 x 2040: (64, 8) 11.7,
+// (256, 8) 10.6; 64 x 16360: (256, 16) 13.8, (512, 16) 12.0.
+// The loss alone reads each chunk once, whatever the rounds: 8388 x 4000: (64, 4) 32.3, (256, 4) 43.6; 2796 x 12000: 27.5 / 29.7; 2048 x 16384:
+// 29.1 / 27.9; 512 x 4000: 10.7 / 9.1; one row a CU or fewer, 64 x 64000: (256, 4) 20.1, (1024, 8) 13.0.
 template <typename T, bool TAIL, bool GRAD>
 int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, float* d_row_loss, float* d_stats, void* d_dlogits,
             int64_t ldd, hipStream_t s) {
     const T* z = (const T*)d_logits;
     T* dz = (T*)d_dlogits;
     const float c = log2e_over(temperature), inv_t = one_over(temperature);
-    const int chunks = V / Chunk<T>::E, cus = ag_device_cus() > 0 ? ag_device_cus() : 256;
+    const int chunks = V / Chunk<T>::E, cus = cu_count();
     if (V <= Small<T, 16>::max_v()) {
         hipLaunchKernelGGL((distill_small_kernel<T, TAIL, GRAD>), dim3(ceil_div(N, 16)), dim3(256), 0, s, z, ld, N, V, temperature, c, inv_t, p, d_row_loss,
                            d_stats, dz, ldd);
@@ -1507,15 +1529,16 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
                        (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1), s, z, ld, N, V, temperature, c, inv_t, p, d_row_loss, d_stats, dz, ldd)
     if constexpr (GRAD) {
         if (chunks <= 4 * 64) LG_CALL(64, 4, false, 6);
-        else if (chunks <= 8 * 64) LG_CALL(64, 8, false, 5);
+        else if (N > 4 * cus && chunks <= 8 * 64) LG_CALL(64, 8, false, 5);
+        else if (N > 4 * cus && chunks <= 16 * 64) LG_CALL(64, 16, false, 4);
         else if (chunks <= 8 * 256) LG_CALL(256, 8, false, 5);
-        else if (chunks <= 16 * 256) LG_CALL(256, 16, false, 4);
+        else if (N > 2 * cus && chunks <= 16 * 256) LG_CALL(256, 16, false, 4);
         else if (chunks <= 16 * 512) LG_CALL(512, 16, false, 2);
         else if (chunks <= 16 * 1024) LG_CALL(1024, 16, false, 1);
         else LG_CALL(1024, 16, true, 1);
     } else {
-        if (chunks <= 8 * 64) LG_CALL(64, 4, true, 6);
-        else if (N <= 256 && chunks >= 4096) LG_CALL(1024, 8, true, 1);
+        if (chunks <= (N <= 4 * cus ? 512 : 2048)) LG_CALL(64, 4, true, 6);
+        else if (N <= cus && chunks >= 4096) LG_CALL(1024, 8, true, 1);
         else LG_CALL(256, 4, true, 6);
     }
 #undef LG_CALL

@@ -780,6 +780,8 @@ def _logit_rows(who: str, logits: Tensor) -> Tuple[Tensor, int, int, int, int]:
     n, v = logits.shape
     if not 1 <= v <= L.AG_LOGITS_MAX_V:
         raise ValueError(f"{who}: rows of {v} logits (1 to {L.AG_LOGITS_MAX_V})")
+    if n >= 1 << 28:      # (what the library takes depends on v, and is told by it)
+        raise ValueError(f"{who}: {n} rows in one call")
     if logits.stride(1) != 1 and v > 1:
         logits = logits.contiguous()
     return logits, n, v, logits.stride(0), dtype
@@ -822,7 +824,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
     ids = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
     top = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
     with L.on(dev):
-        need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 64 else 0
+        need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 128 else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
                                           L.ptr(ids), L.ptr(top), L.ptr(ws), need, L.stream()))

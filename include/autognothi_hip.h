@@ -507,6 +507,7 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
  * d_logits [N, V] in `dtype`, row stride ld elements (any alignment; 0 = one row for all), 1 <= V <= AG_LOGITS_MAX_V; x = z / temperature
  * (2^-20 to 2^20), p = softmax(x), every sum in fp32.  A logit of -inf has probability 0; a row of nothing but -inf has no distribution (below); a NaN or
  * +inf makes its row's results NaN.  Nothing is read back to the host; all calls can be captured.  Outputs must not alias inputs.
+ * N < 2^28 up to 64 logits a row, 2^26 up to 320 16-byte pieces of a row, 2^24 up to 2048, else 2^22.
  * ---------------------------------------------------------------------------------------------- */
 #define AG_LOGITS_MAX_V 524288
 #define AG_LOGITS_MAX_TOP 128

@@ -570,3 +570,57 @@ def test_refused_across_devices(cuda_device):
         ops.token_logprobs(z, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="the logits are on"):
         ops.topk_distill(z, torch.zeros(2, 2, dtype=torch.int64, device=cuda_device), torch.zeros(2, 2))
+
+
+# Calls of many rows take other threads per row than calls of few: some rows of each against the oracle, the others by the sums they enter.
+MANY = [(4500, 40), (1100, 300), (1100, 700), (1100, 1500), (1100, 2040), (1100, 3000), (1100, 9000), (600, 3000), (300, 1000), (300, 3000), (300, 9000), (300, 20000),
+        (200, 20000), (100, 40000), (128, 33000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,chunks", MANY)
+def test_many_rows(cuda_device, dtype, n, chunks):
+    from autognothi_amd import ops
+    v = chunks * (4 if dtype == F32 else 8) + 3
+    gen = torch.Generator(cuda_device).manual_seed(n + chunks)
+    z = (torch.randn(n, v + 5, device=cuda_device, generator=gen) * 3.0).to(dtype)[:, :v]
+    g = np.random.default_rng(n * chunks)
+    pick = np.unique(np.concatenate([[0, n - 1], g.integers(0, n, 6)]))
+    at = torch.from_numpy(pick).to(cuda_device)
+    z64 = z[at].double().cpu().numpy()
+    tokens = g.integers(0, v, n)
+    tok = torch.from_numpy(tokens).to(cuda_device)
+    tau = [1.0, 2.0, 0.7][chunks % 3]
+    for k in (0, 7, 32, 128):
+        r = ops.token_logprobs(z, tok, k, tau)
+        want = ol.token_logprobs(z64, tokens[pick], k, tau)
+        for name in ("logp", "entropy", "lse", "top_logp"):
+            if name in want:
+                _near(getattr(r, name)[at], want[name], want["err_" + name], name)
+        assert torch.isfinite(r.lse).all() and torch.isfinite(r.entropy).all()
+        if k:
+            np.testing.assert_array_equal(r.top_ids[at].cpu().numpy(), want["top_ids"])
+            assert (r.top_logp[:, 1:] <= r.top_logp[:, :-1]).all() and torch.equal(z.gather(1, r.top_ids).float().amax(1), z.float().amax(1))
+    gl, ge = g.standard_normal(n).astype(np.float32), g.standard_normal(n).astype(np.float32)
+    dz = ops.token_logprobs_bwd(z, r, tok, torch.from_numpy(gl).to(cuda_device), torch.from_numpy(ge).to(cuda_device))
+    want, bound = ol.token_logprobs_grad(z64, tokens[pick], None, tau, gl[pick], ge[pick], None, None)
+    _near(dz[at], want, bound, "dlogits", rounded=dtype == BF16)
+    assert torch.isfinite(dz).all()
+    k = [5, 50, 128][chunks % 3]
+    ids, lp, lp64 = _teacher(g, n, v, k, 0.8, True, F32)
+    w = g.random(n).astype(np.float32) / n
+    w[g.integers(0, n, n // 5)] = 0.0
+    args = (torch.from_numpy(ids).to(cuda_device), lp.to(cuda_device), torch.from_numpy(w).to(cuda_device), tau)
+    for tail in (False, True):
+        row, grad, e_row, e_grad = ol.distill(z64, ids[pick], lp64[pick], tau, tail, w[pick].astype(np.float64))
+        r = ops.topk_distill(z, *args, tail)
+        only = ops.topk_distill(z, *args, tail, want_grad=False)
+        apart = ops.topk_distill_bwd(z, only, *args, tail)
+        for a in (r, only):
+            _near(a.row_loss[at], row, e_row, "row_loss")
+            assert torch.isfinite(a.row_loss).all() and (a.row_loss[args[2] == 0] == 0).all()
+            total = (a.row_loss.double() * args[2].double()).sum()
+            assert abs(a.loss.double() - total) <= 2 ** -23 * total.abs()
+        for d in (r.dlogits, apart):
+            _near(d[at], grad, e_grad * (1 + 4 * ol.U), "dlogits", rounded=dtype == BF16)
+            assert torch.isfinite(d).all() and not d[args[2] == 0].any()

@@ -144,3 +144,25 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
                di(tau=-1.0), db(n=0), db(k=0), db(st=None), db(ldd=7), db(dz=None)):
         assert rc < 0 and lib.ag_last_error()
     assert tl(n=0) == 0    # no rows: nothing to do
+
+
+@pytest.mark.parametrize("fn", ALL)
+def test_more_rows_than_a_launch_holds_are_refused(fn):
+    z = torch.zeros(1, 11)
+    with pytest.raises(ValueError, match="rows in one call"):
+        _call(fn, logits=z.expand(1 << 28, 11))
+    with pytest.raises(ValueError, match="rows in one call"):
+        _call(fn, logits=z.expand((1 << 32) + 3, 11))
+
+
+@pytest.mark.parametrize("dtype,v,n", [(0, 64, 1 << 28), (0, 65, 1 << 26), (1, 2567, 1 << 26), (0, 1284, 1 << 24), (0, 8195, 1 << 24), (0, 8196, 1 << 22),
+                                       (1, 16391, 1 << 24), (1, 524288, 1 << 22)])
+def test_c_entries_refuse_more_rows_than_a_launch_holds(dtype, v, n):
+    from autognothi_amd import _lib as L
+    lib = L.lib()
+    x = 0x1000    # never read: every call below is refused on the host
+    for rc in (lib.ag_token_logprobs(x, 0, n, v, dtype, 1.0, None, 0, None, x, x, x, None, None, None, 0, None),
+               lib.ag_token_logprobs_bwd(x, 0, n, v, dtype, 1.0, x, x, None, None, None, None, 0, None, None, x, v, None),
+               lib.ag_topk_distill(x, 0, n, v, dtype, 1.0, x, x, 0, 1, None, 0, x, x, x, x, v, None),
+               lib.ag_topk_distill_bwd(x, 0, n, v, dtype, 1.0, x, x, 0, 1, None, 0, x, None, None, x, v, None)):
+        assert rc < 0 and b"rows of" in lib.ag_last_error()

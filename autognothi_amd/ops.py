@@ -818,11 +818,11 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
     dev = logits.device
     tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
     L.require_gpu(logits)
-    stats = torch.empty((5, n), dtype=torch.float32, device=dev)      # (one allocation: at one row the host's time is the call's)
+    stats = torch.empty(5, n, dtype=torch.float32, device=dev)      # (one allocation, sizes not as a tuple: at one row the host's time is the call's)
     logp, entropy, lse, _, _ = stats.unbind(0)
     at = stats.data_ptr()
-    ids = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
-    top = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
+    ids = torch.empty(n, top_k, dtype=torch.int64, device=dev) if top_k else None
+    top = torch.empty(n, top_k, dtype=torch.float32, device=dev) if top_k else None
     with L.on(dev):
         need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 128 else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -851,7 +851,7 @@ def token_logprobs_bwd(logits: Tensor, fwd: TokenLogprobs, tokens: Optional[Tens
     d_lse, d_top = _row_arg(who, "d_lse", d_lse, (n,), f32, dev), _row_arg(who, "d_top_logp", d_top_logp, (n, k), f32, dev)
     ids = _row_arg(who, "top_ids", fwd.top_ids, (n, k), torch.int64, dev) if k else None
     L.require_gpu(logits)
-    out = torch.empty((n, v), dtype=logits.dtype, device=dev)
+    out = torch.empty(n, v, dtype=logits.dtype, device=dev)
     with L.on(dev):
         L.check(L.lib().ag_token_logprobs_bwd(L.ptr(logits), ld, n, v, dtype, fwd.temperature, at + 12 * n, at + 4 * n, L.ptr(tokens),
                                               L.ptr(d_logp), L.ptr(d_entropy), L.ptr(d_lse), k, L.ptr(ids), L.ptr(d_top), L.ptr(out), v,
@@ -886,8 +886,8 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
     L.require_gpu(logits)
     row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.float32, device=dev)
-    stats = None if want_grad and (n > 32 or v <= 65536) else torch.empty((n, 4), dtype=torch.float32, device=dev)   # (few long rows are done in two steps)
-    out = torch.empty((n, v), dtype=logits.dtype, device=dev) if want_grad else None
+    stats = None if want_grad and (n > 32 or v <= 65536) else torch.empty(n, 4, dtype=torch.float32, device=dev)   # (few long rows are done in two steps)
+    out = torch.empty(n, v, dtype=logits.dtype, device=dev) if want_grad else None
     with L.on(dev):
         L.check(L.lib().ag_topk_distill(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w), 1 if tail else 0,
                                         L.ptr(row), L.ptr(loss), L.ptr(stats), L.ptr(out), v, L.stream()))
@@ -911,7 +911,7 @@ def topk_distill_bwd(logits: Tensor, fwd: TopkDistill, teacher_ids: Tensor, teac
     d_loss = _row_arg(who, "d_loss", d_loss, (1,), torch.float32, dev)
     d_row = _row_arg(who, "d_row_loss", d_row_loss, (n,), torch.float32, dev)
     L.require_gpu(logits)
-    out = torch.empty((n, v), dtype=logits.dtype, device=dev)
+    out = torch.empty(n, v, dtype=logits.dtype, device=dev)
     with L.on(dev):
         L.check(L.lib().ag_topk_distill_bwd(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w),
                                             1 if tail else 0, L.ptr(stats), L.ptr(d_loss), L.ptr(d_row), L.ptr(out), v, L.stream()))

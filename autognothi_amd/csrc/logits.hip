@@ -72,6 +72,7 @@ struct Row {
     }
     __device__ __forceinline__ int full() const { return end - first; }
     __device__ __forceinline__ chunk_t load(int c) const { return *reinterpret_cast<const chunk_t*>(z + (c * E - sh)); }
+    __device__ __forceinline__ chunk_t load_past(int c) const { return __builtin_nontemporal_load(reinterpret_cast<const chunk_t*>(z + (c * E - sh))); }
     // one logit's bits, to be made a number (`value`) where it is wanted: nothing waits for the load here
     __device__ __forceinline__ uint32_t bits(int i) const { return reinterpret_cast<const typename Chunk<T>::Bits*>(z)[i]; }
     static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(E == 8 ? b << 16 : b); }
@@ -82,9 +83,13 @@ struct Row {
         return l < 2 * E && i < V ? i : -1;
     }
     // the chunk's place in another row of the same length (at the logits' alignment: the hardware takes any)
-    __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const {
+    __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const { store<false>(d, c, x); }
+    template <bool PAST> __device__ __forceinline__ void store(T* d, int c, const float (&x)[E]) const {
         typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t any_chunk_t;
-        *reinterpret_cast<any_chunk_t*>(d + (c * E - sh)) = Chunk<T>::pack(x);
+        any_chunk_t* to = reinterpret_cast<any_chunk_t*>(d + (c * E - sh));
+        const any_chunk_t v = Chunk<T>::pack(x);
+        if (PAST) __builtin_nontemporal_store(v, to);
+        else *to = v;
     }
 };
 
@@ -820,6 +825,17 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // exponent), and a few places (the given token, the listed ones) where something is added: those are written again once the row is done.
 // One read and one write of the row; a lane has U chunks in flight.
 
+// Which of a gradient's accesses go past the chip's memory-side cache of 256 MiB.  Logits and gradient that do not fit it together: the stores,
+// so that what the forward pass left of the logits stays (what reads the gradient next is a matrix product, which can wait for memory); logits
+// that do not fit it alone: the loads too.  Rows of 32001 bf16, forward and backward, a copy into the logits before and a sum of the gradient
+// after them taken off: 128 MB of logits 74 us (stores past it: 77), 160 MB 94 -> 86 (loads too: 85), 192 MB 116 -> 99 (103),
+// 256 MB 148 -> 129 (124), 300 MB 178 -> 161 (148; without the copy and the sum 181 -> 149, 150), 320 MB 191 -> 177 (159), 1 GB 542 -> 530 (518).  The kernel that computes loss and gradient in one gains nothing.
+enum Past { PAST_NONE, PAST_STORES, PAST_ALL };
+inline Past past_cache(int64_t bytes) {
+    constexpr int64_t cache = 256 << 20;
+    return bytes <= cache / 2 ? PAST_NONE : bytes <= cache + cache / 8 ? PAST_STORES : PAST_ALL;
+}
+
 // What one of gridDim.y workgroups of a row writes of its gradient: a run of chunks, and the row's ends with the first and the last run.
 template <typename T> struct Share {
     int lo, hi;   // chunks of the row, counted from the first whole one
@@ -841,12 +857,15 @@ template <typename T> struct Share {
 };
 // f(chunk, its 16 bytes) for a run of the row's chunks, U of a lane at once (loads without a condition, so that all are in flight together:
 // behind the run's end its last chunk again)
-template <typename T, int TH, int U, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, int lo, int hi, F f) {
+template <typename T, int TH, int U, Past PAST, typename F> __device__ __forceinline__ void each_chunk(const Row<T>& row, int lo, int hi, F f) {
     const int tid = Team<TH>::rank();
     for (int i0 = lo; i0 < hi; i0 += U * TH) {
         chunk_t v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = row.load(row.first + min(i0 + u * TH + tid, hi - 1));
+        for (int u = 0; u < U; ++u) {
+            const int ch = row.first + min(i0 + u * TH + tid, hi - 1);
+            v[u] = PAST == PAST_ALL ? row.load_past(ch) : row.load(ch);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i0 + u * TH + tid < hi) f(row.first + i0 + u * TH + tid, v[u]);
@@ -866,7 +885,7 @@ struct LogprobsGrad {
     const int64_t *tokens, *top_ids;
     int k;
 };
-template <typename T, int TH>
+template <typename T, int TH, Past PAST>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t, LogprobsGrad q,
                                                                            T* __restrict__ dz, int64_t ldd) {
     constexpr int E = Chunk<T>::E, U = TH < 64 ? 2 : 4, PER = TH < 256 ? 256 / TH : 1;
@@ -895,12 +914,12 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
     const Share<T> share(row);
     const int ei = row.end_index(tid);
     if (ei >= 0 && share.has(ei)) Store<T>::store(d + ei, one(Store<T>::load(row.z + ei)));
-    each_chunk<T, TH, U>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) {
+    each_chunk<T, TH, U, PAST>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) {
         float x[E];
         Chunk<T>::unpack(v, x);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = one(x[e]);
-        row.store(d, ch, x);
+        row.template store<PAST != PAST_NONE>(d, ch, x);
     });
     if (empty) return;
     Team<TH>::sync();
@@ -1036,7 +1055,7 @@ __device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32
         if ((is >> i) & 1u && mine(l.id[lane + i * W])) store(i, l.id[lane + i * W], l.q[lane + i * W]);
     });
 }
-template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const chunk_t& v, float c, const Ref& ref, float ga, T* d) {
+template <bool PAST, typename T> __device__ __forceinline__ void gradient_chunk(const Row<T>& row, int ch, const chunk_t& v, float c, const Ref& ref, float ga, T* d) {
     constexpr int E = Chunk<T>::E;
     float x[E];
     Chunk<T>::unpack(v, x);
@@ -1048,7 +1067,7 @@ template <typename T> __device__ __forceinline__ void gradient_chunk(const Row<T
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = ga * exp2_from(x[e], ref.m, c);
     }
-    row.store(d, ch, x);
+    row.template store<PAST>(d, ch, x);
 }
 // words of LDS for a bit per logit of a row's chunks, whatever its alignment
 template <typename T> __host__ __device__ constexpr int bit_words(int V) { return (V + Chunk<T>::E - 1 + 31) / 32 + 1; }
@@ -1320,7 +1339,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
                 for (int i = 0; i < NC; ++i) {
                     // (a new value for the compiler: else it keeps the sums' unpacked logits, twice the chunks' registers, for the gradient)
                     asm volatile("" : "+v"(v[i]));
-                    if (i0 + i * TH + t1 < n) gradient_chunk(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
+                    if (i0 + i * TH + t1 < n) gradient_chunk<false>(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
                     v[i] = *reinterpret_cast<const chunk_t*>(from + min(i * TH + t1, to) * E);
                 }
             };
@@ -1341,7 +1360,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
     }
 }
 
-template <typename T, int TH, bool TAIL>
+template <typename T, int TH, bool TAIL, Past PAST>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                                                                           const float* __restrict__ g_row, T* __restrict__ dz, int64_t ldd) {
@@ -1368,7 +1387,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     const float ga = g * s.a;
     const int ei = row.end_index(tid);
     if (ei >= 0 && share.has(ei)) Store<T>::store(d + ei, ga * exp2_from(Store<T>::load(row.z + ei), ref.m, c));
-    each_chunk<T, TH, U>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) { gradient_chunk(row, ch, v, c, ref, ga, d); });
+    each_chunk<T, TH, U, PAST>(row, share.lo, share.hi, [&](int ch, const chunk_t& v) { gradient_chunk<PAST != PAST_NONE>(row, ch, v, c, ref, ga, d); });
     uint32_t gx[List<W>::J];
     if (lead) {
         mine.template finish<TAIL>(p, V, list_lds[team]);
@@ -1496,8 +1515,13 @@ int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, 
 
 template <typename T>
 int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const LogprobsGrad& q, void* d_dlogits, int64_t ldd, hipStream_t s) {
-#define LG_CALL(TH, Y) hipLaunchKernelGGL((logprobs_bwd_kernel<T, TH>), team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, \
-                                       log2e_over(temperature), one_over(temperature), q, (T*)d_dlogits, ldd)
+    const Past past = past_cache((int64_t)N * V * (int64_t)sizeof(T));
+#define LG_CALL(TH, Y)                                                                                                                                \
+    const auto kernel = past == PAST_NONE     ? logprobs_bwd_kernel<T, TH, PAST_NONE>                                                                 \
+                        : past == PAST_STORES ? logprobs_bwd_kernel<T, TH, PAST_STORES>                                                               \
+                                              : logprobs_bwd_kernel<T, TH, PAST_ALL>;                                                                 \
+    hipLaunchKernelGGL(kernel, team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, log2e_over(temperature),           \
+                       one_over(temperature), q, (T*)d_dlogits, ldd)
     LG_GRADIENT(V, N, LG_CALL)
 #undef LG_CALL
     AG_LAUNCH_CHECK();
@@ -1546,17 +1570,24 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
     return AG_OK;
 }
 
-template <typename T>
-int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, int tail, const float* d_stats, const float* d_g_loss,
+template <typename T, bool TAIL>
+int distill_bwd(const void* d_logits, int64_t ld, int N, int V, float temperature, const Distill& p, const float* d_stats, const float* d_g_loss,
                 const float* d_g_row, void* d_dlogits, int64_t ldd, hipStream_t s) {
+    const Past past = past_cache((int64_t)N * V * (int64_t)sizeof(T));
 #define LG_CALL(TH, Y)                                                                                                                                \
-    const auto kernel = tail ? distill_bwd_kernel<T, TH, true> : distill_bwd_kernel<T, TH, false>;                                                    \
-    hipLaunchKernelGGL(kernel, team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, temperature, log2e_over(temperature), p, d_stats, \
-                       d_g_loss, d_g_row, (T*)d_dlogits, ldd)
+    const auto kernel = past == PAST_NONE     ? distill_bwd_kernel<T, TH, TAIL, PAST_NONE>                                                            \
+                        : past == PAST_STORES ? distill_bwd_kernel<T, TH, TAIL, PAST_STORES>                                                          \
+                                              : distill_bwd_kernel<T, TH, TAIL, PAST_ALL>;                                                            \
+    hipLaunchKernelGGL(kernel, team_grid<TH>(N, Y), dim3(TH < 256 ? 256 : TH), 0, s, (const T*)d_logits, ld, N, V, temperature,                       \
+                       log2e_over(temperature), p, d_stats, d_g_loss, d_g_row, (T*)d_dlogits, ldd)
     LG_GRADIENT(V, N, LG_CALL)
 #undef LG_CALL
     AG_LAUNCH_CHECK();
     return AG_OK;
+}
+
+auto gradient_of(int dtype, int tail) {
+    return dtype == AG_BF16 ? (tail ? distill_bwd<bf16_t, true> : distill_bwd<bf16_t, false>) : (tail ? distill_bwd<float, true> : distill_bwd<float, false>);
 }
 
 }  // namespace
@@ -1621,7 +1652,7 @@ extern "C" int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, i
     hipLaunchKernelGGL(weighted_sum_kernel, dim3(1), dim3(1024), 0, s, d_row_loss, d_weights, p.weight0, N, d_loss);
     AG_LAUNCH_CHECK();
     if (!apart) return AG_OK;
-    return (dtype == AG_BF16 ? distill_bwd<bf16_t> : distill_bwd<float>)(d_logits, ld, N, V, temperature, p, tail, d_stats, nullptr, nullptr, d_dlogits, ldd, s);
+    return gradient_of(dtype, tail)(d_logits, ld, N, V, temperature, p, d_stats, nullptr, nullptr, d_dlogits, ldd, s);
 }
 
 extern "C" int ag_topk_distill_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_teacher_ids,
@@ -1632,6 +1663,5 @@ extern "C" int ag_topk_distill_bwd(const void* d_logits, int64_t ld, int N, int 
     AG_REQUIRE(N >= 1 && d_stats && d_dlogits, "ag_topk_distill_bwd: no rows or a null pointer");
     AG_REQUIRE(ldd >= V, "ag_topk_distill_bwd: gradient row stride %lld < %d logits", (long long)ldd, V);
     const Distill p = {d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, (float)(1.0 / N)};
-    return (dtype == AG_BF16 ? distill_bwd<bf16_t> : distill_bwd<float>)(d_logits, ld, N, V, temperature, p, tail, d_stats, d_g_loss, d_g_row_loss,
-                                                                         d_dlogits, ldd, (hipStream_t)stream);
+    return gradient_of(dtype, tail)(d_logits, ld, N, V, temperature, p, d_stats, d_g_loss, d_g_row_loss, d_dlogits, ldd, (hipStream_t)stream);
 }

@@ -574,7 +574,7 @@ def test_refused_across_devices(cuda_device):
 
 # Calls of many rows take other threads per row than calls of few: some rows of each against the oracle, the others by the sums they enter.
 MANY = [(4500, 40), (1100, 300), (1100, 700), (1100, 1500), (1100, 2040), (1100, 3000), (1100, 9000), (600, 3000), (300, 1000), (300, 3000), (300, 9000), (300, 20000),
-        (200, 20000), (100, 40000), (128, 33000)]
+        (200, 20000), (100, 40000), (128, 33000), (1300, 16000)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -624,3 +624,29 @@ def test_many_rows(cuda_device, dtype, n, chunks):
         for d in (r.dlogits, apart):
             _near(d[at], grad, e_grad * (1 + 4 * ol.U), "dlogits", rounded=dtype == BF16)
             assert torch.isfinite(d).all() and not d[args[2] == 0].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [9, 100, 1000])
+def test_gradients_of_very_many_short_rows(cuda_device, dtype, v):
+    """more logits than the chip's caches hold: the same bits as a call of the last rows alone"""
+    from autognothi_amd import ops
+    for mb in (200, 340):
+        n = mb * 1000000 // (v * (4 if dtype == F32 else 2))
+        gen = torch.Generator(cuda_device).manual_seed(v)
+        z = torch.randn(n, v, device=cuda_device, generator=gen).to(dtype)
+        tok = torch.randint(0, v, (n,), device=cuda_device, generator=gen)
+        g = torch.randn(n, device=cuda_device, generator=gen)
+        ids = torch.randint(0, v, (n, 4), device=cuda_device, generator=gen)
+        lp = torch.log_softmax(torch.randn(n, 4, device=cuda_device, generator=gen), 1) - 0.3
+        for sl in (slice(None), slice(n - 7, n)):
+            f = ops.token_logprobs(z[sl], tok[sl])
+            d = ops.token_logprobs_bwd(z[sl], f, tok[sl], g[sl], g[sl])
+            t = ops.topk_distill(z[sl], ids[sl], lp[sl], g[sl], tail=True, want_grad=False)
+            e = ops.topk_distill_bwd(z[sl], t, ids[sl], lp[sl], g[sl], tail=True)
+            if sl.start is None:
+                all_ = (f.logp[-7:], f.entropy[-7:], d[-7:], t.row_loss[-7:], e[-7:])
+                assert torch.isfinite(d).all() and torch.isfinite(e).all()
+            else:
+                for a, b in zip(all_, (f.logp, f.entropy, d, t.row_loss, e)):
+                    assert torch.equal(a, b)

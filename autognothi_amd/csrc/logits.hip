@@ -492,6 +492,10 @@ struct Parts {
     unsigned long long* keys;
 };
 
+// A row, or (PART) one part of it, by TH threads.  Bound by the read of the logits: 16384 x 30522 bf16 in 173 us, 2000 x 32000 fp32 in 40 us
+// (5.8 and 6.3 TB/s), with 100 alternatives 8192 x 131072 bf16 in 400 us (6.0 TB/s, 16 % of it the slots that are read again).  A few rows are
+// bound by the chain join, bisection, second read, sort: one row of 30522 fp32 with 5 alternatives 10.3 us.  Two chunks a lane are added up
+// while two are on their way: four gained nothing and cost a quarter of the waves.
 template <typename T, int TH, bool TOP, bool PART>
 __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                          int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
@@ -642,7 +646,8 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
     if (TOP) place_wave<T>(cand, n, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
 }
 
-// Rows of up to 64 (W = 16 lanes a row) or 2041 / 2045 logits (W = 64): the whole row lives in registers, the maximum is found first.
+// Rows of up to 64 (W = 16 lanes a row) or 2048 logits (W = 64; where a list is long for the row's slots): the whole row lives in registers, the
+// maximum is found first.  64000 x 10 fp32 with 3 alternatives 7.8 us, 262144 x 64 123 us: bound by the work per row, not by its bytes.
 template <typename T, int W> struct Small;
 template <typename T> struct Small<T, 16> {   // element j of a lane: lane + 16 j
     static constexpr int NE = 4;
@@ -823,7 +828,8 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // ---- gradients ------------------------------------------------------------------------------------------------------------------
 // Both gradients are one map over the row, e_i = exp2((z_i - m) c) times a number of the row (the entropy's: times a linear function of its
 // exponent), and a few places (the given token, the listed ones) where something is added: those are written again once the row is done.
-// One read and one write of the row; a lane has U chunks in flight.
+// One read and one write of the row; a lane has U chunks in flight.  Bound by memory: 16384 x 30522 bf16 in 335 us (6.1 TB/s), 2000 x 32000 fp32 in
+// 75 us (6.8 TB/s, some of it still cached), with a list of 50 2048 x 65537 bf16 in 84 us (5.9 TB/s).
 
 // Which of a gradient's accesses go past the chip's memory-side cache of 256 MiB.  Logits and gradient that do not fit it together: the stores,
 // so that what the forward pass left of the logits stays (what reads the gradient next is a matrix product, which can wait for memory); logits
@@ -1089,7 +1095,8 @@ template <bool TAIL> __device__ __forceinline__ float row_loss_of(const Teacher&
     return tau * tau * L;
 }
 
-// Rows of up to 64 logits, 16 lanes a row: the row, the listed masses of its tokens and the gradient stay in registers.
+// Rows of up to 64 logits, 16 lanes a row: the row, the listed masses of its tokens and the gradient stay in registers.  Bound by the work on the
+// lists (each lane looks at every slot).
 template <typename T, bool TAIL, bool GRAD>
 __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p,
                                                             float* __restrict__ row_loss, float* __restrict__ stats, T* __restrict__ dz, int64_t ldd) {
@@ -1168,6 +1175,9 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 // the next round's or the next row's chunk as soon as the chunk is done with, so that memory is busy through all of it.
 // The list is the first wave's: it works on it while the row arrives, marks the listed tokens for the sums of all waves, adds their own part,
 // and writes the loss and the listed tokens' gradients.  MULTI: rows of several rounds.
+// Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 928 us (4.6 TB/s; a copy reaches 4.8), 24576 x 1000 fp32 with
+// 25 in 41 us; the loss alone, 2048 x 65537 bf16 with 50, in 42 us (5.5 TB/s).  Reading a row again for its gradient instead of keeping it took
+// 1310 us where this takes 928; 16 rows of 30522 fp32 take 11.2 us, the chain list, sums, join, gradient.
 template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
     const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
@@ -1360,6 +1370,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
     }
 }
 
+// The gradient apart from the loss: the same map and list, with the row's numbers read back.
 template <typename T, int TH, bool TAIL, Past PAST>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, Distill p,
                                                                           const float* __restrict__ stats, const float* __restrict__ g_loss,
@@ -1397,7 +1408,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, list_lds[team], d, [&](int i) { return share.has(i); });
 }
 
-// sum_n w_n L_n in a fixed order
+// sum_n w_n L_n in a fixed order, in doubles (a product of two floats is exact): one workgroup, latency (16 rows 3.8 us, 24576 4.7)
 __global__ __launch_bounds__(1024) void weighted_sum_kernel(const float* __restrict__ row_loss, const float* __restrict__ weights, float weight0, int N,
                                                             float* __restrict__ loss) {
     __shared__ double red[16];

@@ -4,8 +4,8 @@
 // With x = z / temperature, m a reference of the row and s = sum_i exp(x_i - m):
 //     log p_i = (x_i - m) - ln s,   lse = m + ln s,   H = ln s - (1/s) sum_i exp(x_i - m) (x_i - m).
 // One pass over the row computes all of it: every lane keeps its own (m, s, t) and moves its reference only when a logit passes it by more
-// than LG_SLACK, the lanes are joined once at the end.  A row belongs to a TEAM of 16 or 64 lanes (rows of a few to 2048 logits) or to a
-// workgroup of 256, 512 or 1024 threads, and is read in 16-byte pieces ("chunks") from the 16-byte boundary at or below its start, so that
+// than LG_SLACK, the lanes are joined once at the end.  A row belongs to a TEAM of 16 or 64 lanes or to a workgroup of 256, 512
+// or 1024 threads (a few long ones to several workgroups), and is read in 16-byte pieces ("chunks") from the 16-byte boundary at or below its start, so that
 // every whole chunk is one aligned load whatever the row stride is.  Sums are fp32 in a fixed order, no atomics: results are
 // bit-reproducible.
 #include "common.h"
@@ -835,7 +835,9 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // so that what the forward pass left of the logits stays (what reads the gradient next is a matrix product, which can wait for memory); logits
 // that do not fit it alone: the loads too.  Rows of 32001 bf16, forward and backward, a copy into the logits before and a sum of the gradient
 // after them taken off: 128 MB of logits 74 us (stores past it: 77), 160 MB 94 -> 86 (loads too: 85), 192 MB 116 -> 99 (103),
-// 256 MB 148 -> 129 (124), 300 MB 178 -> 161 (148; without the copy and the sum 181 -> 149, 150), 320 MB 191 -> 177 (159), 1 GB 542 -> 530 (518).  The kernel that computes loss and gradient in one gains nothing.
+// 256 MB 148 -> 129 (124), 300 MB 178 -> 161 (148; without the copy and the sum 181 -> 149, 150), 320 MB 191 -> 177 (159), 1 GB 542 -> 530 (518).  The kernel that computes loss and gradient in one gains only
+// where it reads a row twice, and only by the stores: rows of 200001 bf16, 100 MB 62 -> 73 us, 160 MB 106 -> 101, 512 MB 278 -> 239, 2 GB 1020 -> 928
+// (rows of 50001, 410 MB 189 -> 197).
 enum Past { PAST_NONE, PAST_STORES, PAST_ALL };
 inline Past past_cache(int64_t bytes) {
     constexpr int64_t cache = 256 << 20;
@@ -1178,7 +1180,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 // Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 928 us (4.6 TB/s; a copy reaches 4.8), 24576 x 1000 fp32 with
 // 25 in 41 us; the loss alone, 2048 x 65537 bf16 with 50, in 42 us (5.5 TB/s).  Reading a row again for its gradient instead of keeping it took
 // 1310 us where this takes 928; 16 rows of 30522 fp32 take 11.2 us, the chain list, sums, join, gradient.
-template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD>
+template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD, Past PAST = PAST_NONE>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
     const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
     T* __restrict__ dz, int64_t ldd) {
@@ -1349,7 +1351,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : N
                 for (int i = 0; i < NC; ++i) {
                     // (a new value for the compiler: else it keeps the sums' unpacked logits, twice the chunks' registers, for the gradient)
                     asm volatile("" : "+v"(v[i]));
-                    if (i0 + i * TH + t1 < n) gradient_chunk<false>(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
+                    if (i0 + i * TH + t1 < n) gradient_chunk<PAST != PAST_NONE>(row, row.first + i0 + i * TH + t1, v[i], c, ref, ga, d);
                     v[i] = *reinterpret_cast<const chunk_t*>(from + min(i * TH + t1, to) * E);
                 }
             };
@@ -1559,8 +1561,8 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
         AG_LAUNCH_CHECK();
         return AG_OK;
     }
-#define LG_CALL(TH, NC, MULTI, PER_CU)                                                                                                                       \
-    hipLaunchKernelGGL((distill_kernel<T, TH, NC, MULTI, TAIL, GRAD>), dim3(min(ceil_div(N, TH < 256 ? 256 / TH : 1), cus * (PER_CU))), dim3(TH < 256 ? 256 : TH), \
+#define LG_CALL(TH, NC, MULTI, PER_CU, ...)                                                                                                                       \
+    hipLaunchKernelGGL((distill_kernel<T, TH, NC, MULTI, TAIL, GRAD __VA_OPT__(, ) __VA_ARGS__>), dim3(min(ceil_div(N, TH < 256 ? 256 / TH : 1), cus * (PER_CU))), dim3(TH < 256 ? 256 : TH), \
                        (size_t)bit_words<T>(V) * 4 * (TH < 256 ? 256 / TH : 1), s, z, ld, N, V, temperature, c, inv_t, p, d_row_loss, d_stats, dz, ldd)
     if constexpr (GRAD) {
         if (chunks <= 4 * 64) LG_CALL(64, 4, false, 6);
@@ -1570,7 +1572,8 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
         else if (N > 2 * cus && chunks <= 16 * 256) LG_CALL(256, 16, false, 4);
         else if (chunks <= 16 * 512) LG_CALL(512, 16, false, 2);
         else if (chunks <= 16 * 1024) LG_CALL(1024, 16, false, 1);
-        else LG_CALL(1024, 16, true, 1);
+        else if (past_cache((int64_t)N * V * (int64_t)sizeof(T)) == PAST_NONE) LG_CALL(1024, 16, true, 1);
+        else LG_CALL(1024, 16, true, 1, PAST_STORES);
     } else {
         if (chunks <= (N <= 4 * cus ? 512 : 2048)) LG_CALL(64, 4, true, 6);
         else if (N <= cus && chunks >= 4096) LG_CALL(1024, 8, true, 1);

@@ -12,6 +12,9 @@ loss_logits_kl_divergence`` here).  These do the same for rows too wide for that
 Logits are fp32 or bf16 [..., V] on an MI355X; there is no CPU fallback.  Forward and backward read the logits once each and keep a few numbers
 per row between them, so the logits must not be changed in place in the meantime (autograd checks that).  Loops that compute their own gradients
 call ``ops.topk_distill``, which returns loss and gradient from one call.
+
+Forward and backward can be captured into a HIP graph: warm up on a side stream, let no eager graph of the same leaves live on, and take the
+gradient with ``torch.autograd.grad`` (torch ends the process where a captured ``backward`` meets the accumulator of an eager one).
 """
 from __future__ import annotations
 

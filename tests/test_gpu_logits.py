@@ -574,7 +574,7 @@ def test_refused_across_devices(cuda_device):
 
 # Calls of many rows take other threads per row than calls of few: some rows of each against the oracle, the others by the sums they enter.
 MANY = [(4500, 40), (1100, 300), (1100, 700), (1100, 1500), (1100, 2040), (1100, 3000), (1100, 9000), (600, 3000), (300, 1000), (300, 3000), (300, 9000), (300, 20000),
-        (200, 20000), (100, 40000), (128, 33000), (1300, 16000)]
+        (200, 20000), (100, 40000), (128, 33000), (1300, 16000), (400, 33000)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -835,9 +835,9 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
 // so that what the forward pass left of the logits stays (what reads the gradient next is a matrix product, which can wait for memory); logits
 // that do not fit it alone: the loads too.  Rows of 32001 bf16, forward and backward, a copy into the logits before and a sum of the gradient
 // after them taken off: 128 MB of logits 74 us (stores past it: 77), 160 MB 94 -> 86 (loads too: 85), 192 MB 116 -> 99 (103),
-// 256 MB 148 -> 129 (124), 300 MB 178 -> 161 (148; without the copy and the sum 181 -> 149, 150), 320 MB 191 -> 177 (159), 1 GB 542 -> 530 (518).  The kernel that computes loss and gradient in one gains only
-// where it reads a row twice, and only by the stores: rows of 200001 bf16, 100 MB 62 -> 73 us, 160 MB 106 -> 101, 512 MB 278 -> 239, 2 GB 1020 -> 928
-// (rows of 50001, 410 MB 189 -> 197).
+// 256 MB 148 -> 129 (124), 300 MB 178 -> 161 (148; without the copy and the sum 181 -> 149, 150), 320 MB 191 -> 177 (159),
+// 1 GB 542 -> 530 (518).  The kernel that computes loss and gradient in one gains only where it reads a row twice, and only by the stores: rows of
+// 200001 bf16, 100 MB 62 -> 73 us, 160 MB 106 -> 101, 512 MB 278 -> 239, 2 GB 1020 -> 928 (rows of 50001, 410 MB 189 -> 197).
 enum Past { PAST_NONE, PAST_STORES, PAST_ALL };
 inline Past past_cache(int64_t bytes) {
     constexpr int64_t cache = 256 << 20;
@@ -1544,7 +1544,8 @@ int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperatu
 // Threads of a row and chunks of a thread: the fewest threads whose registers hold the row.  With the gradient, 16384 rows fp32, list of 50,
 // the choice against its neighbour: V 1000: (64, 4) 43.6 us, (64, 8) 50.0; 2040: (64, 8) 80.8, (256, 8) 118.6; 2400: (64, 16) 90, (256, 8) 118;
 // 4000: 141 / 143; 8160: (256, 8) 248, (256, 16) 254; 11184 x 12000: (256, 16) 248, (512, 16) 258; 5592 x 24000: (512, 16) 233, (1024, 16) 274;
-// 2048 x 65520: one round of (1024, 16) 245, rounds of (256, 8) 293.  Four rows a CU or fewer are a matter of latency: 512 x 2040: (64, 8) 11.7,
+// 2048 x 65520: one round of (1024, 16) 245, rounds of (256, 8) 293; past the cache two rounds of (512, 16) are better, the second read being the
+// cache's and two workgroups a CU taking turns: 5119 x 100001 bf16 530 -> 498, 8190 x 131072 963 -> 916, but 2559 x 200001 509 -> 533.  Four rows a CU or fewer are a matter of latency: 512 x 2040: (64, 8) 11.7,
 // (256, 8) 10.6; 64 x 16360: (256, 16) 13.8, (512, 16) 12.0.
 // The loss alone reads each chunk once, whatever the rounds: 8388 x 4000: (64, 4) 32.3, (256, 4) 43.6; 2796 x 12000: 27.5 / 29.7; 2048 x 16384:
 // 29.1 / 27.9; 512 x 4000: 10.7 / 9.1; one row a CU or fewer, 64 x 64000: (256, 4) 20.1, (1024, 8) 13.0.
@@ -1571,9 +1572,13 @@ int distill(const void* d_logits, int64_t ld, int N, int V, float temperature, c
         else if (chunks <= 8 * 256) LG_CALL(256, 8, false, 5);
         else if (N > 2 * cus && chunks <= 16 * 256) LG_CALL(256, 16, false, 4);
         else if (chunks <= 16 * 512) LG_CALL(512, 16, false, 2);
-        else if (chunks <= 16 * 1024) LG_CALL(1024, 16, false, 1);
-        else if (past_cache((int64_t)N * V * (int64_t)sizeof(T)) == PAST_NONE) LG_CALL(1024, 16, true, 1);
-        else LG_CALL(1024, 16, true, 1, PAST_STORES);
+        else if (past_cache((int64_t)N * V * (int64_t)sizeof(T)) == PAST_NONE) {
+            if (chunks <= 16 * 1024) LG_CALL(1024, 16, false, 1);
+            else LG_CALL(1024, 16, true, 1);
+        } else {
+            if (chunks <= 16 * 1024) LG_CALL(512, 16, true, 2, PAST_STORES);
+            else LG_CALL(1024, 16, true, 1, PAST_STORES);
+        }
     } else {
         if (chunks <= (N <= 4 * cus ? 512 : 2048)) LG_CALL(64, 4, true, 6);
         else if (N <= cus && chunks >= 4096) LG_CALL(1024, 8, true, 1);

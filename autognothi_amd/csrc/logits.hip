@@ -1177,9 +1177,9 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 // the next round's or the next row's chunk as soon as the chunk is done with, so that memory is busy through all of it.
 // The list is the first wave's: it works on it while the row arrives, marks the listed tokens for the sums of all waves, adds their own part,
 // and writes the loss and the listed tokens' gradients.  MULTI: rows of several rounds.
-// Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 928 us (4.6 TB/s; a copy reaches 4.8), 24576 x 1000 fp32 with
-// 25 in 41 us; the loss alone, 2048 x 65537 bf16 with 50, in 42 us (5.5 TB/s).  Reading a row again for its gradient instead of keeping it took
-// 1310 us where this takes 928; 16 rows of 30522 fp32 take 11.2 us, the chain list, sums, join, gradient.
+// Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 885 us (4.9 TB/s without what the cache gives the second read;
+// a copy reaches 4.8), 24576 x 1000 fp32 with 25 in 41 us; the loss alone, 2048 x 65537 bf16 with 50, in 43 us (5.4 TB/s).  Without the prefetch
+// in place 8192 x 131072 took 1310 us; 16 rows of 30522 fp32 take 11.2 us, the chain list, sums, join, gradient.
 template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD, Past PAST = PAST_NONE>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH, NC == 16 || TH == 1024 ? 4 : NC == 8 ? 5 : 6) void distill_kernel(
     const T* __restrict__ z, int64_t ld, int N, int V, float tau, float c, float inv_t, Distill p, float* __restrict__ row_loss, float* __restrict__ stats,
@@ -1410,7 +1410,8 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void distill_bwd_kernel(const 
     if (lead) listed_gradients<T, W>(row, gx, p.K, 0u, s, g, c, list_lds[team], d, [&](int i) { return share.has(i); });
 }
 
-// sum_n w_n L_n in a fixed order, in doubles (a product of two floats is exact): one workgroup, latency (16 rows 3.8 us, 24576 4.7)
+// sum_n w_n L_n in a fixed order, in doubles (a product of two floats is exact): one workgroup, latency: 16 rows 2.5 us, 24576 4.0,
+// 200000 24 (more loads in flight, 16 or 24 of each array: the same; one wave for few rows: 2.1 us)
 __global__ __launch_bounds__(1024) void weighted_sum_kernel(const float* __restrict__ row_loss, const float* __restrict__ weights, float weight0, int N,
                                                             float* __restrict__ loss) {
     __shared__ double red[16];

@@ -198,8 +198,8 @@ __global__ void softmax_bwd_kernel(const float* __restrict__ y, const float* __r
 }
 
 // LayerNorm backward.  One wave per row, the row held in registers (NC = H/64 columns per lane, one read of x and dy);
-// dgamma/dbeta partials are carried in registers across the wave's rows and folded once per wave through LDS into
-// part[block][2][H].  NC = 0: any H (<= 4096), columns re-read from L2 and LDS atomics per row.
+// dgamma/dbeta partials are carried in registers across the wave's rows and folded once per wave, in the waves' order,
+// through LDS into part[block][2][H].  NC = 0: any H (<= 4096), columns re-read from L2 and LDS atomics per row.
 template <int NC>
 __global__ __launch_bounds__(256) void ln_bwd_kernel(const float* __restrict__ x, const float* __restrict__ g, const float* __restrict__ dy,
                                                      int rows, int H, float eps, float* __restrict__ dx, float* __restrict__ part,
@@ -236,10 +236,15 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const float* __restrict__ x
                 ab[i] += dv[i];
             }
         }
+        for (int w = 0; w < nw; ++w) {   // the waves of the block in their order: the sums repeat bit for bit
+            if (wave == w) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {   // LDS atomics: waves of one block only, once per wave
-            atomicAdd(&sacc[lane + 64 * i], ag[i]);
-            atomicAdd(&sacc[H + lane + 64 * i], ab[i]);
+                for (int i = 0; i < NC; ++i) {
+                    sacc[lane + 64 * i] += ag[i];
+                    sacc[H + lane + 64 * i] += ab[i];
+                }
+            }
+            __syncthreads();
         }
     } else {
         for (int row = blockIdx.x * nw + wave; row < rows; row += gridDim.x * nw) {

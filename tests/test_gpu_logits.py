@@ -650,3 +650,46 @@ def test_gradients_of_very_many_short_rows(cuda_device, dtype, v):
             else:
                 for a, b in zip(all_, (f.logp, f.entropy, d, t.row_loss, e)):
                     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n,v", [(2, 300000), (40, 30522), (1500, 3000)])
+def test_two_threads_on_two_streams(cuda_device, n, v):
+    """calls at the same time share nothing: each thread's results are those of its calls alone"""
+    import threading
+    from autognothi_amd import ops
+    made = []
+    for seed in range(2):
+        gen = torch.Generator(cuda_device).manual_seed(seed)
+        z = torch.randn(n, v, device=cuda_device, generator=gen)
+        ids = torch.randint(0, v, (n, 6), device=cuda_device, generator=gen)
+        lp = torch.log_softmax(torch.randn(n, 6, device=cuda_device, generator=gen), 1) - 0.2
+        made.append((z, ids, lp))
+
+    def calls(z, ids, lp):
+        f = ops.token_logprobs(z, ids[:, 0].contiguous(), 8)
+        d = ops.topk_distill(z, ids, lp, tail=True)
+        return [t.clone() for t in (f.logp, f.entropy, f.lse, f.top_ids, f.top_logp, ops.token_logprobs_bwd(z, f, ids[:, 0].contiguous(), f.lse, f.entropy),
+                                    d.loss, d.row_loss, d.dlogits)]
+
+    alone = [calls(*m) for m in made]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream(cuda_device)
+            with torch.cuda.stream(stream):
+                for _ in range(8):
+                    got = calls(*made[i])
+                    stream.synchronize()
+                    for a, b in zip(got, alone[i]):
+                        assert torch.equal(a, b)
+        except BaseException as e:      # noqa: BLE001 (reported by the main thread)
+            failed.append((i, e))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

@@ -117,6 +117,7 @@ SIGNATURES = {
     "ag_kl_loss": (i32, [vp, vp, i32, i32, vp, vp, vp]),
     "ag_token_logprobs_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "ag_token_logprobs": (i32, [vp, i64, i32, i32, i32, f32, vp, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "ag_token_logprobs_saved": (i32, [vp, i64, i32, i32, i32, f32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "ag_token_logprobs_bwd": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, i64, vp]),
     "ag_topk_distill": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp, i64, vp]),
     "ag_topk_distill_bwd": (i32, [vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp, i64, vp]),

@@ -469,13 +469,19 @@ template <typename T, int TH> __device__ __forceinline__ void place_all(TopLds<T
     }
 }
 
+// what the gradient takes from a row's sums: m and s, together (one store of a row's 8 bytes costs what each of two costs: rows of a 128-byte line
+// come from eight L2s)
+typedef __attribute__((ext_vector_type(2), aligned(4))) float row_sums_t;
+
+// (saved: H once more, where the caller may edit `entropy` before the gradient is computed; NULL: not wanted)
 template <typename T>
-__device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, int64_t N, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
-                                          float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats) {
-    stats[r] = a.m;
-    stats[N + r] = a.s;
+__device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
+                                          float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats, float* __restrict__ saved) {
+    *reinterpret_cast<row_sums_t*>(stats + 2 * r) = row_sums_t{a.m, a.s};
+    const float h = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
     lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
-    entropy[r] = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
+    entropy[r] = h;
+    if (saved) saved[r] = h;
     if (tokens) {
         const int64_t t = tokens[r];
         float v = 0.f;
@@ -499,8 +505,8 @@ struct Parts {
 template <typename T, int TH, bool TOP, bool PART>
 __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                          int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
-                                                         float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp,
-                                                         Parts parts) {
+                                                         float* __restrict__ stats, float* __restrict__ saved, int64_t* __restrict__ top_ids,
+                                                         float* __restrict__ top_logp, Parts parts) {
     constexpr int E = Chunk<T>::E, U = 2;   // 2 U chunks of a lane are in flight
     __shared__ float red[3 * (TH / 64)];
     const int64_t r = PART ? blockIdx.x / parts.count : blockIdx.x;
@@ -547,7 +553,7 @@ __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict_
     if (PART) {
         if (tid == 0) parts.acc[blockIdx.x] = make_float4(a.m, a.s, a.t, 0.f);
     } else if (tid == 0) {
-        write_row(row.z, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+        write_row(row.z, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats, saved);
     }
     if (!TOP) return;
     __shared__ TopLds<TH> lds;
@@ -629,8 +635,8 @@ __global__ __launch_bounds__(TH, 7) void logprobs_wg_kernel(const T* __restrict_
 template <typename T, bool TOP>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__ z, int64_t ld, int V, float c, float inv_t, const int64_t* __restrict__ tokens,
                                                            int k, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse,
-                                                           float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logp,
-                                                           Parts parts) {
+                                                           float* __restrict__ stats, float* __restrict__ saved, int64_t* __restrict__ top_ids,
+                                                           float* __restrict__ top_logp, Parts parts) {
     __shared__ unsigned long long cand[256];
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x, n = parts.count * k;
@@ -641,7 +647,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
     const Acc a = lanes_join<64>(mine, c);
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (lane == 0) write_row(z + r * ld, V, r, gridDim.x, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (lane == 0) write_row(z + r * ld, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats, saved);
     Team<64>::sync();
     if (TOP) place_wave<T>(cand, n, V, {top_ids + r * k, top_logp + r * k, k, a.m, inv_t, log_s, empty});
 }
@@ -707,7 +713,7 @@ template <typename T, int W, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict__ z, int64_t ld, int N, int V, float c, float inv_t,
                                                              const int64_t* __restrict__ tokens, int k, float* __restrict__ logp,
                                                              float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats,
-                                                             int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+                                                             float* __restrict__ saved, int64_t* __restrict__ top_ids, float* __restrict__ top_logp) {
     using S = Small<T, W>;
     constexpr int NE = S::NE, CAP = W == 16 ? 64 : 256;
     const int lane = threadIdx.x & (W - 1), team = threadIdx.x / W;
@@ -731,7 +737,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const T* __restrict
     a.t = lanes_join<W>(a.t, Add());
     const bool empty = a.s == 0.f;
     const float log_s = empty ? -INFINITY : logf(a.s);
-    if (lane == 0) write_row(zr, V, r, N, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats);
+    if (lane == 0) write_row(zr, V, r, a, inv_t, log_s, empty, tokens, logp, entropy, lse, stats, saved);
     if (!TOP) return;
     __shared__ unsigned long long cand_lds[256 / W][CAP];
     unsigned long long* cand = cand_lds[team];
@@ -903,7 +909,8 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void logprobs_bwd_kernel(const
     const int tid = Team<TH>::rank();
     const Row<T> row(z + r * ld, V);
     T* d = dz + r * ldd;
-    const Acc a = {q.stats[r], q.stats[N + r], 0.f};
+    const row_sums_t st = *reinterpret_cast<const row_sums_t*>(q.stats + 2 * r);
+    const Acc a = {st.x, st.y, 0.f};
     const int64_t t = q.tokens ? q.tokens[r] : -1;
     const float gt = t < 0 ? 0.f : t < V ? q.g_logp[r] : NAN, gh = q.g_entropy ? q.g_entropy[r] : 0.f;
     float gs = 0.f;
@@ -1502,19 +1509,19 @@ Parts parts_of(int N, int V, int dtype, int k) {
 //       one row a CU or fewer, longer than 16384: 1024 threads      64 x 240000 fp32, k 128: 35.7 us, 512 threads 42.0; x 65536: 20.3 / 20.1
 template <typename T, bool TOP>
 int logprobs(const void* d_logits, int64_t ld, int N, int V, float temperature, const int64_t* d_tokens, int k, float* d_logp, float* d_entropy, float* d_lse,
-             float* d_stats, int64_t* d_top_ids, float* d_top_logp, Parts parts, hipStream_t s) {
+             float* d_stats, float* d_saved, int64_t* d_top_ids, float* d_top_logp, Parts parts, hipStream_t s) {
     const float c = log2e_over(temperature), inv_t = one_over(temperature);
     const T* z = (const T*)d_logits;
 #define LG_SMALL(W) hipLaunchKernelGGL((logprobs_small_kernel<T, W, TOP>), team_grid<W>(N), dim3(256), 0, s, z, ld, N, V, c, inv_t, d_tokens, k, d_logp, \
-                                       d_entropy, d_lse, d_stats, d_top_ids, d_top_logp)
+                                       d_entropy, d_lse, d_stats, d_saved, d_top_ids, d_top_logp)
 #define LG_WG(TH, PART) hipLaunchKernelGGL((logprobs_wg_kernel<T, TH, TOP, PART>), dim3(N * (PART ? parts.count : 1)), dim3(TH), 0, s, z, ld, V, c, inv_t, \
-                                           d_tokens, k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, parts)
+                                           d_tokens, k, d_logp, d_entropy, d_lse, d_stats, d_saved, d_top_ids, d_top_logp, parts)
     const int chunks = V / Chunk<T>::E, cus = cu_count();
     if (parts.count) {
         LG_WG(256, true);
         AG_LAUNCH_CHECK();
         hipLaunchKernelGGL((logprobs_join_kernel<T, TOP>), dim3(N), dim3(64), 0, s, z, ld, V, c, inv_t, d_tokens, k, d_logp, d_entropy, d_lse, d_stats,
-                           d_top_ids, d_top_logp, parts);
+                           d_saved, d_top_ids, d_top_logp, parts);
     } else if (V <= Small<T, 16>::max_v()) LG_SMALL(16);
     else if (V <= Small<T, 64>::max_v() && (chunks < 16 || min(chunks, 64 * min(max(chunks / 64, 1), 4)) < k + k / 2)) LG_SMALL(64);
     else if (chunks <= (N <= 4 * cus ? 512 : 2048)) LG_WG(64, false);
@@ -1617,16 +1624,15 @@ extern "C" size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int
     return (size_t)std::max(N, 0) * p.count * (sizeof(float4) + (size_t)std::max(top_k, 0) * sizeof(unsigned long long));
 }
 
-extern "C" int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
-                                 float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp,
-                                 void* d_workspace, size_t workspace_bytes, void* stream) {
-    if (int rc = check_rows("ag_token_logprobs", d_logits, ld, N, V, dtype, temperature)) return rc;
-    AG_REQUIRE(top_k >= 0 && top_k <= AG_LOGITS_MAX_TOP && top_k <= V, "ag_token_logprobs: top_k = %d (0 to min(%d, %d logits))", top_k,
-               AG_LOGITS_MAX_TOP, V);
+static int token_logprobs_entry(const char* who, const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
+                                float* d_logp, float* d_entropy, float* d_lse, float* d_stats, float* d_saved, int64_t* d_top_ids, float* d_top_logp,
+                                void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_rows(who, d_logits, ld, N, V, dtype, temperature)) return rc;
+    AG_REQUIRE(top_k >= 0 && top_k <= AG_LOGITS_MAX_TOP && top_k <= V, "%s: top_k = %d (0 to min(%d, %d logits))", who, top_k, AG_LOGITS_MAX_TOP, V);
     if (N == 0) return AG_OK;
-    AG_REQUIRE(d_entropy && d_lse && d_stats && (!d_tokens || d_logp) && (top_k == 0 || (d_top_ids && d_top_logp)), "ag_token_logprobs: null pointer");
+    AG_REQUIRE(d_entropy && d_lse && d_stats && (!d_tokens || d_logp) && (top_k == 0 || (d_top_ids && d_top_logp)), "%s: null pointer", who);
     const size_t need = ag_token_logprobs_workspace_bytes(N, V, dtype, top_k);
-    AG_REQUIRE(!d_workspace || (workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0), "ag_token_logprobs: workspace of %zu bytes (16-byte aligned, %zu needed)",
+    AG_REQUIRE(!d_workspace || (workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0), "%s: workspace of %zu bytes (16-byte aligned, %zu needed)", who,
                workspace_bytes, need);
     Parts parts = {0, 0, nullptr, nullptr};
     if (d_workspace && need) {
@@ -1635,7 +1641,22 @@ extern "C" int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V,
         parts.keys = (unsigned long long*)(parts.acc + (size_t)N * parts.count);
     }
     const auto run = dtype == AG_BF16 ? (top_k ? logprobs<bf16_t, true> : logprobs<bf16_t, false>) : (top_k ? logprobs<float, true> : logprobs<float, false>);
-    return run(d_logits, ld, N, V, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, d_top_ids, d_top_logp, parts, (hipStream_t)stream);
+    return run(d_logits, ld, N, V, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, d_saved, d_top_ids, d_top_logp, parts, (hipStream_t)stream);
+}
+
+extern "C" int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
+                                 float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp,
+                                 void* d_workspace, size_t workspace_bytes, void* stream) {
+    return token_logprobs_entry("ag_token_logprobs", d_logits, ld, N, V, dtype, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats, nullptr, d_top_ids,
+                                d_top_logp, d_workspace, workspace_bytes, stream);
+}
+
+extern "C" int ag_token_logprobs_saved(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
+                                       float* d_logp, float* d_entropy, float* d_lse, float* d_stats, float* d_saved_entropy, int64_t* d_top_ids,
+                                       float* d_top_logp, void* d_workspace, size_t workspace_bytes, void* stream) {
+    AG_REQUIRE(d_saved_entropy || N == 0, "ag_token_logprobs_saved: null pointer");
+    return token_logprobs_entry("ag_token_logprobs_saved", d_logits, ld, N, V, dtype, temperature, d_tokens, top_k, d_logp, d_entropy, d_lse, d_stats,
+                                d_saved_entropy, d_top_ids, d_top_logp, d_workspace, workspace_bytes, stream);
 }
 
 extern "C" int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const float* d_stats,

@@ -37,7 +37,7 @@ class Logprobs(NamedTuple):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature):
-        r = ops.token_logprobs(logits, tokens, top_k, temperature)
+        r = ops._token_logprobs(logits, tokens, top_k, temperature, no_views=True)
         ctx.save_for_backward(logits, tokens, r.stats, r.top_ids)
         ctx.temperature = r.temperature
         ctx.set_materialize_grads(False)

@@ -750,13 +750,14 @@ def kl_loss(ref: Tensor, cur: Tensor, want_grad: bool = True):
 
 # ----------------------------------------------------------------------------- wide rows of logits
 class TokenLogprobs(NamedTuple):
-    """token_logprobs' results for N rows; everything but the ids fp32.  ``stats`` is what the backward reads."""
+    """token_logprobs' results for N rows; everything but the ids fp32.  The backward reads rows 1, 3 and 4 of ``stats``, which share no memory with
+    the results (those may be edited), and for d_top_logp ``top_ids``."""
     logp: Optional[Tensor]        # [N] log-probability of the given token (None: no tokens given)
     entropy: Tensor               # [N]
     lse: Tensor                   # [N] ln sum exp(logits / temperature)
     top_ids: Optional[Tensor]     # [N, top_k] int64, descending, ties by the lower index (None: top_k = 0)
     top_logp: Optional[Tensor]    # [N, top_k]
-    stats: Tensor                 # [5, N]: logp, entropy, lse and two rows of its own
+    stats: Tensor                 # [5, N]: logp and lse (the results' own memory, rows 0 and 2), the entropy once more and 2 N numbers of its own
     temperature: float
 
 
@@ -810,6 +811,11 @@ def _check_temperature(who: str, temperature: float) -> float:
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
     """ln p of a given token in every row of ``logits`` [N, V] (fp32 / bf16, any row stride), the row's entropy and log-normaliser, and its
     ``top_k`` (<= 128) likeliest alternatives, p = softmax(logits / temperature).  tokens [N] int64: negative = ignored (0), >= V = NaN."""
+    return _token_logprobs(logits, tokens, top_k, temperature, False)
+
+
+def _token_logprobs(logits: Tensor, tokens: Optional[Tensor], top_k: int, temperature: float, no_views: bool) -> TokenLogprobs:
+    """no_views: every result a tensor of its own memory (an autograd Function's output that is a view refuses to be edited)"""
     who = "token_logprobs"
     logits, n, v, ld, dtype = _logit_rows(who, logits)
     temperature = _check_temperature(who, temperature)
@@ -818,17 +824,18 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
     dev = logits.device
     tokens = _row_arg(who, "tokens", tokens, (n,), torch.int64, dev)
     L.require_gpu(logits)
-    stats = torch.empty(5, n, dtype=torch.float32, device=dev)      # (one allocation, sizes not as a tuple: at one row the host's time is the call's)
-    logp, entropy, lse, _, _ = stats.unbind(0)
-    at = stats.data_ptr()
+    stats = torch.empty(5, n, dtype=torch.float32, device=dev)      # (few allocations, sizes not as tuples: at one row the host's time is the call's)
+    entropy, lse = stats.new_empty(n), stats.new_empty(n) if no_views else stats[2]
+    logp = None if tokens is None else stats.new_empty(n) if no_views else stats[0]
     ids = torch.empty(n, top_k, dtype=torch.int64, device=dev) if top_k else None
-    top = torch.empty(n, top_k, dtype=torch.float32, device=dev) if top_k else None
+    top = stats.new_empty(n, top_k) if top_k else None
+    at = stats.data_ptr()
     with L.on(dev):
         need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 128 else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        L.check(L.lib().ag_token_logprobs(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
-                                          L.ptr(ids), L.ptr(top), L.ptr(ws), need, L.stream()))
-    return TokenLogprobs(None if tokens is None else logp, entropy, lse, ids, top, stats, temperature)
+        L.check(L.lib().ag_token_logprobs_saved(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, L.ptr(logp), L.ptr(entropy), L.ptr(lse),
+                                                at + 12 * n, at + 4 * n, L.ptr(ids), L.ptr(top), L.ptr(ws), need, L.stream()))
+    return TokenLogprobs(logp, entropy, lse, ids, top, stats, temperature)
 
 
 def token_logprobs_bwd(logits: Tensor, fwd: TokenLogprobs, tokens: Optional[Tensor] = None, d_logp: Optional[Tensor] = None,

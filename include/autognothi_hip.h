@@ -513,15 +513,20 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
 #define AG_LOGITS_MAX_TOP 128
 /* d_lse [N] = ln sum exp x;  d_entropy [N] = -sum p ln p;  d_logp [N] = ln p of d_tokens[n] (NULL: not asked for; a token < 0 is ignored: 0;
  * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
- * all), and their ln p;  d_stats [2, N]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0.
+ * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0.
  * d_workspace (16-byte aligned, ag_token_logprobs_workspace_bytes; NULL: none): with it a few long rows are shared by several workgroups
  * each; its size is 0 for calls that would not be. */
 size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int top_k);
 int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
                       float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp, void* d_workspace,
                       size_t workspace_bytes, void* stream);
+/* the same, and the entropy once more in d_saved_entropy [N]: for callers that hand the results on to code that may edit them before the gradient is
+ * computed (ag_token_logprobs_bwd then takes d_saved_entropy as its d_entropy). */
+int ag_token_logprobs_saved(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
+                            float* d_logp, float* d_entropy, float* d_lse, float* d_stats, float* d_saved_entropy, int64_t* d_top_ids,
+                            float* d_top_logp, void* d_workspace, size_t workspace_bytes, void* stream);
 /* dlogits [N, V] (dtype, row stride ldd >= V) = the gradient of sum(d_g_logp . logp + d_g_entropy . entropy + d_g_lse . lse + d_g_top_logp . top_logp)
- * (each NULL: zero).  d_stats, d_entropy and d_top_ids of the forward call on the same logits.  An ignored token and a row of -inf get zero. */
+ * (each NULL: zero).  d_stats, d_entropy and d_top_ids as the forward call on the same logits wrote them.  An ignored token and a row of -inf get zero. */
 int ag_token_logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const float* d_stats,
                           const float* d_entropy, const int64_t* d_tokens, const float* d_g_logp, const float* d_g_entropy,
                           const float* d_g_lse, int top_k, const int64_t* d_top_ids, const float* d_g_top_logp, void* d_dlogits, int64_t ldd,

@@ -1,0 +1,90 @@
+"""GPU: what the operators over wide rows of logits hand out belongs to the caller: editing a result in place changes no gradient and no other
+result, here as with elementary torch operations."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _made(dev, n, v, seed=0):
+    gen = torch.Generator(dev).manual_seed(seed)
+    z = torch.randn(n, v, device=dev, generator=gen) * 3.0
+    tokens = torch.randint(0, v, (n,), device=dev, generator=gen)
+    return z, tokens, torch.randn(n, device=dev, generator=gen)
+
+
+# (16 lanes a row, one wave, a workgroup, several workgroups a row)
+SIZES = [(6, 40), (6, 700), (600, 20000), (3, 270000)]
+
+
+@pytest.mark.parametrize("n,v", SIZES)
+@pytest.mark.parametrize("edited", ["logp", "entropy", "lse", "top_logp"])
+def test_a_result_edited_before_the_backward_changes_no_gradient(cuda_device, n, v, edited):
+    from autognothi_amd import ops
+    z, tokens, g = _made(cuda_device, n, v)
+    r = ops.token_logprobs(z, tokens, 3)
+    gt = torch.ones(n, 3, device=cuda_device)
+    want = ops.token_logprobs_bwd(z, r, tokens, g, g, g, gt)
+    others = {f: getattr(r, f).clone() for f in ("logp", "entropy", "lse", "top_ids", "top_logp") if f != edited}
+    getattr(r, edited).mul_(-0.25).add_(7.0)
+    assert torch.equal(ops.token_logprobs_bwd(z, r, tokens, g, g, g, gt), want)
+    for f, t in others.items():
+        assert torch.equal(getattr(r, f), t), f
+
+
+@pytest.mark.parametrize("n,v", SIZES)
+def test_stats_hold_what_the_results_do(cuda_device, n, v):
+    from autognothi_amd import ops
+    z, tokens, _ = _made(cuda_device, n, v)
+    r = ops.token_logprobs(z, tokens, 2)
+    assert r.stats.shape == (5, n)
+    for row, t in zip(r.stats, (r.logp, r.entropy, r.lse)):
+        assert torch.equal(row, t)
+    none = ops.token_logprobs(z, top_k=2)
+    assert none.logp is None and torch.equal(none.stats[1:], r.stats[1:])
+
+
+def _edit(t):
+    t.mul_(2.0)
+    t += 1.0
+
+
+def _same(t):
+    return t * 2.0 + 1.0
+
+
+@pytest.mark.parametrize("shape", [(6, 700), (2, 3, 700)])
+@pytest.mark.parametrize("which", ["logp", "entropy", "lse", "top_logp"])
+def test_autograd_outputs_can_be_edited_in_place(cuda_device, shape, which):
+    """out.mul_(w) of any output: the gradient of the edited graph, and of the other outputs what it was"""
+    from autognothi_amd.models import distill
+    z, tokens, _ = _made(cuda_device, 6, 700)
+    z, tokens = z.view(shape), tokens.view(shape[:-1])
+    grads = []
+    for edit in (False, True):
+        x = z.clone().requires_grad_(True)
+        r = distill.token_logprobs(x, tokens, top_k=3)
+        out = getattr(r, which)
+        if edit:
+            _edit(out)
+        else:
+            out = _same(out)
+        total = (out ** 2).sum() + sum(getattr(r, f).sum() for f in ("logp", "entropy", "lse", "top_logp") if f != which)
+        grads.append((total.detach(), *torch.autograd.grad(total, x)))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["logp", "entropy", "lse", "top_logp"])
+def test_autograd_outputs_edited_behind_the_graph(cuda_device, which):
+    """an edit through detach() leaves the gradients as they were, and the other outputs usable"""
+    from autognothi_amd.models import distill
+    z, tokens, _ = _made(cuda_device, 6, 700)
+    x = z.clone().requires_grad_(True)
+    grads = []
+    for edit in (False, True):
+        r = distill.token_logprobs(x, tokens, top_k=3)
+        if edit:
+            getattr(r, which).detach().mul_(-3.0)
+        grads.append(torch.autograd.grad(sum(getattr(r, f).sum() for f in ("logp", "entropy", "lse", "top_logp")), x)[0])
+    assert torch.equal(*grads)

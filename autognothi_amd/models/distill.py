@@ -77,11 +77,11 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int =
 class _TopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logp, weights, temperature, tail):
-        r = ops.topk_distill(logits, teacher_ids, teacher_logp, weights, temperature, tail, want_grad=False)
+        r = ops._topk_distill(logits, teacher_ids, teacher_logp, weights, temperature, tail, want_grad=False, loss_shape=())
         ctx.save_for_backward(logits, teacher_ids, teacher_logp, weights, r.stats)
         ctx.temperature, ctx.tail = temperature, tail
         ctx.set_materialize_grads(False)
-        return r.loss.reshape(()), r.row_loss
+        return r.loss, r.row_loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable

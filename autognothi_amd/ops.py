@@ -884,6 +884,12 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
     token_logprobs gives them.  Row loss: temperature^2 KL(teacher's list, renormalised || student), or with ``tail`` the list as it is and
     the rest of the teacher's mass as one more class.  weights [N] fp32 (None: 1 / N); a row of weight 0 takes no part (its logits are not
     read).  -> loss, row losses and (want_grad) the loss' gradient, rounded to the logits' dtype once."""
+    return _topk_distill(logits, teacher_ids, teacher_logp, weights, temperature, tail, want_grad, (1,))
+
+
+def _topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weights: Optional[Tensor], temperature: float, tail: bool, want_grad: bool,
+                  loss_shape: Tuple[int, ...]) -> TopkDistill:
+    """loss_shape: (1,), or () for an autograd Function's output (which as a view would refuse to be edited)"""
     who = "topk_distill"
     logits, n, v, ld, dtype = _logit_rows(who, logits)
     temperature = _check_temperature(who, temperature)
@@ -892,7 +898,7 @@ def topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, weig
         raise ValueError(f"{who}: no rows")
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
     L.require_gpu(logits)
-    row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.float32, device=dev)
+    row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(loss_shape, dtype=torch.float32, device=dev)
     stats = None if want_grad and (n > 32 or v <= 65536) else torch.empty(n, 4, dtype=torch.float32, device=dev)   # (few long rows are done in two steps)
     out = torch.empty(n, v, dtype=logits.dtype, device=dev) if want_grad else None
     with L.on(dev):

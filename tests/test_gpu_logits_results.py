@@ -88,3 +88,29 @@ def test_autograd_outputs_edited_behind_the_graph(cuda_device, which):
             getattr(r, which).detach().mul_(-3.0)
         grads.append(torch.autograd.grad(sum(getattr(r, f).sum() for f in ("logp", "entropy", "lse", "top_logp")), x)[0])
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("shape", [(6, 700), (2, 3, 700)])
+def test_autograd_loss_can_be_edited_in_place(cuda_device, shape):
+    """loss += ..., loss.div_(steps) and row.mul_(...): as with any loss"""
+    from autognothi_amd import ops
+    from autognothi_amd.models import distill
+    z, _, _ = _made(cuda_device, 6, 700)
+    rec = ops.token_logprobs(_made(cuda_device, 6, 700, seed=1)[0], top_k=5)
+    ids, lp = rec.top_ids.view(*shape[:-1], 5), rec.top_logp.view(*shape[:-1], 5)
+    grads = []
+    for edit in (False, True):
+        x = z.view(shape).clone().requires_grad_(True)
+        loss, row = distill.loss_topk_distillation(x, ids, lp, tail=True)
+        assert loss.shape == () and row.shape == shape[:-1]
+        if edit:
+            loss += row.sum()
+            loss.div_(4.0)
+            _edit(row)
+        else:
+            loss = (loss + row.sum()) / 4.0
+            row = _same(row)
+        total = loss + (row ** 2).sum()
+        grads.append((total.detach(), *torch.autograd.grad(total, x)))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)

@@ -371,6 +371,17 @@ template <typename T, int TH> __device__ void top_radix(const Row<T>& row, int k
     Team<TH>::sync();
 }
 
+// ln p <= 0 and H >= 0 hold for the numbers, not for their roundings: of a row that is sure of one token, s is 1 and a few roundings.  A value on
+// the wrong side is 0 (a NaN stays one).
+__device__ __forceinline__ float log_prob(float z, float m, float inv_t, float log_s) {
+    const float v = (z - m) * inv_t - log_s;
+    return v > 0.f ? 0.f : v;
+}
+__device__ __forceinline__ float entropy_of(const Acc& a, float log_s) {
+    const float h = log_s - LG_LN2 * (a.t / a.s);
+    return h < 0.f ? 0.f : h;
+}
+
 struct TopOut {
     int64_t* ids;
     float* logp;
@@ -383,7 +394,7 @@ struct TopOut {
         if (place >= k) return;
         if (keys) { keys[place] = me - (unsigned long long)base; return; }   // (the key's low half counts down)
         ids[place] = (int64_t)(0xFFFFFFFFu - (uint32_t)me);
-        logp[place] = empty ? -INFINITY : (key_value((uint32_t)(me >> 32)) - m) * inv_t - log_s;
+        logp[place] = empty ? -INFINITY : log_prob(key_value((uint32_t)(me >> 32)), m, inv_t, log_s);
     }
 };
 
@@ -478,7 +489,7 @@ template <typename T>
 __device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_t r, const Acc& a, float inv_t, float log_s, bool empty, const int64_t* __restrict__ tokens,
                                           float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse, float* __restrict__ stats, float* __restrict__ saved) {
     *reinterpret_cast<row_sums_t*>(stats + 2 * r) = row_sums_t{a.m, a.s};
-    const float h = empty ? 0.f : log_s - LG_LN2 * (a.t / a.s);
+    const float h = empty ? 0.f : entropy_of(a, log_s);
     lse[r] = empty ? -INFINITY : a.m * inv_t + log_s;
     entropy[r] = h;
     if (saved) saved[r] = h;
@@ -486,7 +497,7 @@ __device__ __forceinline__ void write_row(const T* __restrict__ z, int V, int64_
         const int64_t t = tokens[r];
         float v = 0.f;
         if (t >= V) v = NAN;
-        else if (t >= 0) v = empty ? -INFINITY : (Store<T>::load(z + t) - a.m) * inv_t - log_s;
+        else if (t >= 0) v = empty ? -INFINITY : log_prob(Store<T>::load(z + t), a.m, inv_t, log_s);
         logp[r] = v;
     }
 }

@@ -513,7 +513,7 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
 #define AG_LOGITS_MAX_TOP 128
 /* d_lse [N] = ln sum exp x;  d_entropy [N] = -sum p ln p;  d_logp [N] = ln p of d_tokens[n] (NULL: not asked for; a token < 0 is ignored: 0;
  * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
- * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  A row of -inf: lse = ln p = -inf, entropy 0.
+ * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  No ln p is above 0 and no entropy below it.  A row of -inf: lse = ln p = -inf, entropy 0.
  * d_workspace (16-byte aligned, ag_token_logprobs_workspace_bytes; NULL: none): with it a few long rows are shared by several workgroups
  * each; its size is 0 for calls that would not be. */
 size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int top_k);

@@ -1,9 +1,13 @@
 """GPU: what the operators over wide rows of logits hand out belongs to the caller: editing a result in place changes no gradient and no other
-result, here as with elementary torch operations."""
+result, here as with elementary torch operations; and the results keep the signs that the definitions give them."""
+import numpy as np
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+U = 2.0 ** -24
 
 
 def _made(dev, n, v, seed=0):
@@ -114,3 +118,31 @@ def test_autograd_loss_can_be_edited_in_place(cuda_device, shape):
         grads.append((total.detach(), *torch.autograd.grad(total, x)))
     for a, b in zip(*grads):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------ signs
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(4000, 40), (4000, 100), (4000, 700), (4000, 5000), (1500, 30522), (600, 70000), (100, 140000)])
+def test_no_probability_above_one_and_no_entropy_below_zero(cuda_device, dtype, n, v):
+    """rows that are sure of one token: ln p <= 0 and H >= 0 in every bit, and within the bounds of the sums' rounding"""
+    from autognothi_amd import ops
+    gen = torch.Generator(cuda_device).manual_seed(v)
+    z = (torch.randn(n, v, device=cuda_device, generator=gen) * 3.0).to(dtype)
+    at = torch.randint(0, v, (n, 1), device=cuda_device, generator=gen)
+    z.scatter_(1, at, (torch.rand(n, 1, device=cuda_device, generator=gen) * 200.0 + 30.0).to(dtype))
+    for tau in (1.0, 0.7):
+        for k in (0, 3):
+            r = ops.token_logprobs(z, at[:, 0].contiguous(), k, tau)
+            assert (r.logp <= 0).all() and (r.entropy >= 0).all()
+            # the token stands at least 10 / 0.7 above the others: s is 1 + v e^-10 at most and every further number a few roundings of it
+            x = z.double() / float(np.float32(tau))
+            lse = torch.logsumexp(x, 1)
+            logp = x.gather(1, at)[:, 0] - lse
+            p = (x - lse[:, None]).exp()
+            ent = -(p * (x - lse[:, None])).sum(1)
+            # (the sums' relative error: chains of at most 32 chunks a lane and the joins; with |y| <= 400 for every term but the largest)
+            rel = (128 + 800 * (1 - p.amax(1))) * U
+            assert ((r.logp.double() - logp).abs() <= rel).all()
+            assert ((r.entropy.double() - ent).abs() <= 8 * rel + 512 * U * ent).all()
+            if k:
+                assert (r.top_logp <= 0).all() and torch.equal(r.top_ids[:, 0], at[:, 0]) and torch.equal(r.top_logp[:, 0], r.logp)

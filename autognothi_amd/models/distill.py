@@ -64,11 +64,12 @@ def _rows(t: Optional[Tensor], dims: int) -> Optional[Tensor]:
 
 
 def _back(t: Optional[Tensor], lead) -> Optional[Tensor]:
-    return t if t is None or len(lead) == 1 else t.view(*lead, *t.shape[1:])
+    return t if t is None or len(lead) == 1 else t.view(lead + t.shape[1:])
 
 
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int = 0, temperature: float = 1.0) -> Logprobs:
-    """``ops.token_logprobs`` on logits [..., V] and tokens [...] int64; every output but the ids is differentiable with respect to the logits."""
+    """``ops.token_logprobs`` on logits [..., V] (a single row [V] among them: results without its dimension) and tokens [...] int64; every output
+    but the ids is differentiable with respect to the logits."""
     lead = logits.shape[:-1]
     out = _TokenLogprobs.apply(_rows(logits, 2), _rows(tokens, 1), top_k, temperature)
     return Logprobs(*(_back(t, lead) for t in out))

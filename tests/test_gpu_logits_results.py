@@ -120,6 +120,26 @@ def test_autograd_loss_can_be_edited_in_place(cuda_device, shape):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_row_without_leading_dimensions(cuda_device, dtype):
+    """logits [V]: the numbers of the call with one row, in forward and backward"""
+    from autognothi_amd.models import distill
+    z, tokens, _ = _made(cuda_device, 1, 1234)
+    z = z.to(dtype)
+    got = []
+    for shape in ((1234,), (1, 1234)):
+        x = z.view(shape).clone().requires_grad_(True)
+        r = distill.token_logprobs(x, tokens.view(shape[:-1]), top_k=4, temperature=2.0)
+        assert r.logp.shape == r.entropy.shape == r.lse.shape == shape[:-1] and r.top_ids.shape == r.top_logp.shape == (*shape[:-1], 4)
+        loss, row = distill.loss_topk_distillation(x, r.top_ids, r.top_logp.detach() - 0.25, torch.ones(shape[:-1], device=cuda_device), tail=True)
+        assert loss.shape == () and row.shape == shape[:-1]
+        total = loss + row.sum() + r.logp.sum() + r.entropy.sum() + r.lse.sum() + r.top_logp.sum()
+        got.append([t.detach().reshape(-1) for t in (r.logp, r.entropy, r.lse, r.top_ids, r.top_logp, loss, row, *torch.autograd.grad(total, x))])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert distill.token_logprobs(z[0]).lse.shape == ()
+
+
 # ------------------------------------------------------------------------------------------------ signs
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n,v", [(4000, 40), (4000, 100), (4000, 700), (4000, 5000), (1500, 30522), (600, 70000), (100, 140000)])

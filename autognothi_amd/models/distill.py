@@ -55,12 +55,23 @@ class _TokenLogprobs(torch.autograd.Function):
         return ops.token_logprobs_bwd(logits, fwd, tokens, g_logp, g_entropy, g_lse, g_top), None, None, None
 
 
-def _rows(t: Optional[Tensor], dims: int) -> Optional[Tensor]:
-    """``t`` with its leading dimensions as one (``dims``: 2 for rows, 1 for a number per row); as it is where it has that form (a view would be a
-    node of the autograd graph)"""
-    if t is None or t.dim() == dims:
+def _lead(who: str, logits: Tensor) -> torch.Size:
+    if logits.dim() == 0:
+        raise ValueError(f"{who}: logits must be [..., vocabulary]; got a number")
+    return logits.shape[:-1]
+
+
+def _rows(who: str, name: str, t: Optional[Tensor], lead: torch.Size, dims: int) -> Optional[Tensor]:
+    """``t`` [*lead, any] (``dims`` 2) or [*lead] (1) with its leading dimensions as one; as it is where it has that form already (a view would be a
+    node of the autograd graph).  Other leading dimensions than the logits' are refused: [3, 2] numbers for [2, 3] rows are as many, not the same."""
+    if t is None:
+        return None
+    own = t.shape[:t.dim() - dims + 1]
+    if t.dim() == dims and own.numel() == lead.numel():
         return t
-    return t.reshape(-1, t.shape[-1]) if dims == 2 else t.reshape(-1)
+    if t.dim() < dims - 1 or own != lead:
+        raise ValueError(f"{who}: {name} must be {[*lead, '...'] if dims == 2 else list(lead)}; got {list(t.shape)}")
+    return t.reshape(lead.numel(), t.shape[-1]) if dims == 2 else t.reshape(-1)
 
 
 def _back(t: Optional[Tensor], lead) -> Optional[Tensor]:
@@ -70,8 +81,9 @@ def _back(t: Optional[Tensor], lead) -> Optional[Tensor]:
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top_k: int = 0, temperature: float = 1.0) -> Logprobs:
     """``ops.token_logprobs`` on logits [..., V] (a single row [V] among them: results without its dimension) and tokens [...] int64; every output
     but the ids is differentiable with respect to the logits."""
-    lead = logits.shape[:-1]
-    out = _TokenLogprobs.apply(_rows(logits, 2), _rows(tokens, 1), top_k, temperature)
+    who = "token_logprobs"
+    lead = _lead(who, logits)
+    out = _TokenLogprobs.apply(_rows(who, "logits", logits, lead, 2), _rows(who, "tokens", tokens, lead, 1), top_k, temperature)
     return Logprobs(*(_back(t, lead) for t in out))
 
 
@@ -99,5 +111,8 @@ def loss_topk_distillation(logits: Tensor, teacher_ids: Tensor, teacher_logp: Te
                            tail: bool = False) -> Tuple[Tensor, Tensor]:
     """``ops.topk_distill`` on logits [..., V], teacher_ids / teacher_logp [..., K] and weights [...] -> (loss, row losses [...]), both
     differentiable with respect to the logits (the teacher's record and the weights get no gradient)."""
-    loss, row = _TopkDistill.apply(_rows(logits, 2), _rows(teacher_ids, 2), _rows(teacher_logp, 2), _rows(weights, 1), temperature, tail)
-    return loss, _back(row, logits.shape[:-1])
+    who = "loss_topk_distillation"
+    lead = _lead(who, logits)
+    loss, row = _TopkDistill.apply(_rows(who, "logits", logits, lead, 2), _rows(who, "teacher_ids", teacher_ids, lead, 2),
+                                   _rows(who, "teacher_logp", teacher_logp, lead, 2), _rows(who, "weights", weights, lead, 1), temperature, tail)
+    return loss, _back(row, lead)

@@ -7,6 +7,44 @@ def _int(*shape):
     return torch.zeros(shape, dtype=torch.int64)
 
 
+@pytest.mark.parametrize("logits,tokens", [((2, 3, 11), (3, 2)), ((2, 3, 11), (5,)), ((6, 11), (2, 3)), ((6, 11), (6, 1)), ((6, 11), (5,)), ((11,), (11,)),
+                                           ((1, 11), ())])
+def test_tokens_of_other_leading_dimensions_are_refused(logits, tokens):
+    """[3, 2] tokens for [2, 3, V] logits are as many, but not the same ones"""
+    from autognothi_amd.models import distill
+    with pytest.raises(ValueError, match="token_logprobs: tokens must be"):
+        distill.token_logprobs(torch.zeros(logits), _int(*tokens))
+
+
+@pytest.mark.parametrize("flat", [False, True])
+def test_one_dimension_for_all_rows_reaches_the_operator(flat):
+    from autognothi_amd.models import distill
+    lead = (6,) if flat else (2, 3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        distill.token_logprobs(torch.zeros(2, 3, 11), _int(*lead))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        distill.loss_topk_distillation(torch.zeros(2, 3, 11), _int(*lead, 4), torch.zeros(*lead, 4), torch.zeros(lead))
+
+
+@pytest.mark.parametrize("logits,ids,logp,weights,what", [
+    ((2, 3, 11), (3, 2, 4), (2, 3, 4), None, "teacher_ids"), ((2, 3, 11), (5, 4), (6, 4), None, "teacher_ids"), ((6, 11), (2, 3, 4), (2, 3, 4), None, "teacher_ids"),
+    ((2, 3, 11), (2, 3, 4), (3, 2, 4), None, "teacher_logp"), ((2, 3, 11), (2, 3, 4), (2, 3, 5), None, "teacher_logp"), ((2, 3, 11), (2, 3, 4), (2, 3, 4), (3, 2), "weights"),
+    ((2, 3, 11), (2, 3, 4), (2, 3, 4), (5,), "weights"), ((6, 11), (6, 4), (6, 4), (6, 1), "weights"), ((11,), (2, 4), (2, 4), None, "teacher_ids"),
+    ((11,), (4,), (4,), (2,), "weights"), ((6, 11), (), (6, 4), None, "teacher_ids")])
+def test_a_record_of_other_leading_dimensions_is_refused(logits, ids, logp, weights, what):
+    from autognothi_amd.models import distill
+    with pytest.raises(ValueError, match=f"{what} must be"):
+        distill.loss_topk_distillation(torch.zeros(logits), _int(*ids), torch.zeros(logp), None if weights is None else torch.zeros(weights))
+
+
+def test_a_number_is_no_row_of_logits():
+    from autognothi_amd.models import distill
+    with pytest.raises(ValueError, match="logits must be"):
+        distill.token_logprobs(torch.zeros(()))
+    with pytest.raises(ValueError, match="logits must be"):
+        distill.loss_topk_distillation(torch.zeros(()), _int(4), torch.zeros(4))
+
+
 @pytest.mark.parametrize("lead", [(), (1,), (6,), (2, 3), (0,), (2, 0)])
 def test_leading_dimensions_as_documented_reach_the_operator(lead):
     """[..., V] with any leading dimensions, none among them (an operator on the CPU: the refusal comes from there)"""
@@ -16,6 +54,9 @@ def test_leading_dimensions_as_documented_reach_the_operator(lead):
         distill.token_logprobs(z, _int(*lead), top_k=2)
     with pytest.raises(RuntimeError, match="no CPU fallback") if 0 not in lead else pytest.raises(ValueError, match="no rows"):
         distill.loss_topk_distillation(z, _int(*lead, 4), torch.zeros(*lead, 4), torch.zeros(lead))
+    if 0 not in lead:
+        with pytest.raises(ValueError, match="teacher_ids must be"):
+            distill.loss_topk_distillation(z, _int(*lead, 0), torch.zeros(*lead, 0))
 
 
 def test_results_get_the_leading_dimensions_back(monkeypatch):

@@ -1504,7 +1504,7 @@ template <int TH> dim3 team_grid(int N, int y = 1) { return dim3(TH < 256 ? ceil
 // (The last part has what the rounding up to 64 logits leaves it: at least 4096 - 63 * 64 logits, and at least k.)
 Parts parts_of(int N, int V, int dtype, int k) {
     const int chunks = V / (dtype == AG_BF16 ? 8 : 4);
-    if (N < 1 || N > 128 || chunks < 32768 || k > 32) return {0, 0, nullptr, nullptr};
+    if (N < 1 || N > 128 || chunks < 32768 || V > AG_LOGITS_MAX_V || k < 0 || k > 32 || (dtype != AG_F32 && dtype != AG_BF16)) return {0, 0, nullptr, nullptr};
     const int count = std::min(std::min(64, chunks / 1024), std::min(k ? 256 / k : 64, 512 / N));
     const int length = (ceil_div(V, count) + 63) / 64 * 64;
     return {ceil_div(V, length), length, nullptr, nullptr};
@@ -1632,7 +1632,7 @@ auto gradient_of(int dtype, int tail) {
 
 extern "C" size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int top_k) {
     const Parts p = parts_of(N, V, dtype, top_k);
-    return (size_t)std::max(N, 0) * p.count * (sizeof(float4) + (size_t)std::max(top_k, 0) * sizeof(unsigned long long));
+    return p.count ? (size_t)N * p.count * (sizeof(float4) + (size_t)top_k * sizeof(unsigned long long)) : 0;
 }
 
 static int token_logprobs_entry(const char* who, const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,

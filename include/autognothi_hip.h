@@ -515,7 +515,7 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
  * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
  * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  No ln p is above 0 and no entropy below it.  A row of -inf: lse = ln p = -inf, entropy 0.
  * d_workspace (16-byte aligned, ag_token_logprobs_workspace_bytes; NULL: none): with it a few long rows are shared by several workgroups
- * each; its size is 0 for calls that would not be. */
+ * each; its size is 0 for calls that would not be, refused ones among them. */
 size_t ag_token_logprobs_workspace_bytes(int N, int V, int dtype, int top_k);
 int ag_token_logprobs(const void* d_logits, int64_t ld, int N, int V, int dtype, float temperature, const int64_t* d_tokens, int top_k,
                       float* d_logp, float* d_entropy, float* d_lse, float* d_stats, int64_t* d_top_ids, float* d_top_logp, void* d_workspace,

@@ -1,4 +1,7 @@
-"""CPU: leading dimensions of the autograd forms over wide rows of logits."""
+"""CPU: leading dimensions of the autograd forms over wide rows of logits, and the workspace query for calls that are refused."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -72,3 +75,20 @@ def test_results_get_the_leading_dimensions_back(monkeypatch):
     for lead in ((), (1,), (6,), (2, 3), (2, 1, 3)):
         r = distill.token_logprobs(torch.zeros(*lead, 11), _int(*lead), top_k=2)
         assert r.logp.shape == r.entropy.shape == r.lse.shape == lead and r.top_ids.shape == r.top_logp.shape == (*lead, 2)
+
+
+def test_workspace_of_a_refused_call_is_nothing():
+    """(in a process of its own: a division by zero at a C entry ends it)"""
+    code = """
+from autognothi_amd import _lib as L
+f = L.lib().ag_token_logprobs_workspace_bytes
+assert f(1, 200000, 0, 4) > 0
+for n in (-5, 0, 1, 100, 2 ** 31 - 1):
+    for v in (-2 ** 31, -1, 0, 1, 200000, L.AG_LOGITS_MAX_V + 1, 2 ** 31 - 1):
+        for k in (-2 ** 31, -1000, -257, -2, -1, 0, 1, 129, 2 ** 31 - 1):
+            for dtype in (L.AG_F32, L.AG_BF16, 2, -1):
+                if n < 0 or not 1 <= v <= L.AG_LOGITS_MAX_V or not 0 <= k <= min(v, L.AG_LOGITS_MAX_TOP) or dtype not in (L.AG_F32, L.AG_BF16):
+                    assert f(n, v, dtype, k) == 0, (n, v, dtype, k)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])

@@ -8,11 +8,13 @@ HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-variable"
 # no packed fp32 instructions (the scalar forms have the same bits; the host pass does not know the feature and says so)
 FLAGS="$FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops"
+# an object is compiled again when its source, a header or this script (its flags) is newer
+stale() { [ ! -f "$2" ] || [ "$1" -nt "$2" ] || [ common.h -nt "$2" ] || [ ../../include/autognothi_hip.h -nt "$2" ] || [ build.sh -nt "$2" ]; }
 OBJS=()
 PIDS=()
 for src in gemm.hip gemm_tn.hip gemm_big.hip side_mlp.hip probe.hip attention.hip cls_last.hip sampler.hip elementwise.hip shapley.hip logits.hip train.hip train_fused.hip encoder.cpp capi.cpp; do
   obj="$OUT/${src%.*}.o"
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ common.h -nt "$obj" ] || [ ../../include/autognothi_hip.h -nt "$obj" ]; then
+  if stale "$src" "$obj"; then
     echo "hipcc $src"
     rm -f "$obj"          # a failed compile must not leave a stale object behind
     $HIPCC $FLAGS -x hip -c "$src" -o "$obj" &
@@ -24,7 +26,7 @@ done
 # the parity tests check the shipped stream kernel bit for bit against them (tests/test_gpu_gemm_ring.py loads this file beside
 # the shipped one); nothing under autognothi_amd/ loads it
 REFOBJ="$OUT/gemm_big_ref.o"
-if [ ! -f "$REFOBJ" ] || [ gemm_big.hip -nt "$REFOBJ" ] || [ common.h -nt "$REFOBJ" ] || [ ../../include/autognothi_hip.h -nt "$REFOBJ" ]; then
+if stale gemm_big.hip "$REFOBJ"; then
   echo "hipcc gemm_big.hip -DAG_REF_KERNELS"
   rm -f "$REFOBJ"
   $HIPCC $FLAGS -DAG_REF_KERNELS -x hip -c gemm_big.hip -o "$REFOBJ" &

@@ -5,6 +5,12 @@ import numpy as np
 U = 2.0 ** -24        # half a step of fp32, relative
 
 
+def chain(v):
+    """additions one after another in a lane's sums over v logits: a row of more than 2048 16-byte pieces (of 4 logits at least) belongs to 256 threads
+    or more and a lane adds a piece's own sum; fewer pieces are at most 32 for each of 64 lanes (of which the shortest rows have v / 64 logits)"""
+    return min(v / 64, max(32, v / 1024))
+
+
 def order_key(z):
     """descending order of a row: NaN first, then by value (-0 = +0)"""
     return np.where(np.isnan(z), np.inf, z), np.isnan(z)
@@ -42,8 +48,8 @@ def token_logprobs(z, tokens, k, tau):
     p = np.exp(lp)
     ent = -_xlogy(p, lp).sum(axis=1)
     n, v = z.shape
-    # a sum of v positive terms in chains of v / 64 and a tree, terms of relative error (4 + 3 |d|) U each, |d| e^-|d| <= 0.37
-    sum_u = (v / 64 + 48) * U
+    # a sum of v positive terms in chains and a tree, terms of relative error (4 + 3 |d|) U each, |d| e^-|d| <= 0.37
+    sum_u = (chain(v) + 48) * U
     out = {"lse": lse, "entropy": ent, "err_lse": sum_u + 4 * U * (np.abs(lse) + np.abs(m)), "err_entropy": sum_u * (4 + 3 * np.log(max(v, 2)))}
 
     def bound(values):
@@ -86,7 +92,7 @@ def token_logprobs_grad(z, tokens, ids, tau, g_logp=None, g_entropy=None, g_lse=
         mass, size = mass + g.sum(axis=1), size + np.abs(g).sum(axis=1)
     grad = p * ((gl - mass)[:, None] - ge[:, None] * (lp0 + ent[:, None])) + sparse
     k = 0 if ids is None else ids.shape[1]
-    rel = U * (v / 64 + 64 + 2 * k + 8 * np.abs(lp0))
+    rel = U * (chain(v) + 64 + 2 * k + 8 * np.abs(lp0))
     bound = p * (size[:, None] + np.abs(ge)[:, None] * np.abs(lp0)) * rel + 8 * U * np.abs(sparse)
     live = live[:, None]
     return np.where(live, grad / tau, 0.0), np.where(live, bound / tau, 0.0)
@@ -129,7 +135,7 @@ def distill(z, ids, t_logp, tau, tail, w):
     grad = p * (Q + rest)[:, None] - qi - rest[:, None] * share
     # bounds: sums as above; 1 - sum q to (k + 8) U of what is left beside its largest term
     d_rest = (k + 8) * U * (1.0 - np.minimum(q.max(axis=1), 1.0) + 4 * U) * (1 if tail else 0)
-    sum_u = (v / 64 + 64 + 2 * k) * U
+    sum_u = (chain(v) + 64 + 2 * k) * U
     fin = lambda a: np.where(np.isfinite(a), np.abs(a), 0.0)   # noqa: E731
     e_row = sum_u * (np.where(q > 0, q * (1 + np.abs(lq) + fin(ls)) * (1 + 4 * U * fin(ls)), 0.0).sum(axis=1) + np.log(max(v, 2)))
     e_row = e_row + (d_rest + sum_u * rest) * (2 + fin(np.log(np.where(rest > 0, rest, 1.0))) + fin(lp_off))

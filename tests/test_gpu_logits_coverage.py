@@ -1,0 +1,217 @@
+"""GPU: every logit of a row is in its sums, and every row's results are near the definition: bounds that follow the kernels' real chains of
+additions, and rows of -inf in which the one or two finite logits decide everything.
+
+Chains: a lane adds at most max(32, pieces / 512) 16-byte pieces of a row in the log-probabilities and max(32, pieces / 256) in the distillation (the launch
+rules give rows of more than 2048 pieces 256 threads or more, of more than 8192 512 or, for the distillation's loss of many rows, 256), then joins of at
+most 6 + 4 + 6 steps; an exponential, its exponent and the moves of a lane's reference are a few roundings of U = 2^-24 each."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+U = 2.0 ** -24
+INF = float("inf")
+
+
+def _pieces(v, dtype):
+    return v // (4 if dtype == F32 else 8)
+
+
+def _poison(n, v, dtype, dev):
+    """what the next result of this size may find in its memory"""
+    torch.full((n, v), float("nan"), dtype=dtype, device=dev)
+
+
+# ------------------------------------------------------------------------------------------------ one or two finite logits
+def _places(v, dtype, g, lengths=()):
+    """logits of every class of place: both ends at every alignment, the first and last piece of a lane's rounds for every number of threads and
+    of pieces a lane holds, the borders of shared rows' parts, and some anywhere"""
+    e = 4 if dtype == F32 else 8
+    at = set(range(2 * e + 2)) | set(range(v - 2 * e - 2, v)) | set(g.integers(0, v, 48).tolist())
+    for th in (64, 256, 512, 1024):
+        for m in (1, 2, 3, 4, 8, 15, 16, 17, 32, 48, 64, 96):
+            at |= {th * e * m + o for o in (-e - 1, -e, -1, 0, 1, e)}
+    for length in lengths:
+        for m in range(1, v // length + 1):
+            at |= {length * m + o for o in (-1, 0)}
+    at = np.array(sorted(i for i in at if 0 <= i < v))
+    g.shuffle(at)
+    return at
+
+
+# rows, 16-byte pieces of a row: each launch rule of the four entry points on both sides of its bound
+CALLS = [(200, 10), (40, 20), (200, 100), (5000, 30), (40, 300), (1100, 700), (1100, 1500), (600, 600), (1100, 2100), (300, 2100), (300, 5000), (200, 5000), (300, 9000), (20, 17000),
+         (100, 17000), (300, 17000), (2, 40000), (20, 40000), (100, 33000), (300, 33000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,pieces", CALLS)
+def test_every_place_of_a_row_counts(cuda_device, dtype, n, pieces):
+    """a row of -inf with logit a at one place and b at another.  Sums of two terms, all others exact zeros: a few roundings of numbers of size 4"""
+    from autognothi_amd import ops
+    e = 4 if dtype == F32 else 8
+    g = np.random.default_rng(n + pieces)
+    v = pieces * e + 3                                     # (rows of every alignment one after another)
+    # part lengths of rows that several workgroups share (1024 pieces or more each, rounded up to 64 logits)
+    lengths = {(-(-v // c) + 63) // 64 * 64 for c in range(4, 65)} if pieces >= 32768 and n <= 4 else ()
+    places = _places(v, dtype, g, sorted(lengths)[:12])
+    dev = cuda_device
+    rows = torch.arange(n, device=dev)
+    near = lambda got, want, size=4.0: bool(((got.double() - want).abs() <= 64 * U * size).all())   # noqa: E731
+    for first in range(0, len(places), n):
+        at = torch.from_numpy(np.resize(places[first: first + n], n)).to(dev)
+        other = torch.from_numpy((np.resize(places[first: first + n], n) + g.integers(1, v, n)) % v).to(dev)
+        a, b = (torch.from_numpy(g.integers(-64, 65, n) / 64.0).to(dev) for _ in range(2))       # (exact in bf16)
+        z = torch.full((n, v), -INF, dtype=dtype, device=dev)
+        z[rows, at] = a.to(dtype)
+        # one finite logit
+        r = ops.token_logprobs(z, at, 2)
+        assert near(r.lse, a) and near(r.entropy, 0.0) and near(r.logp, 0.0) and near(r.top_logp[:, 0], 0.0)
+        assert torch.equal(r.top_ids[:, 0], at) and torch.equal(r.top_ids[:, 1], (at == 0).long()) and (r.top_logp[:, 1] == -INF).all()
+        # two
+        z[rows, other] = b.to(dtype)
+        lse = torch.logaddexp(a, b)
+        pa, pb = (a - lse).exp(), (b - lse).exp()
+        entropy = -(pa * (a - lse) + pb * (b - lse))
+        both = torch.stack([at, other], 1)
+        larger = ((a > b) | ((a == b) & (at < other)))
+        for k in (0, 2):
+            r = ops.token_logprobs(z, at, k)
+            assert near(r.lse, lse) and near(r.logp, a - lse) and near(r.entropy, entropy)
+            if k:
+                assert torch.equal(r.top_ids, torch.where(larger[:, None], both, both.flip(1)))
+        _poison(n, v, dtype, dev)
+        half = 2.0 ** -8 if dtype == BF16 else 0.0
+        d = ops.token_logprobs_bwd(z, r, at, d_entropy=torch.ones(n, device=dev), d_lse=torch.ones(n, device=dev))
+        for i, p, x in ((at, pa, a), (other, pb, b)):
+            want = p * (1.0 - (x - lse + entropy))
+            assert bool(((d[rows, i].double() - want).abs() <= 64 * U * 4 + half * (want.abs() + 1e-4)).all())
+            d[rows, i] = 0
+        assert not d.any() and torch.isfinite(d).all()
+        # the teacher lists `other` alone: L = q (ln q - ln p_b) [+ (1 - q) (ln (1 - q) - ln p_a)]
+        w = torch.ones(n, device=dev)
+        for tail, q in ((False, 1.0), (True, 0.25)):
+            lp = torch.full((n, 1), math.log(q), device=dev)
+            want = q * (math.log(q) - (b - lse)) + ((1 - q) * (math.log(1 - q) - (a - lse)) if tail else 0.0)
+            _poison(n, v, dtype, dev)
+            one = ops.topk_distill(z, other[:, None], lp, w, tail=tail)
+            apart = ops.topk_distill(z, other[:, None], lp, w, tail=tail, want_grad=False)
+            _poison(n, v, dtype, dev)
+            d2 = ops.topk_distill_bwd(z, apart, other[:, None], lp, w, tail=tail)
+            for got in (one.row_loss, apart.row_loss):
+                assert near(got, want)
+            for d in (one.dlogits, d2):
+                for i, grad in ((at, pa - (1 - q if tail else 0.0)), (other, pb - q)):
+                    assert bool(((d[rows, i].double() - grad).abs() <= 64 * U * 4 + half * (grad.abs() + 1e-4)).all())
+                    d[rows, i] = 0
+                assert not d.any() and torch.isfinite(d).all()
+
+
+# ------------------------------------------------------------------------------------------------ every row
+def _per_row(z, tau, f):
+    """f(float64 x = z / tau of some rows, those rows), over all rows"""
+    step = max(1, (1 << 27) // z.shape[1])
+    for i in range(0, z.shape[0], step):
+        f(z[i: i + step].double() / tau, slice(i, min(i + step, z.shape[0])))
+
+
+ROWS = [(5000, 10, F32), (4500, 40, BF16), (1100, 300, F32), (1100, 1500, BF16), (600, 600, F32), (1100, 3000, F32), (300, 9000, BF16), (300, 20000, F32), (64, 17000, BF16), (100, 33000, F32),
+        (400, 33000, F32), (2, 60000, BF16)]
+
+
+@pytest.mark.parametrize("n,pieces,dtype", ROWS)
+def test_every_row_is_near_the_definition(cuda_device, n, pieces, dtype):
+    """the bounds: with d = x - lse, A = E|d|, B = E d^2 under p, m the row's largest x; L additions in a chain
+         s: (L + 64 + 4 (A + 3)) U relative;   lse: s and 4 roundings of |lse|, |m|, ln s;   ln p: s and 6 of 1 + |ln p| + ln V
+         H: s (A + 4), the chain of p y once more (A + 3), 4 (B + 6 A + 9) U of its terms, 8 (A + 3 + ln V) U of the last steps
+    gradients: the sums' errors twice, H's times its factor, 8 roundings of every term and of the exponent of p; a bf16 one half a step more"""
+    from autognothi_amd import ops
+    v = pieces * (4 if dtype == F32 else 8) + 3
+    dev = cuda_device
+    gen = torch.Generator(dev).manual_seed(n + pieces)
+    tau = 1.5
+    z = (torch.randn(n, v + 2, device=dev, generator=gen) * 3.0).to(dtype)[:, :v]
+    tok = torch.randint(0, v, (n,), device=dev, generator=gen)
+    k = min(v, 24)
+    r = ops.token_logprobs(z, tok, k, tau)
+    gl, ge = torch.randn(n, device=dev, generator=gen), torch.randn(n, device=dev, generator=gen)
+    dz = ops.token_logprobs_bwd(z, r, tok, gl, ge)
+    ids = torch.rand(n, v, device=dev, generator=gen).topk(k, dim=1).indices if n * v < 1 << 26 else torch.randint(0, v // k, (n, k), device=dev, generator=gen) + torch.arange(k, device=dev) * (v // k)
+    lp = torch.log_softmax(torch.randn(n, k, device=dev, generator=gen) * 2, 1) + math.log(0.8)
+    w = torch.rand(n, device=dev, generator=gen) + 0.1
+    got = {t: (ops.topk_distill(z, ids, lp, w, tau, t), ops.topk_distill(z, ids, lp, w, tau, t, want_grad=False)) for t in (False, True)}
+    apart = {t: ops.topk_distill_bwd(z, got[t][1], ids, lp, w, tau, t) for t in got}
+    ln_v = math.log(v)
+    half = 2.0 ** -8 if dtype == BF16 else 0.0
+
+    def near(a, want, bound, what):
+        off = (a.double() - want).abs() - bound
+        assert bool((off <= 0).all()), f"{what}: {int((off > 0).sum())} of {off.numel()} off, by {float(off.max()):.3g} more than allowed"
+
+    def check(x, sl):
+        lse = torch.logsumexp(x, 1, keepdim=True)
+        d = x - lse
+        p = d.exp()
+        ent = -(p * d).sum(1, keepdim=True)
+        A, B, m = ent, (p * d * d).sum(1, keepdim=True), x.amax(1, keepdim=True)
+        chain = max(32, pieces // 512)
+        s_err = (chain + 64 + 4 * (A + 3)) * U
+        near(r.lse[sl], lse[:, 0], (s_err + 4 * U * (lse.abs() + m.abs() + lse - m))[:, 0], "lse")
+        h_err = s_err * (A + 4) + (chain + 64) * U * (A + 3) + 4 * U * (B + 6 * A + 9) + 8 * U * (A + 3 + ln_v)
+        near(r.entropy[sl], ent[:, 0], h_err[:, 0], "entropy")
+        given = d.gather(1, tok[sl, None])
+        near(r.logp[sl], given[:, 0], (s_err + 6 * U * (1 + given.abs() + ln_v))[:, 0], "logp")
+        top = d.gather(1, r.top_ids[sl])
+        near(r.top_logp[sl], top, s_err + 6 * U * (1 + top.abs() + ln_v), "top_logp")
+        # (the k-th alternative is not below any logit that is not one)
+        rest = d.scatter(1, r.top_ids[sl], -INF).amax(1)
+        assert (top[:, 1:] <= top[:, :-1]).all() and (rest <= top[:, -1]).all()
+        g, h = gl[sl, None].double(), ge[sl, None].double()
+        want = p * (-g - h * (d + ent)) / tau
+        size = p * (g.abs() + h.abs() * (1 + ent + d.abs())) / tau
+        want.scatter_add_(1, tok[sl, None], g / tau)
+        bound = size * (2 * s_err + (64 + 8 * d.abs() + 8 * ln_v) * U) + p * h.abs() * h_err / tau + 8 * U * want.abs() + 2.0 ** -126
+        bound.scatter_add_(1, tok[sl, None], 8 * U * g.abs() / tau)
+        near(dz[sl], want, bound + half * (want.abs() + bound), "dlogits")
+        del want, size, bound
+        # distillation
+        chain = max(32, pieces // 256)
+        s_err = (chain + 64 + 4 * (A + 3) + 2 * k) * U
+        t = lp[sl].double()
+        ls = d.gather(1, ids[sl])
+        for tail in (False, True):
+            lq = t if tail else t - torch.logsumexp(t, 1, keepdim=True)
+            q = lq.exp()
+            left = 1.0 - q.sum(1, keepdim=True) if tail else torch.zeros_like(lse)
+            row = (q * (lq - ls)).sum(1, keepdim=True)
+            off = d.scatter(1, ids[sl], -INF)
+            l_off = torch.logsumexp(off, 1, keepdim=True)
+            size = (q * (1 + lq.abs() + ls.abs())).sum(1, keepdim=True)
+            err = s_err + (2 * k + 64) * U * size
+            left_err = 0.0
+            if tail:
+                row = row + left * (left.log() - l_off)
+                left_err = (k + 8) * U
+                err = err + left_err * (1 + left.log().abs() + l_off.abs()) + left * (2 * s_err + 8 * U * (left.log().abs() + l_off.abs()))
+            one, only = got[tail]
+            for a in (one, only):
+                near(a.row_loss[sl], (tau * tau * row)[:, 0], (tau * tau * (err + 4 * U * row.abs()))[:, 0], f"row loss, tail {tail}")
+            share = (off - l_off).exp() if tail else torch.zeros_like(p)
+            grad = p * (q.sum(1, keepdim=True) + left) - left * share
+            bound = (p * (1 + left) + left * share) * (2 * s_err + 16 * U * (1 + d.abs())) + left_err * (p + share)
+            grad.scatter_add_(1, ids[sl], -q)
+            bound.scatter_add_(1, ids[sl], q * U * (2 * k + 32 + 4 * lq.abs()))
+            scale = tau * w[sl, None].double()
+            grad, bound = grad * scale, bound * scale + 2.0 ** -126
+            for a in (one.dlogits[sl], apart[tail][sl]):
+                near(a, grad, bound + half * (grad.abs() + bound), f"gradient, tail {tail}")
+
+    _per_row(z, tau, check)
+    for tail, pair in got.items():
+        for a in pair:
+            total = (a.row_loss.double() * w.double()).sum()
+            assert abs(float(a.loss.double() - total)) <= 2.0 ** -23 * abs(float(total))

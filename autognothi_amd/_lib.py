@@ -36,6 +36,7 @@ AG_EPI_BIAS, AG_EPI_BIAS_GELU, AG_EPI_BIAS_RESID, AG_EPI_BIAS_F32, AG_EPI_BIAS_T
 AG_EX_STORE, AG_EX_GELU_DUAL, AG_EX_GELU_BWD, AG_EX_SLABS = 0, 1, 2, 3
 AG_MT_STATE_BYTES = 2560
 AG_LOGITS_MAX_V, AG_LOGITS_MAX_TOP = 524288, 128
+AG_LOGITS_SHARED_ROWS, AG_LOGITS_SHARED_PIECES, AG_LOGITS_APART_ROWS, AG_LOGITS_HELD_PIECES = 128, 32768, 32, 16384
 
 vp, i32, i64, u32, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_float, C.c_size_t
 

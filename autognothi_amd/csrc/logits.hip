@@ -1504,7 +1504,7 @@ template <int TH> dim3 team_grid(int N, int y = 1) { return dim3(TH < 256 ? ceil
 // (The last part has what the rounding up to 64 logits leaves it: at least 4096 - 63 * 64 logits, and at least k.)
 Parts parts_of(int N, int V, int dtype, int k) {
     const int chunks = V / (dtype == AG_BF16 ? 8 : 4);
-    if (N < 1 || N > 128 || chunks < 32768 || V > AG_LOGITS_MAX_V || k < 0 || k > 32 || (dtype != AG_F32 && dtype != AG_BF16)) return {0, 0, nullptr, nullptr};
+    if (N < 1 || N > AG_LOGITS_SHARED_ROWS || chunks < AG_LOGITS_SHARED_PIECES || V > AG_LOGITS_MAX_V || k < 0 || k > 32 || (dtype != AG_F32 && dtype != AG_BF16)) return {0, 0, nullptr, nullptr};
     const int count = std::min(std::min(64, chunks / 1024), std::min(k ? 256 / k : 64, 512 / N));
     const int length = (ceil_div(V, count) + 63) / 64 * 64;
     return {ceil_div(V, length), length, nullptr, nullptr};
@@ -1695,7 +1695,7 @@ extern "C" int ag_topk_distill(const void* d_logits, int64_t ld, int N, int V, i
     hipStream_t s = (hipStream_t)stream;
     const Distill p = {d_teacher_ids, d_teacher_logp, teacher_dtype, K, d_weights, (float)(1.0 / N)};
     // few rows too long for a workgroup's registers: the loss, then the gradient by several workgroups a row (one row of 262144 fp32: 45 -> 32 us)
-    const bool apart = d_dlogits && d_stats && N <= 32 && V / (dtype == AG_BF16 ? 8 : 4) > 16 * 1024, grad = d_dlogits && !apart;
+    const bool apart = d_dlogits && d_stats && N <= AG_LOGITS_APART_ROWS && V / (dtype == AG_BF16 ? 8 : 4) > AG_LOGITS_HELD_PIECES, grad = d_dlogits && !apart;
     const auto bf = tail ? (grad ? distill<bf16_t, true, true> : distill<bf16_t, true, false>)
                          : (grad ? distill<bf16_t, false, true> : distill<bf16_t, false, false>);
     const auto f = tail ? (grad ? distill<float, true, true> : distill<float, true, false>)

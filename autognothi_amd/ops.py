@@ -788,6 +788,11 @@ def _logit_rows(who: str, logits: Tensor) -> Tuple[Tensor, int, int, int, int]:
     return logits, n, v, logits.stride(0), dtype
 
 
+def _pieces(v: int, dtype: int) -> int:
+    """whole 16-byte pieces of a row"""
+    return v // (8 if dtype == BF16 else 4)
+
+
 def _row_arg(who: str, name: str, t: Optional[Tensor], shape: Tuple[int, ...], dtype: torch.dtype, device) -> Optional[Tensor]:
     """a small per-row argument: checked, contiguous"""
     if t is None:
@@ -831,7 +836,8 @@ def _token_logprobs(logits: Tensor, tokens: Optional[Tensor], top_k: int, temper
     top = stats.new_empty(n, top_k) if top_k else None
     at = stats.data_ptr()
     with L.on(dev):
-        need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if n <= 128 else 0
+        shared = n <= L.AG_LOGITS_SHARED_ROWS and _pieces(v, dtype) >= L.AG_LOGITS_SHARED_PIECES
+        need = L.lib().ag_token_logprobs_workspace_bytes(n, v, dtype, top_k) if shared else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         L.check(L.lib().ag_token_logprobs_saved(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(tokens), top_k, L.ptr(logp), L.ptr(entropy), L.ptr(lse),
                                                 at + 12 * n, at + 4 * n, L.ptr(ids), L.ptr(top), L.ptr(ws), need, L.stream()))
@@ -899,7 +905,8 @@ def _topk_distill(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, wei
     ids, tlp, tdt, k, w = _teacher_args(who, n, teacher_ids, teacher_logp, weights, dev)
     L.require_gpu(logits)
     row, loss = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(loss_shape, dtype=torch.float32, device=dev)
-    stats = None if want_grad and (n > 32 or v <= 65536) else torch.empty(n, 4, dtype=torch.float32, device=dev)   # (few long rows are done in two steps)
+    two_steps = n <= L.AG_LOGITS_APART_ROWS and _pieces(v, dtype) > L.AG_LOGITS_HELD_PIECES
+    stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if two_steps or not want_grad else None
     out = torch.empty(n, v, dtype=logits.dtype, device=dev) if want_grad else None
     with L.on(dev):
         L.check(L.lib().ag_topk_distill(L.ptr(logits), ld, n, v, dtype, temperature, L.ptr(ids), L.ptr(tlp), tdt, k, L.ptr(w), 1 if tail else 0,

@@ -511,6 +511,12 @@ int ag_masked_attention_bwd_bf16(const void* d_qkv, const uint32_t* d_mask_bits,
  * ---------------------------------------------------------------------------------------------- */
 #define AG_LOGITS_MAX_V 524288
 #define AG_LOGITS_MAX_TOP 128
+/* ag_token_logprobs shares rows of at least this many whole 16-byte pieces, in calls of at most this many rows (others need no workspace); ag_topk_distill
+ * takes two steps (and for them d_stats) for rows of more pieces than a workgroup's registers hold, in calls of at most this many rows */
+#define AG_LOGITS_SHARED_ROWS 128
+#define AG_LOGITS_SHARED_PIECES 32768
+#define AG_LOGITS_APART_ROWS 32
+#define AG_LOGITS_HELD_PIECES 16384
 /* d_lse [N] = ln sum exp x;  d_entropy [N] = -sum p ln p;  d_logp [N] = ln p of d_tokens[n] (NULL: not asked for; a token < 0 is ignored: 0;
  * >= V: NaN);  d_top_ids / d_top_logp [N, top_k] = the top_k largest logits in descending order, ties by the lower index (-0 = +0, NaN above
  * all), and their ln p;  d_stats [N, 2]: what ag_token_logprobs_bwd reads.  No ln p is above 0 and no entropy below it.  A row of -inf: lse = ln p = -inf, entropy 0.

@@ -1,4 +1,7 @@
-"""CPU: leading dimensions of the autograd forms over wide rows of logits, and the workspace query for calls that are refused."""
+"""CPU: leading dimensions of the autograd forms over wide rows of logits, the workspace query for calls that are refused, and the sizes at which a
+call takes a workspace: the header's on both sides."""
+import os
+import re
 import subprocess
 import sys
 
@@ -92,3 +95,23 @@ for n in (-5, 0, 1, 100, 2 ** 31 - 1):
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+
+
+def test_sizes_of_the_header_and_of_the_binding_agree():
+    from autognothi_amd import _lib as L
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "autognothi_hip.h")
+    found = dict(re.findall(r"^#define (AG_LOGITS_\w+) (\d+)$", open(header).read(), flags=re.M))
+    assert len(found) == 6
+    for name, value in found.items():
+        assert getattr(L, name) == int(value), name
+
+
+def test_no_workspace_below_the_sizes_at_which_it_is_asked_for():
+    from autognothi_amd import _lib as L, ops
+    f = L.lib().ag_token_logprobs_workspace_bytes
+    for dtype, e in ((L.AG_F32, 4), (L.AG_BF16, 8)):
+        least = L.AG_LOGITS_SHARED_PIECES * e
+        for k in (0, 1, 32):
+            assert f(1, least, dtype, k) > 0 and f(L.AG_LOGITS_SHARED_ROWS, least, dtype, k) > 0
+            assert f(1, least - 1, dtype, k) == 0 and f(L.AG_LOGITS_SHARED_ROWS + 1, least, dtype, k) == 0
+        assert ops._pieces(least, dtype) == L.AG_LOGITS_SHARED_PIECES == ops._pieces(least - 1, dtype) + 1

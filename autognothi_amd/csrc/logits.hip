@@ -273,7 +273,10 @@ __device__ __forceinline__ unsigned long long order_key(float x, int i) {
 // rounds of LG_SLOTS).  Each wave finds the j-th largest of its lanes' maxima, j = ceil(k / waves); the least of them over the waves is a
 // bound that at least k logits reach, and few others: the chunks of the slots that reach it (about two per alternative asked for) are read
 // again, their logits at or above the bound are the candidates, and every candidate's place is the number of candidates that beat it.
-// Rows with more candidates than fit (many equal logits) or a NaN take a radix selection over the whole row.
+// Rows with more candidates than fit and rows with a NaN take a radix selection over the whole row, in five more passes that load single logits.
+// The bound counts pieces, so that is not only rows of many equal logits: where the large logits lie next to each other (a descending row, a band of
+// admissible tokens in a row of -inf) up to E k of them reach it, and in a row of fewer than k finite pieces everything does.  8192 x 131072 bf16, k 64:
+// random 0.42 ms, descending, a band of 200 tokens or all equal 6.4-7.0; 4096 x 30522 fp32 0.10, descending 0.37, a band 0.66; 8192 x 8000 bf16 0.04 / 0.53.
 constexpr int LG_SLOTS = 16;
 
 template <int TH> struct TopLds {
@@ -664,7 +667,8 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
 }
 
 // Rows of up to 64 (W = 16 lanes a row) or 2048 logits (W = 64; where a list is long for the row's slots): the whole row lives in registers, the
-// maximum is found first.  64000 x 10 fp32 with 3 alternatives 7.8 us, 262144 x 64 123 us: bound by the work per row, not by its bytes.
+// maximum is found first.  64000 x 10 fp32 with 3 alternatives 7.8 us, 262144 x 64 129 us: bound by the ranking, which with 16 lanes compares each of
+// the row's logits with all of them whatever k is (without alternatives 64000 x 10 takes 4.8 us, of which 0.8 are its bytes).
 template <typename T, int W> struct Small;
 template <typename T> struct Small<T, 16> {   // element j of a lane: lane + 16 j
     static constexpr int NE = 4;
@@ -1054,7 +1058,8 @@ template <int W> struct List {
 struct GradOf { float m_off, a, m, on; };
 
 // The gradients of the listed tokens (W lanes, slots lane + W i; gx: their logits' bits; bit i of `first`: this lane's i-th slot is known to be
-// the first that names its token; mine(i): logit i is this workgroup's).  Where a token may be listed more than once its masses are added up.
+// the first that names its token; mine(i): logit i is this workgroup's).  Where a token may be listed more than once its masses are added up: for the
+// gradient apart, which knows nothing of the list (`first` 0), always; 131072 x 300 fp32 with lists of 50 takes 156 us, of 128 429, without one 68.
 template <typename T, int W, typename F>
 __device__ __forceinline__ void listed_gradients(const Row<T>& row, const uint32_t* gx, int K, uint32_t first, const GradOf& s, float g, float c,
                                                  const ListLds& l, T* d, F mine) {
@@ -1195,7 +1200,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 // the next round's or the next row's chunk as soon as the chunk is done with, so that memory is busy through all of it.
 // The list is the first wave's: it works on it while the row arrives, marks the listed tokens for the sums of all waves, adds their own part,
 // and writes the loss and the listed tokens' gradients.  MULTI: rows of several rounds.
-// Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 885 us (4.9 TB/s without what the cache gives the second read;
+// Bound by memory, reads and writes mixed: 8192 x 131072 bf16 with a list of 100 in 882 us (4.9 TB/s without what the cache gives the second read;
 // a copy reaches 4.8), 24576 x 1000 fp32 with 25 in 41 us; the loss alone, 2048 x 65537 bf16 with 50, in 43 us (5.4 TB/s).  Without the prefetch
 // in place 8192 x 131072 took 1310 us; 16 rows of 30522 fp32 take 11.2 us, the chain list, sums, join, gradient.
 template <typename T, int TH, int NC, bool MULTI, bool TAIL, bool GRAD, Past PAST = PAST_NONE>
@@ -1499,8 +1504,9 @@ template <int TH> dim3 team_grid(int N, int y = 1) { return dim3(TH < 256 ? ceil
 // How many workgroups share a row: up to 128 rows of 32768 chunks and more, as many as the join takes (64 sums, 256 keys), as give each CU two
 // and leave each 1024 chunks (256 threads, four rounds).  Kernels alone, N x V fp32, k alternatives, shared / one workgroup a row: 1 x 131072,
 // k 0: 8.5 / 13.0 us, k 16: 13.8 / 20.2; 1 x 524288, k 4: 13.6 / 50.5; 128 x 131072, k 16: 20.9 / 23.6.  Not for more than 32 alternatives,
-// which leave the join few parts (1 x 131072, k 64: 20.9 / 22.0, k 128: 29.7 / 22.5) nor for shorter rows (1 x 65536, k 16: 14.3 / 14.3): the
-// second launch and the workspace cost the host 5 us.
+// which leave the join of 256 keys few parts (1 x 131072, k 64: 20.9 / 22.0, k 128: 29.7 / 22.5; longer rows were not measured so: there one workgroup
+// is 50 us of a call of 1 x 524288 with k 33 to 64, where k 32, shared, is 28), nor for shorter rows (1 x 65536, k 16: 14.3 / 14.3): the second launch and
+// the workspace cost the host 5 us.
 // (The last part has what the rounding up to 64 logits leaves it: at least 4096 - 63 * 64 logits, and at least k.)
 Parts parts_of(int N, int V, int dtype, int k) {
     const int chunks = V / (dtype == AG_BF16 ? 8 : 4);
@@ -1511,7 +1517,7 @@ Parts parts_of(int N, int V, int dtype, int k) {
 }
 
 // Threads of a row, by its chunks and the rows a CU gets (N rows of V logits, k alternatives, both sides of each bound):
-//   V <= 64: 16 lanes                        262144 x 64 fp32, k 3: 123 us, 64 lanes 282
+//   V <= 64: 16 lanes                        262144 x 64 fp32, k 3: 129 us, 64 lanes 282
 //   up to 2048 chunks: 64 lanes              16384 x 6000 fp32, k 20: 78 us, 256 threads 90; x 8192: 109 / 104 (bf16 x 16384: 111 / 118)
 //       four rows a CU or fewer: up to 512   512 x 4096 bf16, k 50: 11.0 / 9.7 us; 64 x 16384: 17.1 / 10.5; 1024 x 2080: 10.1 / 11.4
 //   up to 8192: 256 threads                  8192 x 32768 bf16, k 20: 103 us, 512 threads 132; 2048 x 65536 fp32, k 100: 112 / 107
@@ -1563,9 +1569,11 @@ int logprobs_bwd(const void* d_logits, int64_t ld, int N, int V, float temperatu
 // Threads of a row and chunks of a thread: the fewest threads whose registers hold the row.  With the gradient, 16384 rows fp32, list of 50,
 // the choice against its neighbour: V 1000: (64, 4) 43.6 us, (64, 8) 50.0; 2040: (64, 8) 80.8, (256, 8) 118.6; 2400: (64, 16) 90, (256, 8) 118;
 // 4000: 141 / 143; 8160: (256, 8) 248, (256, 16) 254; 11184 x 12000: (256, 16) 248, (512, 16) 258; 5592 x 24000: (512, 16) 233, (1024, 16) 274;
-// 2048 x 65520: one round of (1024, 16) 245, rounds of (256, 8) 293; past the cache two rounds of (512, 16) are better, the second read being the
-// cache's and two workgroups a CU taking turns: 5119 x 100001 bf16 530 -> 498, 8190 x 131072 963 -> 916, but 2559 x 200001 509 -> 533.  Four rows a CU or fewer are a matter of latency: 512 x 2040: (64, 8) 11.7,
-// (256, 8) 10.6; 64 x 16360: (256, 16) 13.8, (512, 16) 12.0.
+// 2048 x 65520: one round of (1024, 16) 245, rounds of (256, 8) 293; past the cache two rounds of (512, 16) instead, the second read being the cache's and
+// two workgroups a CU taking turns.  bf16 rows of 72001 / 96001 / 130401, list of 64 + rest, two rounds / one: 140 MB 74 / 77, 63 / 77, 65 / 89 us; 300 MB
+// 158 / 166, 143 / 167, 131 / 159; 500 MB 259 / 250, 239 / 252, 237 / 250; 1 GB 498 / 482, 456 / 463, 458 / 463; 2 GB 973 / 926, 897 / 889, 912 / 895, but
+// 8192 x 131072 (2.1 GB, aligned rows) 882 / 918.  Four rows a CU or fewer are a matter of latency: 512 x 2040: (64, 8) 11.7, (256, 8) 10.6; 64 x 16360:
+// (256, 16) 13.8, (512, 16) 12.0.
 // The loss alone reads each chunk once, whatever the rounds: 8388 x 4000: (64, 4) 32.3, (256, 4) 43.6; 2796 x 12000: 27.5 / 29.7; 2048 x 16384:
 // 29.1 / 27.9; 512 x 4000: 10.7 / 9.1; one row a CU or fewer, 64 x 64000: (256, 4) 20.1, (1024, 8) 13.0.
 template <typename T, bool TAIL, bool GRAD>

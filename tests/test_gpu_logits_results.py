@@ -48,6 +48,25 @@ def test_stats_hold_what_the_results_do(cuda_device, n, v):
     assert none.logp is None and torch.equal(none.stats[1:], r.stats[1:])
 
 
+@pytest.mark.parametrize("n,v", SIZES)
+def test_c_entry_with_a_saved_entropy_writes_its_rows_alone(cuda_device, n, v):
+    """the results of ag_token_logprobs, the entropy twice, and nothing behind any of them"""
+    from autognothi_amd import _lib as L, ops
+    z, tokens, g = _made(cuda_device, n, v)
+    k = 3
+    r = ops.token_logprobs(z, tokens, k)
+    logp, entropy, lse, saved = (torch.full((n + 1,), 7.0, device=cuda_device) for _ in range(4))
+    stats, top = torch.full((2 * n + 1,), 7.0, device=cuda_device), torch.full((n * k + 1,), 7.0, device=cuda_device)
+    ids = torch.full((n * k + 1,), 77, dtype=torch.int64, device=cuda_device)
+    need = L.lib().ag_token_logprobs_workspace_bytes(n, v, L.AG_F32, k)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=cuda_device)
+    L.check(L.lib().ag_token_logprobs_saved(z.data_ptr(), v, n, v, L.AG_F32, 1.0, tokens.data_ptr(), k, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+                                            stats.data_ptr(), saved.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr() if need else None, need, L.stream()))
+    for got, want in ((logp, r.logp), (entropy, r.entropy), (lse, r.lse), (saved, r.entropy), (stats, r.stats[3:].reshape(-1)), (top, r.top_logp.reshape(-1)),
+                      (ids, r.top_ids.reshape(-1))):
+        assert torch.equal(got[:-1], want) and float(got[-1]) in (7.0, 77.0)
+
+
 def _edit(t):
     t.mul_(2.0)
     t += 1.0

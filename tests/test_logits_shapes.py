@@ -115,3 +115,16 @@ def test_no_workspace_below_the_sizes_at_which_it_is_asked_for():
             assert f(1, least, dtype, k) > 0 and f(L.AG_LOGITS_SHARED_ROWS, least, dtype, k) > 0
             assert f(1, least - 1, dtype, k) == 0 and f(L.AG_LOGITS_SHARED_ROWS + 1, least, dtype, k) == 0
         assert ops._pieces(least, dtype) == L.AG_LOGITS_SHARED_PIECES == ops._pieces(least - 1, dtype) + 1
+
+
+def test_c_entry_with_a_saved_entropy_refuses_before_any_launch():
+    from autognothi_amd import _lib as L
+    lib = L.lib()
+    x = 0x1000    # never read: every call below is refused on the host
+
+    def call(n=1, v=8, dtype=0, k=0, z=x, ent=x, stats=x, saved=x, ws=None, have=0):
+        return lib.ag_token_logprobs_saved(z, 8, n, v, dtype, 1.0, None, k, None, ent, x, stats, saved, None, None, ws, have, None)
+
+    for rc in (call(saved=None), call(stats=None), call(ent=None), call(z=None), call(n=-1), call(v=0), call(dtype=2), call(k=2), call(k=9), call(ws=x + 4)):
+        assert rc < 0 and b"ag_token_logprobs_saved" in lib.ag_last_error()
+    assert call(n=0, saved=None) == 0
